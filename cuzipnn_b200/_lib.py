@@ -53,6 +53,28 @@ SIGNATURES = {
 }
 
 
+class Weight(ctypes.Structure):
+    """zn_weight: a 2-D float16 or bfloat16 weight held as a blob."""
+
+    _fields_ = [("blob", _p), ("blob_bytes", _i64), ("rows", _i64), ("cols", _i64), ("chunk_bytes", _i64),
+                ("dtype", _i32)]
+
+
+_w = ctypes.POINTER(Weight)
+_f = ctypes.c_float
+SIGNATURES |= {
+    "zn_linear_temp_bytes": (_sz, [_w, _p, _i64, _i64]),
+    "zn_linear": (_i32, [_w, _p, _i64, _i64, _p, _i32, _p, _i64, _p, _p, _p, _p, _sz, _p]),
+    "zn_linear_grad_temp_bytes": (_sz, [_w, _p, _i64, _i64, _i32, _i32, _i32]),
+    "zn_linear_grad": (_i32, [_w, _p, _i64, _i64, _p, _p, _p, _p, _p, _sz, _p]),
+    "zn_loss_state_bytes": (_sz, [_i64, _i32]),
+    "zn_loss_temp_bytes": (_sz, [_w, _p, _i64, _i64]),
+    "zn_loss": (_i32, [_w, _p, _i64, _i64, _p, _p, _i32, _i64, _f, _i32, _p, _p, _p, _p, _sz, _p]),
+    "zn_loss_grad_temp_bytes": (_sz, [_w, _p, _i64, _i64]),
+    "zn_loss_grad": (_i32, [_w, _p, _i64, _i64, _i32, _f, _i32, _p, _p, _p, _p, _p, _sz, _p]),
+}
+
+
 def _load() -> ctypes.CDLL:
     if not os.path.exists(LIB_PATH):
         raise ImportError(
@@ -87,7 +109,7 @@ def launch_count() -> int:
     return int(lib.zn_launch_count())
 
 
-KERNELS = ("hist", "encode", "scan", "pack", "dscan", "decode", "decode_overflow", "crc")
+KERNELS = ("hist", "encode", "scan", "pack", "dscan", "decode", "decode_overflow", "crc", "gemm", "finish")
 
 
 class KernelTimer:

@@ -1,0 +1,362 @@
+"""Operators on compressed weights: products with a 2-D float16 or bfloat16 weight that stays a blob.
+
+A model whose weights are kept compressed in GPU memory is used through these calls instead of
+decompress_tensor followed by a product: the weight is decoded a piece of rows at a time into a
+bounded scratch buffer (or, for a few tokens, only in the decoder's registers) and is frozen, so
+gradients go to the other operands.  The reference has no counterpart.
+
+Blobs must be on the GPU of the other operands.  A blob that compress_tensor(..., readback_to_cpu=
+False) or upload_blob returned carries its header, and the calls neither read anything back nor
+synchronise, so they can be captured into a CUDA graph; another GPU blob costs one header read per
+call.  Decoding errors are reported by last_decode_status(), as for decompress_tensor (a malformed
+chunk counts as zeros).
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from ._codec import (_CODES, _FIXED, _FLAG_REORDER, _FLAG_STORED, _MAX_NDIM, _REORDER, _check_device, _gpu,
+                     _known_header, _on, _parse_header, _remember, _set_status, _stream, _upload)
+
+_ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+_REDUCTIONS = {"mean": 0, "sum": 1, "none": 2}
+_MAX_TOP = 256
+_MAX_DIM = 1 << 31
+
+
+def upload_blob(blob: torch.Tensor, *, compute_device: torch.device | str | None = None) -> torch.Tensor:
+    """A GPU blob with its header remembered, from a blob on the CPU or the GPU (returned as it is
+    when it is a GPU blob that carries its header already): what a program that loads blobs from
+    storage does once, so that decompressing or multiplying with them reads nothing back."""
+    compute_device = _check_device(compute_device)
+    _check_blob(blob)
+    device = _gpu(blob, compute_device)
+    if blob.device == device and _known_header(blob) is not None:
+        return blob
+    dtype, shape, flags, chunk_bytes, _, n = _read_header(blob)
+    with _on(device):
+        if blob.is_cuda:
+            out = blob.detach().to(device, non_blocking=True).clone(memory_format=torch.contiguous_format)
+        else:
+            src = blob.detach().contiguous()
+            out = _upload(src, device)
+            if src.is_pinned():  # asynchronous, but the caller may reuse the blob once we return
+                torch.cuda.current_stream(device).synchronize()
+    return _remember(out, dtype, shape, flags, chunk_bytes, n)
+
+
+def _check_blob(blob: torch.Tensor) -> None:
+    if blob.dtype != torch.uint8 or blob.dim() != 1:
+        raise ValueError("blob must be a 1-D uint8 tensor")
+
+
+def _read_header(blob: torch.Tensor) -> tuple:
+    """(dtype, shape, flags, chunk_bytes, n_comp, n) of a blob without a record, checked."""
+    if blob.is_cuda and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("a blob without a remembered header cannot be read during stream capture: "
+                           "pass it through upload_blob first")
+    prefix = blob.detach()[: _FIXED.size + 8 * _MAX_NDIM].cpu().contiguous()
+    dtype, shape, flags, chunk_bytes, n_comp, n = _parse_header(prefix.numpy())
+    stored = bool(flags & _FLAG_STORED)
+    if any(d < 0 for d in shape) or math.prod(shape) != n or (not stored and n and chunk_bytes <= 0):
+        raise ValueError("not a cuzipnn blob")
+    if stored and blob.numel() < _FIXED.size + 8 * len(shape) + n * dtype.itemsize:
+        raise ValueError("blob is truncated")
+    return dtype, tuple(shape), flags, chunk_bytes, n_comp, n
+
+
+class _Weight:
+    """A blob as the weight of a product with `x`: its fields checked against `x` (no GPU work), then,
+    by place(), its description for the C calls."""
+
+    __slots__ = ("blob", "rows", "cols", "device", "dtype", "chunk_bytes", "desc")
+
+    def __init__(self, blob: torch.Tensor, x: torch.Tensor, name: str):
+        _check_blob(blob)
+        known = _known_header(blob)
+        if known is not None:
+            dtype, shape, flags, chunk_bytes, _ = known
+        else:
+            dtype, shape, flags, chunk_bytes, _, _ = _read_header(blob)
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise TypeError(f"the blob holds {dtype}: float16 or bfloat16 weights are supported")
+        if x.dtype != dtype:
+            raise TypeError(f"{name} has dtype {x.dtype}, the blob holds {dtype}")
+        if len(shape) != 2 or not all(0 < d < _MAX_DIM for d in shape):
+            raise ValueError(f"the blob holds a tensor of shape {tuple(shape)}, a weight has two nonempty dimensions")
+        stored = bool(flags & _FLAG_STORED)
+        if not stored and (bool(flags & _FLAG_REORDER) != (dtype in _REORDER) or chunk_bytes % 8):
+            raise ValueError("not a cuzipnn blob")
+        self.rows, self.cols = shape
+        if x.dim() < 1 or x.shape[-1] != self.cols:
+            raise ValueError(f"{name} has shape {tuple(x.shape)}, the weight has {self.cols} columns")
+        if x.numel() // self.cols >= _MAX_DIM:
+            raise ValueError(f"{name} has too many rows")
+        self.device, self.dtype = x.device, dtype
+        self.chunk_bytes = 0 if stored else chunk_bytes
+        self.blob = blob.detach()
+
+    def place(self, name: str) -> None:
+        if self.device.type != "cuda":
+            raise ValueError(f"{name} must be a CUDA tensor")
+        if self.blob.device != self.device:
+            raise ValueError(f"the blob is on {self.blob.device}, {name} on {self.device}")
+        b = self.blob
+        if not b.is_contiguous() or b.data_ptr() % 8:
+            with _on(self.device):
+                self.blob = b = b.clone(memory_format=torch.contiguous_format)
+        self.desc = _lib.Weight(b.data_ptr(), b.numel(), self.rows, self.cols, self.chunk_bytes, _CODES[self.dtype])
+
+    def call(self, name: str, query: tuple, args: tuple, status: torch.Tensor) -> None:
+        """Run entry point `name` on the device's current stream: scratch from <name>_temp_bytes
+        (with the `query` arguments), then (weight, *args, status, scratch, stream)."""
+        w = ctypes.byref(self.desc)
+        nbytes = int(getattr(_lib.lib, name + "_temp_bytes")(w, *query))
+        temp = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=self.device)
+        _lib.check(getattr(_lib.lib, name)(w, *args, status.data_ptr(), temp.data_ptr(), nbytes,
+                                           _stream(self.device)), name)
+
+
+def _rows(t: torch.Tensor, cols: int) -> tuple[torch.Tensor, int]:
+    """`t` as rows of `cols` adjacent elements, and the pitch between them (a copy if it must be)."""
+    t = t.detach().reshape(-1, cols)
+    if (cols > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < cols):
+        t = t.contiguous()
+    # One row has any pitch: the next multiple of 8, which the kernels read in place.
+    return t, t.stride(0) if t.shape[0] > 1 else (cols + 7) & ~7
+
+
+def _ptr(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
+def _linear_forward(w: _Weight, x, bias, act: int, residual, want_slope: bool, status):
+    shape = (*x.shape[:-1], w.rows)
+    y = torch.empty(shape, dtype=w.dtype, device=w.device)
+    slope = torch.empty_like(y) if want_slope else None
+    x2, ldx = _rows(x, w.cols)
+    r2, ldr = (None, 0) if residual is None else _rows(residual, w.rows)
+    b = None if bias is None else bias.detach().contiguous()
+    tokens = x2.shape[0]
+    if tokens:
+        w.call("zn_linear", (x2.data_ptr(), ldx, tokens),
+               (x2.data_ptr(), ldx, tokens, _ptr(b), act, _ptr(r2), ldr, y.data_ptr(), _ptr(slope)), status)
+    else:
+        status.zero_()
+    return y, slope
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, blob, bias, residual, w, act):
+        status = torch.empty(1, dtype=torch.int32, device=w.device)
+        want = act != 0 and (ctx.needs_input_grad[0] or ctx.needs_input_grad[2])
+        y, slope = _linear_forward(w, x, bias, act, residual, want, status)
+        _set_status(w.device, status)
+        ctx.w, ctx.status, ctx.x_shape = w, status, x.shape
+        ctx.save_for_backward(blob, slope)  # the blob: an in-place change before backward raises
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        w = ctx.w
+        _, slope = ctx.saved_tensors
+        need_x, _, need_b, need_r = ctx.needs_input_grad[:4]
+        dx = torch.empty(ctx.x_shape, dtype=w.dtype, device=w.device) if need_x else None
+        db = torch.zeros(w.rows, dtype=w.dtype, device=w.device) if need_b else None
+        if (need_x or need_b) and dy.numel():
+            with _on(w.device):
+                g, ldy = _rows(dy, w.rows)
+                w.call("zn_linear_grad",
+                       (g.data_ptr(), ldy, g.shape[0], int(slope is not None), int(need_x), int(need_b)),
+                       (g.data_ptr(), ldy, g.shape[0], _ptr(slope), _ptr(dx), _ptr(db)), ctx.status)
+        return dx, None, db, dy if need_r else None, None, None
+
+
+def blob_linear(
+    x: torch.Tensor,
+    blob: torch.Tensor,
+    *,
+    bias: torch.Tensor | None = None,
+    activation: str | None = None,
+    residual: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """activation(x W^T + bias) + residual with the compressed weight W [rows, cols] of `blob`.
+
+    `x` is [..., cols] on the blob's GPU, of the weight's dtype (float16 or bfloat16), with any
+    strides; the result is [..., rows].  `bias` [rows] and `residual` (exactly the result's shape)
+    have the same dtype and device.  `activation` is None, "relu", "gelu" (erf), "gelu_tanh" or
+    "silu".  Products are summed in 32 bits and the result is rounded once.
+
+    Differentiable in x, bias and residual (the weight is frozen).  With an activation the forward
+    pass keeps its derivative, rounded to the dtype, for the backward pass; the weight is decoded
+    again there."""
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"activation must be one of {sorted(map(str, _ACTIVATIONS))}, not {activation!r}")
+    w = _Weight(blob, x, "x")
+    for name, t, shape in (("bias", bias, (w.rows,)), ("residual", residual, (*x.shape[:-1], w.rows))):
+        if t is None:
+            continue
+        if t.dtype != w.dtype:
+            raise TypeError(f"{name} has dtype {t.dtype}, the blob holds {w.dtype}")
+        if tuple(t.shape) != shape:
+            raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {shape}")
+        if t.device != w.device:
+            raise ValueError(f"{name} is on {t.device}, x on {w.device}")
+    w.place("x")
+    act = _ACTIVATIONS[activation]
+    with _on(w.device):
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, bias, residual)):
+            return _Linear.apply(x, blob, bias, residual, w, act)
+        status = torch.empty(1, dtype=torch.int32, device=w.device)
+        y, _ = _linear_forward(w, x, bias, act, residual, False, status)
+        _set_status(w.device, status)
+        return y
+
+
+def _loss_forward(w: _Weight, hidden, ids, logits, top, ignore_index, temperature, reduction, status):
+    """(loss, state, hidden as rows, their pitch)"""
+    h, ldh = _rows(hidden, w.cols)
+    tokens = h.shape[0]
+    loss = torch.empty(ids.shape[0] if reduction == 2 else (), dtype=torch.float32, device=w.device)
+    state = torch.empty(max(1, int(_lib.lib.zn_loss_state_bytes(tokens, top))), dtype=torch.uint8, device=w.device)
+    if tokens:
+        w.call("zn_loss", (h.data_ptr(), ldh, tokens),
+               (h.data_ptr(), ldh, tokens, ids.data_ptr(), _ptr(logits), top, ignore_index, temperature, reduction,
+                loss.data_ptr(), state.data_ptr()), status)
+    else:
+        loss.zero_()
+        status.zero_()
+    return loss, state
+
+
+class _Loss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, blob, w, ids, logits, top, ignore_index, temperature, reduction):
+        status = torch.empty(1, dtype=torch.int32, device=w.device)
+        loss, state = _loss_forward(w, hidden, ids, logits, top, ignore_index, temperature, reduction, status)
+        _set_status(w.device, status)
+        ctx.w, ctx.status, ctx.args = w, status, (top, temperature, reduction)
+        ctx.save_for_backward(hidden, blob, state)
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        w = ctx.w
+        hidden, _, state = ctx.saved_tensors
+        top, temperature, reduction = ctx.args
+        dh = torch.empty(hidden.shape, dtype=w.dtype, device=w.device)
+        if dh.numel():
+            with _on(w.device):
+                h, ldh = _rows(hidden, w.cols)
+                g = grad.float().contiguous()
+                w.call("zn_loss_grad", (h.data_ptr(), ldh, h.shape[0]),
+                       (h.data_ptr(), ldh, h.shape[0], top, temperature, reduction, state.data_ptr(), g.data_ptr(),
+                        dh.data_ptr()), ctx.status)
+        return dh, *(None,) * 8
+
+
+def _loss(hidden, blob, w, ids, logits, top, ignore_index, temperature, reduction, shape):
+    w.place("hidden")
+    red = _REDUCTIONS[reduction]
+    args = (ids, logits, top, ignore_index, temperature, red)
+    with _on(w.device):
+        if torch.is_grad_enabled() and hidden.requires_grad:
+            loss = _Loss.apply(hidden, blob, w, *args)
+        else:
+            status = torch.empty(1, dtype=torch.int32, device=w.device)
+            loss, _ = _loss_forward(w, hidden, *args, status)
+            _set_status(w.device, status)
+        return loss.reshape(shape) if red == 2 else loss
+
+
+def _check_reduction(reduction: str) -> None:
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"reduction must be one of {sorted(_REDUCTIONS)}, not {reduction!r}")
+
+
+def _check_ids(name: str, t: torch.Tensor, shape: tuple[int, ...], w: _Weight) -> None:
+    if t.dtype != torch.int64:
+        raise TypeError(f"{name} must be int64, not {t.dtype}")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {shape}")
+    if t.device != w.device:
+        raise ValueError(f"{name} is on {t.device}, hidden on {w.device}")
+
+
+def blob_cross_entropy(
+    hidden: torch.Tensor,
+    blob: torch.Tensor,
+    targets: torch.Tensor,
+    *,
+    ignore_index: int = -100,
+    reduction: str = "mean",
+) -> torch.Tensor:
+    """Softmax cross entropy of the logits hidden W^T with the compressed head W [vocabulary, cols]
+    of `blob`, without keeping the logits.
+
+    `hidden` is [..., cols] (the weight's dtype, any strides), `targets` int64 [...].  Returns
+    float32: the mean over the rows whose target is not ignore_index (0 when there is none), their
+    "sum", or with "none" one loss per row (0 where ignored).  Any other target outside the
+    vocabulary makes the row's loss and gradient NaN.
+
+    Differentiable in hidden; the backward pass decodes the head and computes the logits again, a
+    piece of the vocabulary at a time.  A piece of softmax - onehot is rounded to the dtype before
+    the product with the piece (sums are in 32 bits); ignored rows get zero gradients whatever they
+    hold."""
+    _check_reduction(reduction)
+    w = _Weight(blob, hidden, "hidden")
+    shape = tuple(hidden.shape[:-1])
+    _check_ids("targets", targets, shape, w)
+    ids = targets.detach().reshape(-1).contiguous()
+    return _loss(hidden, blob, w, ids, None, 1, int(ignore_index), 1.0, reduction, shape)
+
+
+def blob_distillation(
+    hidden: torch.Tensor,
+    blob: torch.Tensor,
+    teacher_logits: torch.Tensor,
+    teacher_ids: torch.Tensor,
+    *,
+    temperature: float = 1.0,
+    reduction: str = "mean",
+) -> torch.Tensor:
+    """Distillation loss temperature^2 * KL(q || softmax(hidden W^T / temperature)) per row, from a
+    teacher's top logits, with the compressed head W [vocabulary, cols] of `blob` and without keeping
+    the student's logits.
+
+    `teacher_ids` int64 and `teacher_logits` (a float type) are [..., top] with top in [1, 256]: the
+    ids of the teacher's best tokens, in any order, and their logits; q is their softmax at the same
+    temperature, over these entries alone.  An id < 0 marks an empty entry (rows may be of different
+    lengths) and an id given twice counts twice.  A row without entries, or whose logits are all
+    -inf, does not count: its loss and gradient are 0 and a "mean" leaves it out (0 when no row
+    counts).  An id past the vocabulary makes the row's loss and gradient NaN.
+
+    Returns float32, "mean", "sum" or per row ("none").  Differentiable in hidden, as
+    blob_cross_entropy; the teacher is a constant."""
+    _check_reduction(reduction)
+    temperature = float(temperature)
+    if not 0.0 < temperature < math.inf:
+        raise ValueError("temperature must be positive and finite")
+    w = _Weight(blob, hidden, "hidden")
+    if teacher_ids.dim() < 1 or not 1 <= teacher_ids.shape[-1] <= _MAX_TOP:
+        raise ValueError(f"teacher_ids must have between 1 and {_MAX_TOP} entries per row")
+    shape, top = tuple(hidden.shape[:-1]), teacher_ids.shape[-1]
+    _check_ids("teacher_ids", teacher_ids, (*shape, top), w)
+    if not teacher_logits.dtype.is_floating_point:
+        raise TypeError(f"teacher_logits must be a float type, not {teacher_logits.dtype}")
+    if tuple(teacher_logits.shape) != (*shape, top):
+        raise ValueError(f"teacher_logits has shape {tuple(teacher_logits.shape)}, expected {(*shape, top)}")
+    if teacher_logits.device != w.device:
+        raise ValueError(f"teacher_logits is on {teacher_logits.device}, hidden on {w.device}")
+    ids = teacher_ids.detach().reshape(-1, top).contiguous()
+    logits = teacher_logits.detach().reshape(-1, top).float().contiguous()
+    return _loss(hidden, blob, w, ids, logits, top, 0, temperature, reduction, shape)

@@ -1,0 +1,1231 @@
+// Operators on compressed weights (the zn_linear_* and zn_loss_* entry points).
+//
+// The weight W [rows, cols] stays a blob.  A call decodes it a piece of rows at a time into its
+// scratch (about one wave of the decoder, so that a weight of any size needs a bounded buffer) and
+// multiplies each piece on the tensor cores (zn_gemm.cuh), with the rest of the operator in the
+// product's epilogue:
+//   linear          y = act(x W^T + b) + r                       EpiLinear
+//   loss, forward   running max and sum of exp over the columns  EpiStats (per row and column tile)
+//   loss, backward  P = softmax(s) - q, one piece wide           EpiProb, then dh += P W by EpiAccum
+// A product with at most kDotRows rows is bound by decoding; it runs inside the decoder instead
+// (weight_dot) and W is never written at all.
+//
+// Losses.  With s = h W^T / T, lse = log sum_v exp s_v and a sparse distribution q over the ids of
+// a row (sum q = 1):  L = T^2 (sum_k q_k (log q_k - s_{id_k}) + lse),  dL/dh = T (softmax(s) - q) W.
+// A cross entropy is the case of one id with q = 1 and T = 1.  The logits are never kept: the
+// backward pass computes a piece of them again.
+#include <algorithm>
+
+#include "zn_gemm.cuh"
+#include "zn_weight.cuh"
+
+namespace zn {
+
+int make_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t pitch, int box_rows, bool bf16) {
+  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static const Encode encode = [] {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult q{};
+    const cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q);
+    return e == cudaSuccess && q == cudaDriverEntryPointSuccess ? reinterpret_cast<Encode>(fn) : nullptr;
+  }();
+  if (!encode) return set_error(ZN_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+  const cuuint64_t dims[2] = {cuuint64_t(cols), cuuint64_t(rows)};
+  const cuuint64_t strides[1] = {cuuint64_t(pitch) * 2};
+  const cuuint32_t box[2] = {kBK, cuuint32_t(box_rows)};
+  const cuuint32_t step[2] = {1, 1};
+  const CUresult r = encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+                            const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(ZN_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", int(r));
+  return ZN_OK;
+}
+
+int sm_count(int* sms) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev);
+  return e == cudaSuccess ? ZN_OK : set_error(ZN_ERR_CUDA, "SM count: %s", cudaGetErrorString(e));
+}
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr int kNone = 0, kRelu = 1, kGelu = 2, kGeluTanh = 3, kSilu = 4;
+constexpr int kMean = 0, kRows = 2;  // reductions (1: sum)
+constexpr int kMaxTop = 256;
+
+// ---- epilogues ------------------------------------------------------------------------------
+
+// act(z) and its derivative (where asked for), in 32 bits.
+template <bool SLOPE>
+__device__ __forceinline__ float activate(int act, float z, float& slope) {
+  switch (act) {
+    case kRelu:
+      if (SLOPE) slope = z > 0.0f ? 1.0f : 0.0f;
+      return z < 0.0f ? 0.0f : z;  // keeps NaN
+    case kGelu: {
+      const float cdf = 0.5f * erfcf(-0.70710678118654752f * z);
+      if (SLOPE) slope = cdf + z * 0.3989422804014327f * __expf(-0.5f * z * z);
+      return z * cdf;
+    }
+    case kGeluTanh: {  // 0.5 z (1 + tanh u) = z sigmoid(2u)
+      const float c = 0.7978845608028654f, z2 = z * z;
+      const float sig = 1.0f / (1.0f + __expf(-2.0f * c * z * (1.0f + 0.044715f * z2)));
+      if (SLOPE) slope = sig + z * sig * (1.0f - sig) * 2.0f * c * (1.0f + 3.0f * 0.044715f * z2);
+      return z * sig;
+    }
+    case kSilu: {
+      const float sig = 1.0f / (1.0f + __expf(-z));
+      if (SLOPE) slope = sig * (1.0f + z * (1.0f - sig));
+      return z * sig;
+    }
+    default:
+      if (SLOPE) slope = 1.0f;
+      return z;
+  }
+}
+
+// y = act(acc + bias) + residual, rounded once to 16 bits; the slope act'(z), which the backward
+// pass multiplies with, is rounded to 16 bits too (it is of order one, so its rounding is that of
+// the gradient it scales).
+template <typename T>
+struct EpiLinear {
+  const T* bias;  // or null
+  const T* res;   // or null
+  T* y;
+  T* slope;  // or null
+  int64_t ldr, ldy, M, N;
+  int act;
+  bool vec;  // 16-byte accesses: every pointer and pitch allows them
+
+  __device__ __forceinline__ float2 pair(float a, float b, float2& sl) const {
+    if (slope) return make_float2(activate<true>(act, a, sl.x), activate<true>(act, b, sl.y));
+    return make_float2(activate<false>(act, a, sl.x), activate<false>(act, b, sl.y));
+  }
+
+  struct Row {
+    int64_t m, n0;
+    __device__ __forceinline__ Row(const EpiLinear&, int64_t m_, int64_t n0_, int) : m(m_), n0(n0_) {}
+    __device__ __forceinline__ void cols(const EpiLinear& e, int c, const float* v) {
+      if (m >= e.M) return;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int64_t n = n0 + c + 8 * g;
+        const float* w = v + 8 * g;
+        if (e.vec && n + 8 <= e.N) {
+          uint32_t bw[4] = {}, rw[4] = {}, yw[4], sw[4];
+          if (e.bias) load16(e.bias + n, bw);
+          if (e.res) load16(e.res + m * e.ldr + n, rw);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float2 sl;
+            float2 z = make_float2(w[2 * i], w[2 * i + 1]);
+            if (e.bias) z = make_float2(z.x + Num<T>::lo(bw[i]), z.y + Num<T>::hi(bw[i]));
+            z = e.pair(z.x, z.y, sl);
+            if (e.res) z = make_float2(z.x + Num<T>::lo(rw[i]), z.y + Num<T>::hi(rw[i]));
+            yw[i] = Num<T>::pack(z.x, z.y);
+            if (e.slope) sw[i] = Num<T>::pack(sl.x, sl.y);
+          }
+          *reinterpret_cast<uint4*>(e.y + m * e.ldy + n) = make_uint4(yw[0], yw[1], yw[2], yw[3]);
+          if (e.slope) *reinterpret_cast<uint4*>(e.slope + m * e.ldy + n) = make_uint4(sw[0], sw[1], sw[2], sw[3]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (n + i < e.N) {
+              float sl, z = w[i] + (e.bias ? Num<T>::to(e.bias[n + i]) : 0.0f);
+              z = e.slope ? activate<true>(e.act, z, sl) : activate<false>(e.act, z, sl);
+              if (e.res) z += Num<T>::to(e.res[m * e.ldr + n + i]);
+              e.y[m * e.ldy + n + i] = Num<T>::from(z);
+              if (e.slope) e.slope[m * e.ldy + n + i] = Num<T>::from(sl);
+            }
+        }
+      }
+    }
+    __device__ __forceinline__ void end(const EpiLinear&) {}
+    static __device__ __forceinline__ void load16(const T* p, uint32_t* w) {
+      const uint4 q = *reinterpret_cast<const uint4*>(p);
+      w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w;
+    }
+  };
+};
+
+// acc[split][m][n] (32 bits) = or += the tile: the parts of a contraction that is cut, across the
+// CTAs of one product or across the pieces of a weight.  finish_kernel adds the splits in order.
+struct EpiAccum {
+  float* acc;
+  int64_t M, N, ld;  // ld: a multiple of 4
+  bool add;
+  struct Row {
+    int64_t m, n0;
+    float* p;
+    __device__ __forceinline__ Row(const EpiAccum& e, int64_t m_, int64_t n0_, int split)
+        : m(m_), n0(n0_), p(e.acc + (int64_t(split) * e.M + m_) * e.ld + n0_) {}
+    __device__ __forceinline__ void cols(const EpiAccum& e, int c, const float* v) {
+      if (m >= e.M) return;
+#pragma unroll
+      for (int g = 0; g < 8; ++g) {
+        if (n0 + c + 4 * g >= e.N) break;  // the pitch covers the last group of 4
+        float4* q = reinterpret_cast<float4*>(p + c + 4 * g);
+        float4 s = make_float4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
+        if (e.add) {
+          const float4 o = *q;
+          s = make_float4(s.x + o.x, s.y + o.y, s.z + o.z, s.w + o.w);
+        }
+        *q = s;
+      }
+    }
+    __device__ __forceinline__ void end(const EpiAccum&) {}
+  };
+};
+
+// Per-row state of a loss (state buffer of a call, kept for the backward pass).
+struct LossRows {
+  float* lse;      // log sum exp of s (NaN for a row with an id out of range)
+  float* q0;       // sum_k q_k log q_k
+  int32_t* count;  // ids of the row (0: the row does not count; -1: an id is out of range)
+  int32_t* ids;    // [tokens][top], ascending
+  float* q;        // [tokens][top], in the order of ids
+  float* rows;     // [1] rows that count
+  int top;
+};
+
+// Position of the first id >= n.
+__device__ __forceinline__ int first_id(const int32_t* ids, int count, int64_t n) {
+  int lo = 0, hi = count;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (ids[mid] < n) lo = mid + 1;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// One pass over the logits of a row: running maximum and sum of 2^(s' - max) with s' = s log2(e),
+// and sum_k q_k s'_{id_k} over the row's ids among the columns seen.
+struct RowStats {
+  float mx, sum, hit;
+};
+__device__ __forceinline__ void stats_join(RowStats& a, float mx, float sum, float hit) {
+  const float m = fmaxf(a.mx, mx);
+  const float base = m == -INFINITY ? 0.0f : m;
+  a.sum = a.sum * exp2f(a.mx - base) + sum * exp2f(mx - base);
+  a.mx = m;
+  a.hit += hit;
+}
+
+struct EpiStats {
+  LossRows rows;
+  float* part;    // [tile][3][M]: max, sum, hit
+  int64_t M, N;   // N: columns of this piece
+  int64_t v0;     // first vocabulary row of this piece
+  int64_t tile0;  // its first column tile
+  int tile_cols;
+  float scale;    // log2(e) / T
+  struct Row {
+    int64_t m, n0;
+    RowStats st;
+    const int32_t* ids;
+    const float* q;
+    int at, count;
+    int64_t next;  // column (of the piece) of the next id
+    __device__ __forceinline__ Row(const EpiStats& e, int64_t m_, int64_t n0_, int) : m(m_), n0(n0_) {
+      st = {-INFINITY, 0.0f, 0.0f};
+      at = count = 0;
+      next = INT64_MAX;
+      ids = nullptr;
+      q = nullptr;
+      if (m < e.M) {
+        count = e.rows.count[m];
+        ids = e.rows.ids + m * e.rows.top;
+        q = e.rows.q + m * e.rows.top;
+        at = first_id(ids, count, e.v0 + n0);
+        if (at < count) next = ids[at] - e.v0;
+      }
+    }
+    __device__ __forceinline__ void cols(const EpiStats& e, int c, const float* v) {
+      if (m >= e.M) return;
+      const int left = int(min(int64_t(32), e.N - n0 - c));
+      if (left <= 0) return;
+      float s[32], mx = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        s[i] = i < left ? v[i] * e.scale : -INFINITY;
+        mx = fmaxf(mx, s[i]);
+      }
+      const float m2 = fmaxf(st.mx, mx), base = m2 == -INFINITY ? 0.0f : m2;
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) sum += exp2f(s[i] - base);
+      st.sum = st.sum * exp2f(st.mx - base) + sum;
+      st.mx = m2;
+      if (next < n0 + c + 32) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          while (next == n0 + c + i) {
+            st.hit += q[at] * s[i];
+            ++at;
+            next = at < count ? ids[at] - e.v0 : INT64_MAX;
+          }
+      }
+    }
+    __device__ __forceinline__ void end(const EpiStats& e) {
+      if (m >= e.M) return;
+      float* p = e.part + (e.tile0 + n0 / e.tile_cols) * 3 * e.M + m;
+      p[0] = st.mx;
+      p[e.M] = st.sum;
+      p[2 * e.M] = st.hit;
+    }
+  };
+};
+
+// P = (softmax(s) - q) * gain of one piece, in 16 bits, as the operand of the product with the
+// piece.  gain keeps small probabilities out of fp16's subnormals (2^15: |softmax - q| <= 1); bf16
+// has the range of 32 bits (gain 1).  Rows that do not count are zero whatever their logits are.
+template <typename T>
+struct EpiProb {
+  LossRows rows;
+  T* p;
+  int64_t M, N, ld, v0;  // ld: a multiple of 8
+  float scale, gain;
+  struct Row {
+    int64_t m, n0;
+    const int32_t* ids;
+    const float* q;
+    float off;
+    int at, count;
+    int64_t next;
+    __device__ __forceinline__ Row(const EpiProb& e, int64_t m_, int64_t n0_, int) : m(m_), n0(n0_) {
+      at = count = 0;
+      next = INT64_MAX;
+      off = 0.0f;
+      ids = nullptr;
+      q = nullptr;
+      if (m < e.M) {
+        count = e.rows.count[m];
+        off = e.rows.lse[m] * kLog2e;
+        ids = e.rows.ids + m * e.rows.top;
+        q = e.rows.q + m * e.rows.top;
+        at = first_id(ids, count, e.v0 + n0);
+        if (at < count) next = ids[at] - e.v0;
+      }
+    }
+    __device__ __forceinline__ void cols(const EpiProb& e, int c, float* v) {
+      if (m >= e.M || n0 + c >= e.N) return;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = count == 0 ? 0.0f : exp2f(v[i] * e.scale - off);
+      if (next < n0 + c + 32) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          while (next == n0 + c + i) {
+            v[i] -= q[at];
+            ++at;
+            next = at < count ? ids[at] - e.v0 : INT64_MAX;
+          }
+      }
+      T* out = e.p + m * e.ld + n0 + c;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        if (n0 + c + 8 * g >= e.N) break;  // the pitch covers the last group of 8
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = Num<T>::pack(v[8 * g + 2 * i] * e.gain, v[8 * g + 2 * i + 1] * e.gain);
+        *reinterpret_cast<uint4*>(out + 8 * g) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+    __device__ __forceinline__ void end(const EpiProb&) {}
+  };
+};
+
+// ---- small kernels --------------------------------------------------------------------------
+
+// Rows of `cols` 16-bit elements to another pitch (a multiple of 8; the padding is not read).
+__global__ void __launch_bounds__(256) pitch_kernel(const uint16_t* src, int64_t lds, uint16_t* dst, int64_t ldd,
+                                                    int64_t rows, int64_t cols) {
+  const int64_t total = rows * cols, step = int64_t(gridDim.x) * blockDim.x;
+  for (int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += step) {
+    const int64_t r = i / cols, c = i - r * cols;
+    dst[r * ldd + c] = src[r * lds + c];
+  }
+}
+
+// z[t, r] of weight_dot: from z, or the parts of a row that spans chunks, in order.
+struct DotValue {
+  const float* z;
+  const float* part;
+  int64_t rows, cols, chunk;
+  __device__ __forceinline__ float get(int64_t t, int64_t r) const {
+    const int64_t c0 = r * cols / chunk, c1 = ((r + 1) * cols - 1) / chunk;
+    if (c0 == c1) return z[t * rows + r];
+    float v = part[(2 * c0 + 1) * kDotRows + t];
+    for (int64_t c = c0 + 1; c <= c1; ++c) v += part[2 * c * kDotRows + t];
+    return v;
+  }
+};
+
+// y = act(z + bias) + residual from z = sum of the splits of acc, or from weight_dot; or
+// y = z * (a scale per row) for the gradient of a loss.
+template <typename T>
+struct Finish {
+  const float* acc;  // [splits][M][ld], or null: dot
+  int64_t M, N, ld;
+  int splits;
+  DotValue dot;
+  EpiLinear<T> lin;
+  // gradient of a loss: row m is scaled by T * grad / (rows that count for a mean) / gain
+  const float* grad;  // or null
+  int64_t grad_step;
+  const int32_t* count;
+  const float* mean_rows;  // or null
+  float factor;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Finish<T> f) {
+  const int64_t total = f.M * f.N, step = int64_t(gridDim.x) * blockDim.x;
+  for (int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += step) {
+    const int64_t m = i / f.N, n = i - m * f.N;
+    float z = 0.0f;
+    if (f.acc)
+      for (int s = 0; s < f.splits; ++s) z += f.acc[(s * f.M + m) * f.ld + n];
+    else z = f.dot.get(m, n);
+    const EpiLinear<T>& e = f.lin;
+    if (f.grad) {
+      if (f.count[m] == 0) z = 0.0f;
+      else z *= f.factor * f.grad[m * f.grad_step] / (f.mean_rows ? *f.mean_rows : 1.0f);
+      e.y[m * e.ldy + n] = Num<T>::from(z);
+      continue;
+    }
+    if (e.bias) z += Num<T>::to(e.bias[n]);
+    float sl;
+    z = e.slope ? activate<true>(e.act, z, sl) : activate<false>(e.act, z, sl);
+    if (e.res) z += Num<T>::to(e.res[m * e.ldr + n]);
+    e.y[m * e.ldy + n] = Num<T>::from(z);
+    if (e.slope) e.slope[m * e.ldy + n] = Num<T>::from(sl);
+  }
+}
+
+// dz = dy * slope in 16 bits (the operand of dx = dz W; dz null: not wanted) and the column sums of
+// the unrounded products over kSumRows rows per block (part[row block][n], 32 bits).
+constexpr int kSumRows = 64;
+template <typename T>
+__global__ void __launch_bounds__(256) slope_kernel(const T* dy, int64_t ldy, const T* slope, T* dz, int64_t ldz,
+                                                    float* part, int64_t M, int64_t N) {
+  const int64_t col_blocks = cdiv(N, 64), mb = blockIdx.x / col_blocks;
+  const int64_t n = (blockIdx.x - mb * col_blocks) * 64 + 2 * (threadIdx.x & 31);
+  const int sub = threadIdx.x >> 5;
+  float2 s = make_float2(0.0f, 0.0f);
+  const int64_t m1 = min(M, (mb + 1) * kSumRows);
+  for (int64_t m = mb * kSumRows + sub; m < m1; m += 8) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (n + i >= N) break;
+      float d = Num<T>::to(dy[m * ldy + n + i]);
+      if (slope) d *= Num<T>::to(slope[m * N + n + i]);
+      if (dz) dz[m * ldz + n + i] = Num<T>::from(d);
+      (i ? s.y : s.x) += d;
+    }
+  }
+  if (!part) return;
+  __shared__ float2 sm[8][32];
+  sm[sub][threadIdx.x & 31] = s;
+  __syncthreads();
+  if (sub == 0) {
+    for (int i = 1; i < 8; ++i) {
+      s.x += sm[i][threadIdx.x].x;
+      s.y += sm[i][threadIdx.x].y;
+    }
+    if (n < N) part[mb * N + n] = s.x;
+    if (n + 1 < N) part[mb * N + n + 1] = s.y;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) column_sum_kernel(const float* part, int64_t blocks, int64_t N, T* out) {
+  const int64_t n = int64_t(blockIdx.x) * 32 + (threadIdx.x & 31);
+  const int sub = threadIdx.x >> 5;
+  float s = 0.0f;
+  if (n < N)
+    for (int64_t b = sub; b < blocks; b += 8) s += part[b * N + n];
+  __shared__ float sm[8][32];
+  sm[sub][threadIdx.x & 31] = s;
+  __syncthreads();
+  if (sub == 0 && n < N) {
+    for (int i = 1; i < 8; ++i) s += sm[i][threadIdx.x];
+    out[n] = Num<T>::from(s);
+  }
+}
+
+// One warp per row: the row's ids in ascending order with their q.  Without logits the row has one
+// id (a target, left out when it equals `ignore`) and q = 1; with them, q = softmax(logits / T)
+// over the ids >= 0.  A row without ids, or whose logits are all -inf, does not count.  The rank of
+// an entry is counted against all others (top <= 256), so no sort network is needed.
+__global__ void __launch_bounds__(128) loss_prep_kernel(const int64_t* ids, const float* logits, int64_t tokens,
+                                                        int64_t vocab, int64_t ignore, float inv_t, LossRows out) {
+  const int64_t m = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (m >= tokens) return;
+  const int top = out.top;
+  int32_t* oid = out.ids + m * top;
+  float* oq = out.q + m * top;
+  if (!logits) {
+    if (lane == 0) {
+      const int64_t id = ids[m];
+      const bool in = id >= 0 && id < vocab;
+      out.count[m] = id == ignore ? 0 : in ? 1 : -1;
+      out.q0[m] = 0.0f;
+      oid[0] = in ? int32_t(id) : 0;
+      oq[0] = 1.0f;
+    }
+    return;
+  }
+  const int64_t* rid = ids + m * top;
+  const float* rl = logits + m * top;
+  float mx = -INFINITY;
+  bool nan = false, bad = false;
+  int held = 0;
+  for (int k = lane; k < top; k += 32) {
+    const int64_t id = rid[k];
+    if (id < 0) continue;
+    ++held;
+    bad |= id >= vocab;
+    nan |= rl[k] != rl[k];
+    mx = fmaxf(mx, rl[k]);
+  }
+  for (int o = 16; o; o >>= 1) {
+    mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
+    held += __shfl_xor_sync(0xFFFFFFFFu, held, o);
+  }
+  nan = __any_sync(0xFFFFFFFFu, nan);
+  bad = __any_sync(0xFFFFFFFFu, bad);
+  if (held == 0 || bad || (mx == -INFINITY && !nan)) {
+    if (lane == 0) {
+      out.count[m] = bad ? -1 : 0;
+      out.q0[m] = 0.0f;
+    }
+    return;
+  }
+  float sum = 0.0f, zq = 0.0f;  // sum of e^z, and of z e^z
+  for (int k = lane; k < top; k += 32)
+    if (rid[k] >= 0) {
+      const float z = (rl[k] - mx) * inv_t, e = expf(z);
+      sum += e;
+      if (e > 0.0f) zq += z * e;
+    }
+  for (int o = 16; o; o >>= 1) {
+    sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    zq += __shfl_xor_sync(0xFFFFFFFFu, zq, o);
+  }
+  for (int k = lane; k < top; k += 32) {
+    const int64_t id = rid[k];
+    if (id < 0) continue;
+    int rank = 0;
+    for (int i = 0; i < top; ++i) {
+      const int64_t o = rid[i];
+      rank += o >= 0 && (o < id || (o == id && i < k));
+    }
+    oid[rank] = int32_t(id);
+    oq[rank] = expf((rl[k] - mx) * inv_t) / sum;
+  }
+  if (lane == 0) {
+    out.count[m] = held;
+    out.q0[m] = nan ? NAN : zq / sum - logf(sum);
+  }
+}
+
+// Statistics of the logits of weight_dot: a block per (column tile of kStatCols, token).
+constexpr int kStatCols = 2048;
+__global__ void __launch_bounds__(256) dot_stats_kernel(DotValue v, LossRows rows, float* part, int64_t tokens,
+                                                        float scale) {
+  const int64_t m = blockIdx.y, n0 = int64_t(blockIdx.x) * kStatCols;
+  const int64_t n1 = min(v.rows, n0 + kStatCols);
+  const int count = rows.count[m];
+  const int32_t* ids = rows.ids + m * rows.top;
+  const float* q = rows.q + m * rows.top;
+  constexpr int kPer = kStatCols / 256;
+  float s[kPer], mx = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int64_t n = n0 + threadIdx.x + 256 * i;
+    s[i] = n < n1 ? v.get(m, n) * scale : -INFINITY;
+    mx = fmaxf(mx, s[i]);
+  }
+  const float base = mx == -INFINITY ? 0.0f : mx;
+  float sum = 0.0f, hit = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    sum += exp2f(s[i] - base);
+    const int64_t n = n0 + threadIdx.x + 256 * i;
+    if (n < n1)
+      for (int k = first_id(ids, count, n); k < count && ids[k] == n; ++k) hit += q[k] * s[i];
+  }
+  __shared__ RowStats sm[8];
+  RowStats st{mx, sum, hit};
+  for (int o = 16; o; o >>= 1) {
+    const float a = __shfl_xor_sync(0xFFFFFFFFu, st.mx, o), b = __shfl_xor_sync(0xFFFFFFFFu, st.sum, o),
+                c = __shfl_xor_sync(0xFFFFFFFFu, st.hit, o);
+    stats_join(st, a, b, c);
+  }
+  if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = st;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 8; ++i) stats_join(st, sm[i].mx, sm[i].sum, sm[i].hit);
+    float* p = part + int64_t(blockIdx.x) * 3 * tokens + m;
+    p[0] = st.mx;
+    p[tokens] = st.sum;
+    p[2 * tokens] = st.hit;
+  }
+}
+
+// Joins the tiles' statistics of 32 rows per block (in a fixed order) into lse and the rows' losses.
+__global__ void __launch_bounds__(1024) loss_rows_kernel(const float* part, int64_t tiles, int64_t tokens,
+                                                         float temperature, LossRows rows, float* loss) {
+  const int64_t m = int64_t(blockIdx.x) * 32 + (threadIdx.x & 31);
+  const int sub = threadIdx.x >> 5;
+  RowStats st{-INFINITY, 0.0f, 0.0f};
+  if (m < tokens)
+    for (int64_t t = sub; t < tiles; t += 32) {
+      const float* p = part + t * 3 * tokens + m;
+      stats_join(st, p[0], p[tokens], p[2 * tokens]);
+    }
+  __shared__ RowStats sm[32][33];
+  sm[sub][threadIdx.x & 31] = st;
+  __syncthreads();
+  if (sub != 0 || m >= tokens) return;
+  for (int i = 1; i < 32; ++i) stats_join(st, sm[i][threadIdx.x].mx, sm[i][threadIdx.x].sum, sm[i][threadIdx.x].hit);
+  const int count = rows.count[m];
+  const float lse = count < 0 ? NAN : (st.mx + log2f(st.sum)) * kLn2;
+  rows.lse[m] = lse;
+  loss[m] = count == 0 ? 0.0f : temperature * temperature * (rows.q0[m] + (lse - st.hit * kLn2));
+}
+
+// Sum or mean over the rows that count, added in 64 bits by one block in a fixed order.
+__global__ void __launch_bounds__(1024) loss_reduce_kernel(const float* row_loss, LossRows rows, int64_t tokens,
+                                                           bool mean, float* loss) {
+  double s = 0.0;
+  int64_t n = 0;
+  for (int64_t m = threadIdx.x; m < tokens; m += 1024) {
+    s += row_loss[m];
+    n += rows.count[m] != 0;
+  }
+  __shared__ double ss[1024];
+  __shared__ int64_t sn[1024];
+  ss[threadIdx.x] = s;
+  sn[threadIdx.x] = n;
+  __syncthreads();
+  for (int o = 512; o; o >>= 1) {
+    if (int(threadIdx.x) < o) {
+      ss[threadIdx.x] += ss[threadIdx.x + o];
+      sn[threadIdx.x] += sn[threadIdx.x + o];
+    }
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) {
+    const double count = sn[0] > 0 ? double(sn[0]) : 1.0;
+    *loss = float(mean ? ss[0] / count : ss[0]);
+    *rows.rows = float(count);
+  }
+}
+
+// ---- host side ------------------------------------------------------------------------------
+
+// Carves a scratch buffer into 256-byte aligned parts; with a null base it only counts.
+struct Arena {
+  uint8_t* base;
+  size_t used = 0;
+  template <typename T = void>
+  T* take(size_t bytes) {
+    const size_t at = used;
+    used += (bytes + 255) & ~size_t(255);
+    return base ? reinterpret_cast<T*>(base + at) : nullptr;
+  }
+};
+
+int64_t round8(int64_t n) { return (n + 7) & ~int64_t(7); }
+unsigned grid_1d(int64_t items, int per, int64_t most) {
+  return unsigned(std::max<int64_t>(1, std::min(most, cdiv(items, per))));
+}
+
+// A 16-bit matrix that TMA can read.
+struct Matrix {
+  const void* p;
+  int64_t rows, cols, pitch;
+};
+bool tma_ready(const void* p, int64_t pitch) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && pitch % 8 == 0; }
+
+int copy_pitch(const void* src, int64_t lds, void* dst, int64_t ldd, int64_t rows, int64_t cols, cudaStream_t s) {
+  if (rows * cols == 0) return ZN_OK;
+  pitch_kernel<<<grid_1d(rows * cols, 1024, 148 * 16), 256, 0, s>>>(static_cast<const uint16_t*>(src), lds,
+                                                                    static_cast<uint16_t*>(dst), ldd, rows, cols);
+  count_launch();
+  return check_launch("pitch_kernel");
+}
+
+// A weight and the scratch that its pieces are decoded into.
+struct Weight {
+  WeightBlob b;
+  bool stored;
+  int64_t piece_rows, pieces;
+  void* temp;
+  uint8_t* flat;    // decoded chunks of a piece
+  uint8_t* padded;  // its rows at a pitch that TMA can read, when cols is not a multiple of 8
+  int64_t pitch;
+  int32_t* status;
+};
+
+// rows_cap bounds the rows of a piece (0: no bound).
+int plan_weight(const zn_weight* w, int64_t rows_cap, int32_t* status, Arena& ar, Weight* out) {
+  *out = {};
+  out->b = {static_cast<const uint8_t*>(w->blob), w->blob_bytes, w->rows, w->cols, w->chunk_bytes, w->dtype == 8};
+  out->stored = w->chunk_bytes == 0;
+  out->status = status;
+  out->pitch = round8(w->cols);
+  const int64_t n = w->rows * w->cols;
+  int64_t rows = w->rows;
+  if (!out->stored) {
+    // A piece is one wave of the decoder (5 blocks per SM, 128 Ki elements each at the default
+    // chunk size: 194 MB), so that no piece ends in a nearly empty wave; a weight of up to two
+    // waves is one piece.
+    int64_t wave = 0;
+    if (int rc = weight_wave(out->b, &wave)) return rc;
+    if (cdiv(n, w->chunk_bytes) > 2 * wave) rows = std::max<int64_t>(1, wave * w->chunk_bytes / w->cols);
+  }
+  if (rows_cap > 0) rows = std::min(rows, rows_cap);
+  if (rows < w->rows) rows = std::max<int64_t>(256, rows / 256 * 256);
+  out->piece_rows = std::min(rows, w->rows);
+  out->pieces = cdiv(w->rows, out->piece_rows);
+  if (!out->stored) {
+    out->temp = ar.take(weight_temp_bytes(out->b));
+    const int64_t chunks = std::min(cdiv(n, w->chunk_bytes), cdiv(out->piece_rows * w->cols, w->chunk_bytes) + 1);
+    out->flat = ar.take<uint8_t>(size_t(chunks) * w->chunk_bytes * 2);
+  }
+  if (out->stored || w->cols % 8) out->padded = ar.take<uint8_t>(size_t(out->piece_rows) * out->pitch * 2);
+  return ZN_OK;
+}
+
+int start_weight(const Weight& w, cudaStream_t s) {
+  if (!w.stored) return weight_scan(w.b, w.temp, w.status, s);
+  const cudaError_t e = cudaMemsetAsync(w.status, 0, sizeof(int32_t), s);
+  return e == cudaSuccess ? ZN_OK : set_error(ZN_ERR_CUDA, "status: %s", cudaGetErrorString(e));
+}
+
+// Rows [r0, r1) as a matrix in memory.
+int load_piece(const Weight& w, int64_t r0, int64_t r1, Matrix* out, cudaStream_t s) {
+  const int64_t cols = w.b.cols;
+  const uint8_t* src;
+  if (w.stored) {
+    src = w.b.blob + 24 + 8 * 2 + r0 * cols * 2;
+  } else {
+    const int64_t c0 = r0 * cols / w.b.chunk, c1 = cdiv(r1 * cols, w.b.chunk);
+    if (int rc = weight_decode(w.b, w.temp, c0, c1, w.flat, w.status, s)) return rc;
+    src = w.flat + (r0 * cols - c0 * w.b.chunk) * 2;
+  }
+  *out = {src, r1 - r0, cols, cols};
+  if (!w.padded) return ZN_OK;  // cols and the chunk size are multiples of 8: the rows are aligned
+  *out = {w.padded, r1 - r0, cols, w.pitch};
+  return copy_pitch(src, cols, w.padded, w.pitch, r1 - r0, cols, s);
+}
+
+// A caller's matrix, copied to an aligned pitch when TMA cannot read it as it lies.
+void* plan_matrix(const void* p, int64_t rows, int64_t cols, int64_t pitch, Arena& ar) {
+  return tma_ready(p, pitch) ? nullptr : ar.take(size_t(rows) * round8(cols) * 2);
+}
+int load_matrix(const void* p, int64_t rows, int64_t cols, int64_t pitch, void* copy, Matrix* out, cudaStream_t s) {
+  *out = {p, rows, cols, pitch};
+  if (!copy) return ZN_OK;
+  *out = {copy, rows, cols, round8(cols)};
+  return copy_pitch(p, pitch, copy, round8(cols), rows, cols, s);
+}
+
+// How a product [M, K] x [N, K] is cut.  Tiles of 128 x 256 when they fill the GPU; else tiles of
+// 128 x 128, and the contraction is split until there is about one tile per SM (at least 4 blocks
+// of 64 per part).
+struct Cut {
+  int bn, splits;
+};
+Cut cut_of(int64_t M, int64_t N, int64_t K, int sms, bool split) {
+  const int64_t tm = cdiv(M, kBM);
+  if (tm * cdiv(N, 256) >= sms) return {256, 1};
+  const int64_t tiles = tm * cdiv(N, 128), kb = cdiv(K, kBK);
+  if (!split) return {128, 1};
+  return {128, int(std::max<int64_t>(1, std::min(sms / std::max<int64_t>(1, tiles), kb / 4)))};
+}
+
+template <typename T, bool BMN, class Epi>
+int product(const Matrix& a, const Matrix& b, const Cut& cut, const Epi& epi, int32_t* status, cudaStream_t s) {
+  const int64_t M = a.rows, K = a.cols, N = BMN ? b.cols : b.rows;
+  constexpr bool bf16 = Num<T>::kCode == 1;
+  CUtensorMap ma, mb;
+  if (int rc = make_map(&ma, a.p, a.rows, a.cols, a.pitch, kBM, bf16)) return rc;
+  if (int rc = make_map(&mb, b.p, b.rows, b.cols, b.pitch, BMN ? kBK : cut.bn, bf16)) return rc;
+  GemmShape g = gemm_shape(M, N, K, cut.bn, status);
+  g.splits = cut.splits;
+  if (cut.bn == 256) return launch_gemm<T, 256, BMN>(ma, mb, g, epi, s);
+  return launch_gemm<T, 128, BMN>(ma, mb, g, epi, s);
+}
+
+template <typename T>
+int run_finish(const Finish<T>& f, cudaStream_t s) {
+  TimedLaunch tl("finish", s);
+  finish_kernel<T><<<grid_1d(f.M * f.N, 1024, 148 * 16), 256, 0, s>>>(f);
+  count_launch();
+  return check_launch("finish_kernel");
+}
+
+int bad(const char* what) { return set_error(ZN_ERR_INVALID, "%s: bad arguments", what); }
+
+bool weight_ok(const zn_weight* w) {
+  constexpr int64_t kMost = int64_t(1) << 31;
+  if (!w || w->rows <= 0 || w->cols <= 0 || w->rows >= kMost || w->cols >= kMost) return false;
+  if (w->rows > (int64_t(1) << 46) / w->cols || (w->dtype != 7 && w->dtype != 8)) return false;
+  if (w->chunk_bytes < 0 || w->chunk_bytes % 8 || w->chunk_bytes > kMaxChunkBytes) return false;
+  if (w->chunk_bytes == 0) return w->blob_bytes >= 24 + 16 + w->rows * w->cols * 2;
+  return w->blob_bytes >= 40 && cdiv(w->rows * w->cols, w->chunk_bytes) <= 0x7FFFFFFF;
+}
+bool sizes_ok(int64_t tokens, int64_t pitch, int64_t cols) {
+  return tokens > 0 && tokens < (int64_t(1) << 31) && pitch >= cols && pitch < (int64_t(1) << 39);
+}
+
+// ---- linear ---------------------------------------------------------------------------------
+
+struct LinearPlan {
+  Weight w;
+  bool dot;
+  Cut cut;
+  void* x_copy;
+  float* acc;   // split parts of a piece, or z of the dot path
+  float* part;  // dot path
+  int64_t ld;
+  int sms;
+};
+
+int plan_linear(const zn_weight* w, const void* x, int64_t ldx, int64_t tokens, int32_t* status, Arena& ar,
+                LinearPlan* p) {
+  *p = {};
+  if (int rc = sm_count(&p->sms)) return rc;
+  p->dot = w->chunk_bytes > 0 && dot_shape(tokens, w->cols, w->chunk_bytes);
+  p->x_copy = plan_matrix(x, tokens, w->cols, ldx, ar);
+  if (p->dot) {
+    p->w.b = {static_cast<const uint8_t*>(w->blob), w->blob_bytes, w->rows, w->cols, w->chunk_bytes, w->dtype == 8};
+    p->w.status = status;
+    p->w.temp = ar.take(weight_temp_bytes(p->w.b));
+    p->acc = ar.take<float>(size_t(tokens) * w->rows * 4);
+    p->part = ar.take<float>(dot_part_bytes(p->w.b));
+    return ZN_OK;
+  }
+  if (int rc = plan_weight(w, 0, status, ar, &p->w)) return rc;
+  p->cut = cut_of(tokens, p->w.piece_rows, w->cols, p->sms, true);
+  p->ld = (p->w.piece_rows + 3) & ~int64_t(3);
+  if (p->cut.splits > 1) p->acc = ar.take<float>(size_t(p->cut.splits) * tokens * p->ld * 4);
+  return ZN_OK;
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+template <typename T>
+EpiLinear<T> linear_epilogue(const void* bias, const void* res, int64_t ldr, void* y, void* slope, int64_t ldy,
+                             int64_t M, int64_t r0, int64_t r1, int act) {
+  EpiLinear<T> e{};
+  e.bias = bias ? static_cast<const T*>(bias) + r0 : nullptr;
+  e.res = res ? static_cast<const T*>(res) + r0 : nullptr;
+  e.y = static_cast<T*>(y) + r0;
+  e.slope = slope ? static_cast<T*>(slope) + r0 : nullptr;
+  e.ldr = ldr;
+  e.ldy = ldy;
+  e.M = M;
+  e.N = r1 - r0;
+  e.act = act;
+  e.vec = aligned16(e.bias) && aligned16(e.res) && aligned16(e.y) && aligned16(e.slope) && ldy % 8 == 0 &&
+          (!res || ldr % 8 == 0);
+  return e;
+}
+
+template <typename T>
+int run_linear(const LinearPlan& p, const void* x, int64_t ldx, int64_t tokens, const void* bias, int act,
+               const void* res, int64_t ldr, void* y, void* slope, cudaStream_t s) {
+  const int64_t rows = p.w.b.rows, cols = p.w.b.cols;
+  if (int rc = start_weight(p.w, s)) return rc;
+  Matrix xm;
+  if (int rc = load_matrix(x, tokens, cols, ldx, p.x_copy, &xm, s)) return rc;
+  Finish<T> f{};
+  f.M = tokens;
+  if (p.dot) {
+    if (int rc = weight_dot(p.w.b, p.w.temp, xm.p, xm.pitch, int(tokens), p.acc, p.part, p.w.status, s)) return rc;
+    f.N = rows;
+    f.dot = {p.acc, p.part, rows, cols, p.w.b.chunk};
+    f.lin = linear_epilogue<T>(bias, res, ldr, y, slope, rows, tokens, 0, rows, act);
+    return run_finish(f, s);
+  }
+  for (int64_t r0 = 0; r0 < rows; r0 += p.w.piece_rows) {
+    const int64_t r1 = std::min(rows, r0 + p.w.piece_rows);
+    Matrix wm;
+    if (int rc = load_piece(p.w, r0, r1, &wm, s)) return rc;
+    const EpiLinear<T> e = linear_epilogue<T>(bias, res, ldr, y, slope, rows, tokens, r0, r1, act);
+    if (p.cut.splits == 1) {
+      if (int rc = product<T, false>(xm, wm, p.cut, e, p.w.status, s)) return rc;
+      continue;
+    }
+    const EpiAccum a{p.acc, tokens, r1 - r0, p.ld, false};
+    if (int rc = product<T, false>(xm, wm, p.cut, a, p.w.status, s)) return rc;
+    f.acc = p.acc;
+    f.N = r1 - r0;
+    f.ld = p.ld;
+    f.splits = p.cut.splits;
+    f.lin = e;
+    if (int rc = run_finish(f, s)) return rc;
+  }
+  return ZN_OK;
+}
+
+struct LinearGradPlan {
+  Weight w;
+  Cut cut;
+  void* dz;  // dy * slope, or an aligned copy of dy
+  int64_t ldz;
+  float* acc;
+  float* part;
+  int64_t ld, sum_blocks;
+};
+
+int plan_linear_grad(const zn_weight* w, const void* dy, int64_t ldy, int64_t tokens, bool slope, bool dx, bool dbias,
+                     int32_t* status, Arena& ar, LinearGradPlan* p) {
+  *p = {};
+  int sms = 0;
+  if (int rc = sm_count(&sms)) return rc;
+  p->sum_blocks = cdiv(tokens, kSumRows);
+  if (dbias) p->part = ar.take<float>(size_t(p->sum_blocks) * w->rows * 4);
+  p->w.status = status;
+  if (!dx) return ZN_OK;
+  p->ldz = round8(w->rows);
+  if (slope || !tma_ready(dy, ldy)) p->dz = ar.take(size_t(tokens) * p->ldz * 2);
+  if (int rc = plan_weight(w, 0, status, ar, &p->w)) return rc;
+  p->cut = cut_of(tokens, w->cols, p->w.piece_rows, sms, true);
+  p->ld = (w->cols + 3) & ~int64_t(3);
+  if (p->cut.splits > 1 || p->w.pieces > 1) p->acc = ar.take<float>(size_t(p->cut.splits) * tokens * p->ld * 4);
+  return ZN_OK;
+}
+
+template <typename T>
+int run_linear_grad(const LinearGradPlan& p, const zn_weight* w, const void* dy, int64_t ldy, int64_t tokens,
+                    const void* slope, void* dx, void* dbias, cudaStream_t s) {
+  const int64_t rows = w->rows, cols = w->cols;
+  const T* g = static_cast<const T*>(dy);
+  if (slope || dbias) {
+    T* dz = slope ? static_cast<T*>(p.dz) : nullptr;
+    const int64_t grid = cdiv(rows, 64) * p.sum_blocks;
+    if (grid > 0x7FFFFFFF) return bad("zn_linear_grad");
+    slope_kernel<T><<<unsigned(grid), 256, 0, s>>>(g, ldy, static_cast<const T*>(slope), dz, p.ldz, p.part, tokens, rows);
+    count_launch();
+    if (int rc = check_launch("slope_kernel")) return rc;
+  }
+  if (dbias) {
+    column_sum_kernel<T><<<unsigned(cdiv(rows, 32)), 256, 0, s>>>(p.part, p.sum_blocks, rows, static_cast<T*>(dbias));
+    count_launch();
+    if (int rc = check_launch("column_sum_kernel")) return rc;
+  }
+  if (!dx) {
+    const cudaError_t e = cudaMemsetAsync(p.w.status, 0, sizeof(int32_t), s);
+    return e == cudaSuccess ? ZN_OK : set_error(ZN_ERR_CUDA, "status: %s", cudaGetErrorString(e));
+  }
+  if (int rc = start_weight(p.w, s)) return rc;
+  Matrix dzm{p.dz, tokens, rows, p.ldz};
+  if (!slope)
+    if (int rc = load_matrix(dy, tokens, rows, ldy, p.dz, &dzm, s)) return rc;
+  const EpiLinear<T> e = linear_epilogue<T>(nullptr, nullptr, 0, dx, nullptr, cols, tokens, 0, cols, kNone);
+  for (int64_t r0 = 0; r0 < rows; r0 += p.w.piece_rows) {
+    const int64_t r1 = std::min(rows, r0 + p.w.piece_rows);
+    Matrix wm;
+    if (int rc = load_piece(p.w, r0, r1, &wm, s)) return rc;
+    // Columns [r0, r1) of dz (r0 is a multiple of 256: the rows stay 16-byte aligned).
+    const Matrix a{static_cast<const T*>(dzm.p) + r0, tokens, r1 - r0, dzm.pitch};
+    if (!p.acc) {
+      if (int rc = product<T, true>(a, wm, p.cut, e, p.w.status, s)) return rc;
+      continue;
+    }
+    const EpiAccum acc{p.acc, tokens, cols, p.ld, r0 > 0};
+    if (int rc = product<T, true>(a, wm, p.cut, acc, p.w.status, s)) return rc;
+  }
+  if (!p.acc) return ZN_OK;
+  Finish<T> f{};
+  f.acc = p.acc;
+  f.M = tokens;
+  f.N = cols;
+  f.ld = p.ld;
+  f.splits = p.cut.splits;
+  f.lin = e;
+  return run_finish(f, s);
+}
+
+// ---- losses ---------------------------------------------------------------------------------
+
+LossRows loss_state(void* state, int64_t tokens, int top, size_t* bytes) {
+  Arena ar{static_cast<uint8_t*>(state)};
+  LossRows r{};
+  r.lse = ar.take<float>(size_t(tokens) * 4);
+  r.q0 = ar.take<float>(size_t(tokens) * 4);
+  r.count = ar.take<int32_t>(size_t(tokens) * 4);
+  r.ids = ar.take<int32_t>(size_t(tokens) * top * 4);
+  r.q = ar.take<float>(size_t(tokens) * top * 4);
+  r.rows = ar.take<float>(4);
+  r.top = top;
+  if (bytes) *bytes = ar.used;
+  return r;
+}
+
+struct LossPlan {
+  Weight w;
+  bool dot;
+  Cut cut;
+  void* x_copy;
+  float* part;      // tile statistics
+  float* row_loss;  // when the call returns their sum or mean
+  float* z;         // dot path
+  float* z_part;
+  int64_t tiles;
+};
+
+int plan_loss(const zn_weight* w, const void* x, int64_t ldx, int64_t tokens, int32_t* status, Arena& ar, LossPlan* p) {
+  *p = {};
+  int sms = 0;
+  if (int rc = sm_count(&sms)) return rc;
+  p->x_copy = plan_matrix(x, tokens, w->cols, ldx, ar);
+  p->row_loss = ar.take<float>(size_t(tokens) * 4);
+  p->dot = w->chunk_bytes > 0 && dot_shape(tokens, w->cols, w->chunk_bytes);
+  if (p->dot) {
+    p->w.b = {static_cast<const uint8_t*>(w->blob), w->blob_bytes, w->rows, w->cols, w->chunk_bytes, w->dtype == 8};
+    p->w.status = status;
+    p->w.temp = ar.take(weight_temp_bytes(p->w.b));
+    p->z = ar.take<float>(size_t(tokens) * w->rows * 4);
+    p->z_part = ar.take<float>(dot_part_bytes(p->w.b));
+    p->tiles = cdiv(w->rows, kStatCols);
+  } else {
+    if (int rc = plan_weight(w, 0, status, ar, &p->w)) return rc;
+    p->cut = cut_of(tokens, p->w.piece_rows, w->cols, sms, false);
+    // Every piece but the last is a multiple of 256 rows.
+    p->tiles = cdiv(w->rows, p->cut.bn);
+  }
+  p->part = ar.take<float>(size_t(p->tiles) * 3 * tokens * 4);
+  return ZN_OK;
+}
+
+template <typename T>
+int run_loss(const LossPlan& p, const void* x, int64_t ldx, int64_t tokens, const int64_t* ids, const float* logits,
+             int64_t ignore, float temperature, int reduction, float* loss, const LossRows& rows, cudaStream_t s) {
+  const int64_t vocab = p.w.b.rows, cols = p.w.b.cols;
+  const float inv_t = 1.0f / temperature;
+  loss_prep_kernel<<<unsigned(cdiv(tokens, 4)), 128, 0, s>>>(ids, logits, tokens, vocab, ignore, inv_t, rows);
+  count_launch();
+  if (int rc = check_launch("loss_prep_kernel")) return rc;
+  if (int rc = start_weight(p.w, s)) return rc;
+  Matrix xm;
+  if (int rc = load_matrix(x, tokens, cols, ldx, p.x_copy, &xm, s)) return rc;
+  if (p.dot) {
+    if (int rc = weight_dot(p.w.b, p.w.temp, xm.p, xm.pitch, int(tokens), p.z, p.z_part, p.w.status, s)) return rc;
+    const DotValue v{p.z, p.z_part, vocab, cols, p.w.b.chunk};
+    dot_stats_kernel<<<dim3(unsigned(p.tiles), unsigned(tokens)), 256, 0, s>>>(v, rows, p.part, tokens, kLog2e * inv_t);
+    count_launch();
+    if (int rc = check_launch("dot_stats_kernel")) return rc;
+  } else {
+    for (int64_t r0 = 0; r0 < vocab; r0 += p.w.piece_rows) {
+      const int64_t r1 = std::min(vocab, r0 + p.w.piece_rows);
+      Matrix wm;
+      if (int rc = load_piece(p.w, r0, r1, &wm, s)) return rc;
+      const EpiStats e{rows, p.part, tokens, r1 - r0, r0, r0 / p.cut.bn, p.cut.bn, kLog2e * inv_t};
+      if (int rc = product<T, false>(xm, wm, p.cut, e, p.w.status, s)) return rc;
+    }
+  }
+  float* row_loss = reduction == kRows ? loss : p.row_loss;
+  loss_rows_kernel<<<unsigned(cdiv(tokens, 32)), 1024, 0, s>>>(p.part, p.tiles, tokens, temperature, rows, row_loss);
+  count_launch();
+  if (int rc = check_launch("loss_rows_kernel")) return rc;
+  if (reduction == kRows) return ZN_OK;
+  loss_reduce_kernel<<<1, 1024, 0, s>>>(row_loss, rows, tokens, reduction == kMean, loss);
+  count_launch();
+  return check_launch("loss_reduce_kernel");
+}
+
+// The backward pass's pieces are bounded so that P [tokens, piece] stays within 512 MB too.
+constexpr int64_t kProbBytes = int64_t(1) << 29;
+
+struct LossGradPlan {
+  Weight w;
+  Cut cut, cut_dh;
+  void* x_copy;
+  void* prob;
+  int64_t ldp, ld;
+  float* acc;
+};
+
+int plan_loss_grad(const zn_weight* w, const void* x, int64_t ldx, int64_t tokens, int32_t* status, Arena& ar,
+                   LossGradPlan* p) {
+  *p = {};
+  int sms = 0;
+  if (int rc = sm_count(&sms)) return rc;
+  p->x_copy = plan_matrix(x, tokens, w->cols, ldx, ar);
+  if (int rc = plan_weight(w, std::max<int64_t>(256, kProbBytes / 2 / tokens), status, ar, &p->w)) return rc;
+  p->cut = cut_of(tokens, p->w.piece_rows, w->cols, sms, false);
+  p->cut_dh = cut_of(tokens, w->cols, p->w.piece_rows, sms, true);
+  p->ldp = round8(p->w.piece_rows);
+  p->prob = ar.take(size_t(tokens) * p->ldp * 2);
+  p->ld = (w->cols + 3) & ~int64_t(3);
+  p->acc = ar.take<float>(size_t(p->cut_dh.splits) * tokens * p->ld * 4);
+  return ZN_OK;
+}
+
+template <typename T>
+int run_loss_grad(const LossGradPlan& p, const void* x, int64_t ldx, int64_t tokens, float temperature, int reduction,
+                  const LossRows& rows, const float* grad, void* dx, cudaStream_t s) {
+  const int64_t vocab = p.w.b.rows, cols = p.w.b.cols;
+  const float gain = Num<T>::kCode == 1 ? 1.0f : 32768.0f;
+  if (int rc = start_weight(p.w, s)) return rc;
+  Matrix xm;
+  if (int rc = load_matrix(x, tokens, cols, ldx, p.x_copy, &xm, s)) return rc;
+  for (int64_t r0 = 0; r0 < vocab; r0 += p.w.piece_rows) {
+    const int64_t r1 = std::min(vocab, r0 + p.w.piece_rows);
+    Matrix wm;
+    if (int rc = load_piece(p.w, r0, r1, &wm, s)) return rc;
+    const EpiProb<T> e{rows, static_cast<T*>(p.prob), tokens, r1 - r0, p.ldp, r0, kLog2e / temperature, gain};
+    if (int rc = product<T, false>(xm, wm, p.cut, e, p.w.status, s)) return rc;
+    const Matrix pm{p.prob, tokens, r1 - r0, p.ldp};
+    const EpiAccum a{p.acc, tokens, cols, p.ld, r0 > 0};
+    if (int rc = product<T, true>(pm, wm, p.cut_dh, a, p.w.status, s)) return rc;
+  }
+  Finish<T> f{};
+  f.acc = p.acc;
+  f.M = tokens;
+  f.N = cols;
+  f.ld = p.ld;
+  f.splits = p.cut_dh.splits;
+  f.lin.y = static_cast<T*>(dx);
+  f.lin.ldy = cols;
+  f.grad = grad;
+  f.grad_step = reduction == kRows;
+  f.count = rows.count;
+  f.mean_rows = reduction == kMean ? rows.rows : nullptr;
+  f.factor = temperature / gain;
+  return run_finish(f, s);
+}
+
+bool loss_ok(const zn_weight* w, int64_t tokens, int64_t ldx, int top, float temperature, int reduction) {
+  return weight_ok(w) && sizes_ok(tokens, ldx, w->cols) && top >= 1 && top <= kMaxTop && temperature > 0.0f &&
+         temperature < INFINITY && reduction >= kMean && reduction <= kRows;
+}
+
+}  // namespace
+}  // namespace zn
+
+using namespace zn;
+
+extern "C" {
+
+size_t zn_linear_temp_bytes(const zn_weight* w, const void* x, int64_t ldx, int64_t tokens) {
+  if (!weight_ok(w) || !sizes_ok(tokens, ldx, w->cols)) return 0;
+  Arena ar{nullptr};
+  LinearPlan p;
+  return plan_linear(w, x, ldx, tokens, nullptr, ar, &p) ? 0 : ar.used;
+}
+
+int zn_linear(const zn_weight* w, const void* x, int64_t ldx, int64_t tokens, const void* bias, int activation,
+              const void* residual, int64_t ldr, void* y, void* slope, int32_t* status, void* temp, size_t temp_bytes,
+              void* stream) {
+  if (!weight_ok(w) || !sizes_ok(tokens, ldx, w->cols) || (residual && !sizes_ok(tokens, ldr, w->rows)) ||
+      activation < kNone || activation > kSilu || !w->blob || (reinterpret_cast<uintptr_t>(w->blob) & 7) || !x || !y ||
+      !status)
+    return bad("zn_linear");
+  NvtxScope range("zn_linear");
+  Arena ar{static_cast<uint8_t*>(temp)};
+  LinearPlan p;
+  if (int rc = plan_linear(w, x, ldx, tokens, status, ar, &p)) return rc;
+  if (!temp || temp_bytes < ar.used) return set_error(ZN_ERR_SPACE, "zn_linear: temp buffer too small");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return w->dtype == 8
+             ? run_linear<__nv_bfloat16>(p, x, ldx, tokens, bias, activation, residual, ldr, y, slope, s)
+             : run_linear<__half>(p, x, ldx, tokens, bias, activation, residual, ldr, y, slope, s);
+}
+
+size_t zn_linear_grad_temp_bytes(const zn_weight* w, const void* dy, int64_t ldy, int64_t tokens, int slope, int dx,
+                                 int dbias) {
+  if (!weight_ok(w) || !sizes_ok(tokens, ldy, w->rows)) return 0;
+  Arena ar{nullptr};
+  LinearGradPlan p;
+  return plan_linear_grad(w, dy, ldy, tokens, slope != 0, dx != 0, dbias != 0, nullptr, ar, &p) ? 0 : ar.used;
+}
+
+int zn_linear_grad(const zn_weight* w, const void* dy, int64_t ldy, int64_t tokens, const void* slope, void* dx,
+                   void* dbias, int32_t* status, void* temp, size_t temp_bytes, void* stream) {
+  if (!weight_ok(w) || !sizes_ok(tokens, ldy, w->rows) || !w->blob || (reinterpret_cast<uintptr_t>(w->blob) & 7) ||
+      !dy || !status || (!dx && !dbias))
+    return bad("zn_linear_grad");
+  NvtxScope range("zn_linear_grad");
+  Arena ar{static_cast<uint8_t*>(temp)};
+  LinearGradPlan p;
+  if (int rc = plan_linear_grad(w, dy, ldy, tokens, slope, dx, dbias, status, ar, &p)) return rc;
+  if (!temp || temp_bytes < ar.used) return set_error(ZN_ERR_SPACE, "zn_linear_grad: temp buffer too small");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return w->dtype == 8 ? run_linear_grad<__nv_bfloat16>(p, w, dy, ldy, tokens, slope, dx, dbias, s)
+                       : run_linear_grad<__half>(p, w, dy, ldy, tokens, slope, dx, dbias, s);
+}
+
+size_t zn_loss_state_bytes(int64_t tokens, int top) {
+  if (tokens <= 0 || top < 1 || top > kMaxTop) return 0;
+  size_t bytes = 0;
+  loss_state(nullptr, tokens, top, &bytes);
+  return bytes;
+}
+
+size_t zn_loss_temp_bytes(const zn_weight* w, const void* hidden, int64_t ldh, int64_t tokens) {
+  if (!loss_ok(w, tokens, ldh, 1, 1.0f, 0)) return 0;
+  Arena ar{nullptr};
+  LossPlan p;
+  return plan_loss(w, hidden, ldh, tokens, nullptr, ar, &p) ? 0 : ar.used;
+}
+
+int zn_loss(const zn_weight* w, const void* hidden, int64_t ldh, int64_t tokens, const int64_t* ids,
+            const float* logits, int top, int64_t ignore_index, float temperature, int reduction, float* loss,
+            void* state, int32_t* status, void* temp, size_t temp_bytes, void* stream) {
+  if (!loss_ok(w, tokens, ldh, top, temperature, reduction) || (!logits && top != 1) || !w->blob ||
+      (reinterpret_cast<uintptr_t>(w->blob) & 7) || !hidden || !ids || !loss || !state || !status)
+    return bad("zn_loss");
+  NvtxScope range("zn_loss");
+  Arena ar{static_cast<uint8_t*>(temp)};
+  LossPlan p;
+  if (int rc = plan_loss(w, hidden, ldh, tokens, status, ar, &p)) return rc;
+  if (!temp || temp_bytes < ar.used) return set_error(ZN_ERR_SPACE, "zn_loss: temp buffer too small");
+  const LossRows rows = loss_state(state, tokens, top, nullptr);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return w->dtype == 8 ? run_loss<__nv_bfloat16>(p, hidden, ldh, tokens, ids, logits, ignore_index, temperature,
+                                                 reduction, loss, rows, s)
+                       : run_loss<__half>(p, hidden, ldh, tokens, ids, logits, ignore_index, temperature, reduction,
+                                          loss, rows, s);
+}
+
+size_t zn_loss_grad_temp_bytes(const zn_weight* w, const void* hidden, int64_t ldh, int64_t tokens) {
+  if (!loss_ok(w, tokens, ldh, 1, 1.0f, 0)) return 0;
+  Arena ar{nullptr};
+  LossGradPlan p;
+  return plan_loss_grad(w, hidden, ldh, tokens, nullptr, ar, &p) ? 0 : ar.used;
+}
+
+int zn_loss_grad(const zn_weight* w, const void* hidden, int64_t ldh, int64_t tokens, int top, float temperature,
+                 int reduction, const void* state, const float* grad_loss, void* dhidden, int32_t* status, void* temp,
+                 size_t temp_bytes, void* stream) {
+  if (!loss_ok(w, tokens, ldh, top, temperature, reduction) || !w->blob ||
+      (reinterpret_cast<uintptr_t>(w->blob) & 7) || !hidden || !state || !grad_loss || !dhidden || !status)
+    return bad("zn_loss_grad");
+  NvtxScope range("zn_loss_grad");
+  Arena ar{static_cast<uint8_t*>(temp)};
+  LossGradPlan p;
+  if (int rc = plan_loss_grad(w, hidden, ldh, tokens, status, ar, &p)) return rc;
+  if (!temp || temp_bytes < ar.used) return set_error(ZN_ERR_SPACE, "zn_loss_grad: temp buffer too small");
+  const LossRows rows = loss_state(const_cast<void*>(state), tokens, top, nullptr);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return w->dtype == 8 ? run_loss_grad<__nv_bfloat16>(p, hidden, ldh, tokens, temperature, reduction, rows, grad_loss,
+                                                      dhidden, s)
+                       : run_loss_grad<__half>(p, hidden, ldh, tokens, temperature, reduction, rows, grad_loss,
+                                               dhidden, s);
+}
+
+}  // extern "C"

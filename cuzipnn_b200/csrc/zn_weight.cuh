@@ -1,0 +1,43 @@
+// A compressed weight as the operand of a product: a rows x cols matrix of 16-bit floats held as a
+// blob (the non-stored layout), decoded a range of chunks at a time into a caller's buffer, or
+// multiplied with a few vectors inside the decoder.  Implemented in zn_decode.cu.
+#pragma once
+
+#include "zn_common.cuh"
+
+namespace zn {
+
+struct WeightBlob {
+  const uint8_t* blob;
+  int64_t blob_bytes;
+  int64_t rows, cols;
+  int64_t chunk;  // elements per chunk
+  bool bf16;      // else fp16
+};
+
+// Rows of one product inside the decoder, and the shape rule of that path (see DotSink).
+constexpr int kDotRows = 8;
+inline bool dot_shape(int64_t tokens, int64_t cols, int64_t chunk) {
+  return tokens >= 1 && tokens <= kDotRows && cols % 16 == 0 && cols >= kRound && cols < (int64_t(1) << 30) &&
+         chunk % 16 == 0;
+}
+
+inline int64_t weight_chunks(const WeightBlob& w) { return cdiv(w.rows * w.cols, w.chunk); }
+// Scratch of one weight (unit offsets, overflow flags), filled by weight_scan.
+size_t weight_temp_bytes(const WeightBlob& w);
+// First step of every call: the offsets of the blob's units; sets the status word to 0 or errors.
+int weight_scan(const WeightBlob& w, void* temp, int32_t* status, cudaStream_t s);
+// Decode chunks [c0, c1) to `out` (the address of chunk c0's first element, 16-byte aligned).
+int weight_decode(const WeightBlob& w, void* temp, int64_t c0, int64_t c1, void* out, int32_t* status, cudaStream_t s);
+// Chunks that the decoder works on at once on this device (its resident blocks).
+int weight_wave(const WeightBlob& w, int64_t* chunks);
+
+// Product inside the decoder: z[t, r] = sum_c x[t, c] * W[r, c] for tokens <= kDotRows rows of x
+// (16-bit, 16-byte aligned, pitch ldx a multiple of 8).  Rows that lie in one chunk go to z (pitch
+// w.rows); the parts of rows that span chunks go to `part` ([chunk][2][kDotRows], dot_part_bytes):
+// slot 1 holds the part of a row that starts in the chunk, slot 0 of one that started before it.
+size_t dot_part_bytes(const WeightBlob& w);
+int weight_dot(const WeightBlob& w, void* temp, const void* x, int64_t ldx, int tokens, float* z, float* part,
+               int32_t* status, cudaStream_t s);
+
+}  // namespace zn

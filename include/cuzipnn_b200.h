@@ -155,6 +155,57 @@ int zn_decompress_batch(int njobs, const void *const *blobs, const int64_t *blob
                         int reorder, const int *ndim, const int64_t *chunk_bytes, const int64_t *n_comp,
                         void *const *out, int32_t *status, void *temp, size_t temp_bytes, void *stream);
 
+/* ---- operators on compressed weights ------------------------------------------------------- */
+
+/* No counterpart in the reference: products with a weight W [rows, cols] that stays a blob of
+ * zn_compress (2 dimensions, float16 or bfloat16).  A call decodes it a piece of rows at a time into
+ * its scratch; x, y and the other matrices are device memory of W's type, row-major, with a pitch
+ * (ld*) in elements between rows.  `status` is a device int32: 0, then the OR of the decoding errors
+ * (as zn_decompress) and of 16 when a bounded wait inside a kernel gave up.  The *_temp_bytes
+ * queries give the scratch on the current device (0: bad arguments); pass the same matrix pointer
+ * and pitch as to the call (an unaligned one needs room for a copy). */
+typedef struct {
+  const void *blob;    /* device, 8-byte aligned, blob_bytes long */
+  int64_t blob_bytes;
+  int64_t rows, cols;
+  int64_t chunk_bytes; /* the header's chunk_bytes; 0 for a stored blob */
+  int dtype;           /* the header's dtype code: 7 float16, 8 bfloat16 */
+} zn_weight;
+
+/* y [tokens, rows] (contiguous) = act(x W^T + bias) + residual.  activation: 0 none, 1 relu, 2 gelu
+ * (erf), 3 gelu (tanh), 4 silu.  bias, residual and slope may be NULL; slope (as y) gets act'(z),
+ * which zn_linear_grad takes. */
+size_t zn_linear_temp_bytes(const zn_weight *w, const void *x, int64_t ldx, int64_t tokens);
+int zn_linear(const zn_weight *w, const void *x, int64_t ldx, int64_t tokens, const void *bias, int activation,
+              const void *residual, int64_t ldr, void *y, void *slope, int32_t *status, void *temp,
+              size_t temp_bytes, void *stream);
+/* dx [tokens, cols] = (dy * slope) W and dbias [rows] = column sums of dy * slope (slope NULL: 1;
+ * dx or dbias may be NULL). */
+size_t zn_linear_grad_temp_bytes(const zn_weight *w, const void *dy, int64_t ldy, int64_t tokens, int slope, int dx,
+                                 int dbias);
+int zn_linear_grad(const zn_weight *w, const void *dy, int64_t ldy, int64_t tokens, const void *slope, void *dx,
+                   void *dbias, int32_t *status, void *temp, size_t temp_bytes, void *stream);
+
+/* Losses over the logits s = hidden W^T / temperature, which are never kept.
+ * logits NULL (top = 1): cross entropy with the target ids[m] (ignore_index: the row does not
+ * count).  Else ids and logits are [tokens, top] (top <= 256), the teacher's best ids and their
+ * logits (an id < 0: no entry), q = softmax(logits / temperature) over them, and a row's loss is
+ * temperature^2 * KL(q || softmax(s)).  A row without entries, or whose logits are all -inf, does not
+ * count; a row with an id >= rows (or a negative target other than ignore_index) has loss and
+ * gradient NaN.  reduction: 0 the mean of the rows that count (0 if none does), 1 their sum, 2 one
+ * loss per row (0 where it does not count).  `state` (zn_loss_state_bytes) is filled for
+ * zn_loss_grad, which computes the logits again: dhidden [tokens, cols], with grad_loss one float
+ * (one per row for reduction 2). */
+size_t zn_loss_state_bytes(int64_t tokens, int top);
+size_t zn_loss_temp_bytes(const zn_weight *w, const void *hidden, int64_t ldh, int64_t tokens);
+int zn_loss(const zn_weight *w, const void *hidden, int64_t ldh, int64_t tokens, const int64_t *ids,
+            const float *logits, int top, int64_t ignore_index, float temperature, int reduction, float *loss,
+            void *state, int32_t *status, void *temp, size_t temp_bytes, void *stream);
+size_t zn_loss_grad_temp_bytes(const zn_weight *w, const void *hidden, int64_t ldh, int64_t tokens);
+int zn_loss_grad(const zn_weight *w, const void *hidden, int64_t ldh, int64_t tokens, int top, float temperature,
+                 int reduction, const void *state, const float *grad_loss, void *dhidden, int32_t *status, void *temp,
+                 size_t temp_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
