@@ -139,7 +139,7 @@ def _ptr(t: torch.Tensor | None) -> int | None:
 def _linear_forward(w: _Weight, x, bias, act: int, residual, want_slope: bool, status):
     shape = (*x.shape[:-1], w.rows)
     y = torch.empty(shape, dtype=w.dtype, device=w.device)
-    slope = torch.empty_like(y) if want_slope else None
+    slope = torch.empty(shape, dtype=torch.int16, device=w.device) if want_slope else None
     x2, ldx = _rows(x, w.cols)
     r2, ldr = (None, 0) if residual is None else _rows(residual, w.rows)
     b = None if bias is None else bias.detach().contiguous()
@@ -196,7 +196,7 @@ def blob_linear(
     "silu".  Products are summed in 32 bits and the result is rounded once.
 
     Differentiable in x, bias and residual (the weight is frozen).  With an activation the forward
-    pass keeps its derivative, rounded to the dtype, for the backward pass; the weight is decoded
+    pass keeps its derivative, in 16-bit fixed point of step 2^-14, for the backward pass; the weight is decoded
     again there."""
     if activation not in _ACTIVATIONS:
         raise ValueError(f"activation must be one of {sorted(map(str, _ACTIVATIONS))}, not {activation!r}")

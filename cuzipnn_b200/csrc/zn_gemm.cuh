@@ -5,14 +5,17 @@
 // rows, as in x W^T) or row-major [K, N] (BMN = true: the contraction runs down its columns, as in
 // dz W), so a decoded weight serves both directions as it lies in memory.
 //
-// One persistent CTA per SM takes output tiles of 128 x BN in turn.  Warp 0 loads 64-wide blocks of
-// both operands with TMA (128-byte swizzle) into a ring of shared-memory stages, one thread of warp
-// 1 issues tcgen05.mma into one of two accumulators in tensor memory, and warps 4-7 read the other
-// accumulator (a thread owns a row of the tile) and run the epilogue meanwhile.
+// Persistent CTAs (CG = 1) or pairs of CTAs on neighbouring SMs (CG = 2) take output tiles in turn:
+// 128 x 128 for one CTA, 256 x 256 for a pair, where each CTA loads its half of both operands and
+// holds its 128 rows of the result, so that a byte loaded is used twice as often.  Warp 0 loads
+// 64-wide blocks with TMA (128-byte swizzle) into a ring of shared-memory stages, one thread of warp
+// 1 (of the pair's first CTA) issues tcgen05.mma into one of two accumulators in tensor memory, and
+// warps 4-7 read the other accumulator (a thread owns a row of the tile) and run the epilogue
+// meanwhile.
 //
 // Every wait has an iteration limit.  A wait that gives up sets kErrWait in the status word and the
 // abort flag, upon which all warps leave their loops, the loads in flight are waited for (again
-// with a limit) and the tensor memory is freed.
+// with a limit) and the tensor memory is freed; the other CTA of a pair runs into its own limits.
 #pragma once
 
 #include <cuda.h>
@@ -25,7 +28,7 @@ namespace zn {
 
 constexpr int32_t kErrWait = 16;  // a bounded wait inside a product kernel gave up
 
-constexpr int kBM = 128;          // rows of a tile (tensor memory lanes)
+constexpr int kBM = 128;          // rows of a tile per CTA (tensor memory lanes)
 constexpr int kBK = 64;           // contraction block: 128 bytes of a 16-bit type, one swizzle row
 constexpr int kGemmThreads = 256;
 constexpr uint32_t kWaitLimit = 1u << 24;  // polls of up to kPollNs each (about 4 s at most)
@@ -69,19 +72,82 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
   *abort_flag = 1;
   return false;
 }
+__device__ __forceinline__ uint32_t cta_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+// The same shared address in the pair's first CTA.
+__device__ __forceinline__ uint32_t in_leader(uint32_t addr) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+  return r;
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void group_sync() {
+  if constexpr (CG == 2) {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  } else {
+    __syncthreads();
+  }
+}
+// With CG = 2 the barrier may lie in the other CTA of the pair.
+template <int CG>
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-      ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+  if constexpr (CG == 2) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3}], [%4];"
+        ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+  } else {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+        ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+  }
 }
+// Arrive on the barrier (of both CTAs of a pair) when the MMAs issued so far have ended.
+template <int CG>
 __device__ __forceinline__ void tc_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+  if constexpr (CG == 2) {
+    asm volatile(
+        "{\n .reg .b16 m;\n mov.b16 m, 3;\n"
+        " tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], m;\n}\n"
+        ::"r"(bar) : "memory");
+  } else {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+  }
 }
+template <int CG>
 __device__ __forceinline__ void tc_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n"
-      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+  if constexpr (CG == 2) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+  } else {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+  }
+}
+template <int CG, int COLS>
+__device__ __forceinline__ void tmem_alloc(uint32_t dst) {
+  if constexpr (CG == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst), "n"(COLS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst), "n"(COLS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+}
+template <int CG, int COLS>
+__device__ __forceinline__ void tmem_free(uint32_t addr) {
+  if constexpr (CG == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "n"(COLS));
+  else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "n"(COLS));
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -142,39 +208,44 @@ struct Num<__half> {
   static __device__ __forceinline__ __half from(float v) { return __float2half_rn(v); }
 };
 
-// Instruction descriptor: f32 accumulator, 16-bit operands of one type, B's major-ness, N and M.
-template <typename T, int BN, bool BMN>
-__device__ constexpr uint32_t instr_desc() {
-  return (1u << 4) | (Num<T>::kCode << 7) | (Num<T>::kCode << 10) | (uint32_t(BMN) << 16) | (uint32_t(BN / 8) << 17) |
-         (uint32_t(kBM / 16) << 24);
-}
-
-template <int BN>
+// A tile of CG CTAs: 128 CG x 128 CG.
+template <int CG>
 struct GemmCfg {
-  static constexpr int kStageBytes = (kBM + BN) * kBK * 2;
-  static constexpr int kStages = 196608 / kStageBytes;
-  static constexpr int kSmem = kStages * kStageBytes + 1024;  // + alignment of the first stage
+  static constexpr int kBN = 128 * CG;
+  static constexpr int kOperand = 128 * kBK * 2;  // bytes of A, and of B, that a CTA holds per stage
+  static constexpr int kStageBytes = 2 * kOperand;
+  static constexpr int kStages = 5;
+  static constexpr int kWarpBuf = 4096;  // per epilogue warp, to turn rows into whole sectors
+  static constexpr int kSmem = kStages * kStageBytes + 4 * kWarpBuf + 1024;  // + alignment of the first stage
 };
 
-// Epilogue interface: Epi::Row row(epi, m, n0, split) at the start of a thread's tile row (m may be
-// past the last row: nothing may be accessed then), row.cols(epi, c, v) for each 32 columns
-// n0 + c .. n0 + c + 31, row.end(epi) after the last.
-template <typename T, int BN, bool BMN, class Epi>
+// Instruction descriptor: f32 accumulator, 16-bit operands of one type, B's major-ness, N and M.
+template <typename T, int CG, bool BMN>
+__device__ constexpr uint32_t instr_desc() {
+  return (1u << 4) | (Num<T>::kCode << 7) | (Num<T>::kCode << 10) | (uint32_t(BMN) << 16) |
+         (uint32_t(GemmCfg<CG>::kBN / 8) << 17) | (uint32_t(kBM * CG / 16) << 24);
+}
+
+// Epilogue interface.  Epi::Row row(epi, m, n0, split, buf) at the start of a thread's tile row (the
+// warp holds rows m - lane .. m - lane + 31; m may be past the last row: nothing may be accessed
+// then), row.cols(epi, c, v) for each 32 columns n0 + c .. n0 + c + 31, by whole warps, row.end(epi)
+// after the last.  buf: kWarpBuf bytes of the warp's own shared memory.
+template <typename T, int CG, bool BMN, class Epi>
 __global__ void __launch_bounds__(kGemmThreads, 1)
 gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
             const __grid_constant__ GemmShape g, const __grid_constant__ Epi epi) {
-  using Cfg = GemmCfg<BN>;
-  constexpr int kStages = Cfg::kStages;
-  constexpr uint32_t kIdesc = instr_desc<T, BN, BMN>();
+  using Cfg = GemmCfg<CG>;
+  constexpr int kStages = Cfg::kStages, BN = Cfg::kBN;
+  constexpr uint32_t kIdesc = instr_desc<T, CG, BMN>();
   extern __shared__ uint8_t smem_dyn[];
   __shared__ __align__(8) uint64_t bars[2 * kStages + 5];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
   const uint32_t stage0 = (smem_addr(smem_dyn) + 1023) & ~1023u;
   const uint32_t full0 = smem_addr(bars), empty0 = full0 + 8 * kStages;
-  const uint32_t accfull0 = empty0 + 8 * kStages, accempty0 = accfull0 + 16,
-                 drain = accempty0 + 16;
+  const uint32_t accfull0 = empty0 + 8 * kStages, accempty0 = accfull0 + 16, drain = accempty0 + 16;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = CG == 2 ? cta_rank() : 0;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
@@ -183,25 +254,23 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(accfull0 + 8 * i, 1);
-      mbar_init(accempty0 + 8 * i, 128);
+      mbar_init(accempty0 + 8 * i, 4 * CG);  // one arrival per epilogue warp
     }
     mbar_init(drain, 1);
     s_abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
-  if (warp == 2) {  // both accumulators: 2 * BN columns
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s_tmem)),
-                 "n"(2 * BN) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
+  if (warp == 2) tmem_alloc<CG, 2 * BN>(smem_addr(&s_tmem));  // both accumulators
   tc_fence_before();
   __syncthreads();
+  if constexpr (CG == 2) group_sync<2>();
   tc_fence_after();
   const uint32_t tmem = s_tmem;
   volatile int* abort_flag = &s_abort;
 
   const int64_t total = int64_t(g.tiles_m) * g.tiles_n * g.splits;
+  const int64_t first = blockIdx.x / CG, step = gridDim.x / CG;
   // Tile order: within a group of row tiles, the row tile runs fastest, then the column tile, so
   // that the CTAs of one wave share a few column blocks of B and a group's rows of A in L2.
   auto tile_of = [&](int64_t t, int& tm, int& tn, int& ks) {
@@ -223,25 +292,27 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     if (lane == 0) {
       int64_t it = 0;  // blocks loaded
       bool ok = true;
-      for (int64_t t = blockIdx.x; t < total && ok; t += gridDim.x) {
+      for (int64_t t = first; t < total && ok; t += step) {
         int tm, tn, ks, kb0, kb1;
         tile_of(t, tm, tn, ks);
         k_range(ks, kb0, kb1);
+        const int ya = (tm * CG + int(rank)) * kBM, yb = tn * BN + int(rank) * 128;
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const int s = int(it % kStages);
           if (it >= kStages && !mbar_wait(empty0 + 8 * s, uint32_t((it / kStages - 1) & 1), abort_flag)) {
             ok = false;
             break;
           }
-          const uint32_t a = stage0 + s * Cfg::kStageBytes, b = a + kBM * kBK * 2, bar = full0 + 8 * s;
-          mbar_expect(bar, Cfg::kStageBytes);
-          tma_load(a, &map_a, kb * kBK, tm * kBM, bar);
+          const uint32_t a = stage0 + s * Cfg::kStageBytes, b = a + Cfg::kOperand;
+          // The first CTA's barrier counts the bytes of both.
+          if (rank == 0) mbar_expect(full0 + 8 * s, CG * Cfg::kStageBytes);
+          const uint32_t bar = CG == 2 ? in_leader(full0 + 8 * s) : full0 + 8 * s;
+          tma_load<CG>(a, &map_a, kb * kBK, ya, bar);
           if constexpr (!BMN) {
-            tma_load(b, &map_b, kb * kBK, tn * BN, bar);
+            tma_load<CG>(b, &map_b, kb * kBK, yb, bar);
           } else {
-#pragma unroll
-            for (int i = 0; i < BN / 64; ++i)
-              tma_load(b + i * (kBK * 128), &map_b, tn * BN + 64 * i, kb * kBK, bar);
+            tma_load<CG>(b, &map_b, yb, kb * kBK, bar);
+            tma_load<CG>(b + kBK * 128, &map_b, yb + 64, kb * kBK, bar);
           }
         }
       }
@@ -250,21 +321,24 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
       for (int64_t j = it > kStages ? it - kStages : 0; j < it; ++j) {
         const int s = int(j % kStages);
         if (ok) ok = mbar_wait(empty0 + 8 * s, uint32_t((j / kStages) & 1), abort_flag);
-        if (!ok)
+        if (!ok && rank == 0)
           for (uint32_t i = 0; i < kWaitLimit && !mbar_try(full0 + 8 * s, uint32_t((j / kStages) & 1)); ++i) {}
       }
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (lane == 0 && rank == 0) {
       int64_t it = 0, n = 0;  // blocks consumed, tiles done
       bool ok = true;
-      for (int64_t t = blockIdx.x; t < total && ok; t += gridDim.x, ++n) {
+      for (int64_t t = first; t < total && ok; t += step, ++n) {
         int tm, tn, ks, kb0, kb1;
         tile_of(t, tm, tn, ks);
         k_range(ks, kb0, kb1);
         const int acc = int(n & 1);
-        if (n >= 2 && !mbar_wait(accempty0 + 8 * acc, uint32_t((n / 2 - 1) & 1), abort_flag)) break;
+        if (n >= 2 && !mbar_wait(accempty0 + 8 * acc, uint32_t((n / 2 - 1) & 1), abort_flag)) {
+          ok = false;
+          break;
+        }
         tc_fence_after();
         const uint32_t d = tmem + acc * BN;
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
@@ -274,26 +348,27 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             break;
           }
           tc_fence_after();
-          const uint32_t a = stage0 + s * Cfg::kStageBytes, b = a + kBM * kBK * 2;
+          const uint32_t a = stage0 + s * Cfg::kStageBytes, b = a + Cfg::kOperand;
           const uint64_t da = desc_kmajor(a), db = BMN ? desc_mnmajor(b) : desc_kmajor(b);
 #pragma unroll
           for (int k = 0; k < kBK / 16; ++k)
-            tc_mma(d, da + uint64_t(k * 2), db + uint64_t(BMN ? k * (2048 >> 4) : k * 2), kIdesc,
-                   uint32_t(kb > kb0 || k > 0));
-          tc_commit(empty0 + 8 * s);
+            tc_mma<CG>(d, da + uint64_t(k * 2), db + uint64_t(BMN ? k * (2048 >> 4) : k * 2), kIdesc,
+                       uint32_t(kb > kb0 || k > 0));
+          tc_commit<CG>(empty0 + 8 * s);
         }
-        if (ok) tc_commit(accfull0 + 8 * acc);
+        if (ok) tc_commit<CG>(accfull0 + 8 * acc);
       }
-      if (!ok || *abort_flag) {  // MMAs in flight end before the tensor memory is freed
-        tc_commit(drain);
+      if (!ok) {  // MMAs in flight end before the tensor memory is freed
+        tc_commit<CG>(drain);
         for (uint32_t i = 0; i < kWaitLimit && !mbar_try(drain, 0); ++i) {}
       }
     }
     __syncwarp();
   } else if (warp >= 4) {
     const int quarter = warp & 3;
+    uint8_t* buf = smem_dyn + (stage0 - smem_addr(smem_dyn)) + kStages * Cfg::kStageBytes + quarter * Cfg::kWarpBuf;
     int64_t n = 0;
-    for (int64_t t = blockIdx.x; t < total; t += gridDim.x, ++n) {
+    for (int64_t t = first; t < total; t += step, ++n) {
       int tm, tn, ks;
       tile_of(t, tm, tn, ks);
       const int acc = int(n & 1);
@@ -301,7 +376,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
       if (!__all_sync(0xFFFFFFFFu, ok)) break;
       tc_fence_after();
       const uint32_t src = tmem + (uint32_t(quarter * 32) << 16) + acc * BN;
-      typename Epi::Row row(epi, int64_t(tm) * kBM + quarter * 32 + lane, int64_t(tn) * BN, ks);
+      typename Epi::Row row(epi, (int64_t(tm) * CG + rank) * kBM + quarter * 32 + lane, int64_t(tn) * BN, ks, buf);
 #pragma unroll 1
       for (int c = 0; c < BN; c += 32) {
         float v[32];
@@ -309,7 +384,11 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         tc_wait_load();
         if (c + 32 >= BN) {  // the accumulator is read: hand it back before the last columns' work
           tc_fence_before();
-          mbar_arrive(accempty0 + 8 * acc);
+          __syncwarp();
+          if (lane == 0) {
+            if constexpr (CG == 2) mbar_arrive_cluster(in_leader(accempty0 + 8 * acc));
+            else mbar_arrive(accempty0 + 8 * acc);
+          }
         }
         row.cols(epi, c, v);
       }
@@ -318,9 +397,9 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
   }
   tc_fence_before();
   __syncthreads();
+  if constexpr (CG == 2) group_sync<2>();
   tc_fence_after();
-  if (warp == 2)
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(2 * BN));
+  if (warp == 2) tmem_free<CG, 2 * BN>(tmem);
   if (threadIdx.x == 0 && s_abort) atomicOr(g.status, kErrWait);
 }
 
@@ -331,30 +410,41 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
 int make_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t pitch, int box_rows, bool bf16);
 int sm_count(int* sms);
 
-inline GemmShape gemm_shape(int64_t M, int64_t N, int64_t K, int BN, int32_t* status) {
+inline GemmShape gemm_shape(int64_t M, int64_t N, int64_t K, int cg, int32_t* status) {
   GemmShape g{};
   g.M = M;
   g.N = N;
   g.K = K;
-  g.tiles_m = int(cdiv(M, kBM));
-  g.tiles_n = int(cdiv(N, BN));
+  g.tiles_m = int(cdiv(M, kBM * cg));
+  g.tiles_n = int(cdiv(N, 128 * cg));
   g.kblocks = int(cdiv(K, kBK));
   g.splits = 1;
-  g.group_m = 32;
+  g.group_m = 32 / cg;
   g.status = status;
   return g;
 }
 
-template <typename T, int BN, bool BMN, class Epi>
+template <typename T, int CG, bool BMN, class Epi>
 int launch_gemm(const CUtensorMap& a, const CUtensorMap& b, const GemmShape& g, const Epi& epi, cudaStream_t s) {
-  auto fn = gemm_kernel<T, BN, BMN, Epi>;
-  if (int rc = set_max_smem(reinterpret_cast<const void*>(fn), GemmCfg<BN>::kSmem)) return rc;
+  auto fn = gemm_kernel<T, CG, BMN, Epi>;
+  if (int rc = set_max_smem(reinterpret_cast<const void*>(fn), GemmCfg<CG>::kSmem)) return rc;
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
   const int64_t total = int64_t(g.tiles_m) * g.tiles_n * g.splits;
   if (total <= 0) return ZN_OK;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(CG * (total < sms / CG ? total : sms / CG)));
+  cfg.blockDim = dim3(kGemmThreads);
+  cfg.dynamicSmemBytes = GemmCfg<CG>::kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = CG;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = CG > 1 ? 1 : 0;
   TimedLaunch tl("gemm", s);
-  fn<<<unsigned(total < sms ? total : sms), kGemmThreads, GemmCfg<BN>::kSmem, s>>>(a, b, g, epi);
+  cudaLaunchKernelEx(&cfg, fn, a, b, g, epi);
   count_launch();
   return check_launch("gemm_kernel");
 }

@@ -61,100 +61,160 @@ constexpr int kMaxTop = 256;
 // ---- epilogues ------------------------------------------------------------------------------
 
 // act(z) and its derivative (where asked for), in 32 bits.
+template <int ACT, bool SLOPE>
+__device__ __forceinline__ float activate(float z, float& slope) {
+  if constexpr (ACT == kRelu) {
+    if (SLOPE) slope = z > 0.0f ? 1.0f : 0.0f;
+    return z < 0.0f ? 0.0f : z;  // keeps NaN
+  } else if constexpr (ACT == kGelu) {
+    const float cdf = 0.5f * erfcf(-0.70710678118654752f * z);
+    if (SLOPE) slope = cdf + z * 0.3989422804014327f * __expf(-0.5f * z * z);
+    return z * cdf;
+  } else if constexpr (ACT == kGeluTanh) {  // 0.5 z (1 + tanh u) = z sigmoid(2u)
+    const float c = 0.7978845608028654f, z2 = z * z;
+    const float sig = __fdividef(1.0f, 1.0f + __expf(-2.0f * c * z * (1.0f + 0.044715f * z2)));
+    if (SLOPE) slope = sig + z * sig * (1.0f - sig) * 2.0f * c * (1.0f + 3.0f * 0.044715f * z2);
+    return z * sig;
+  } else if constexpr (ACT == kSilu) {
+    const float sig = __fdividef(1.0f, 1.0f + __expf(-z));
+    if (SLOPE) slope = sig * (1.0f + z * (1.0f - sig));
+    return z * sig;
+  } else {
+    if (SLOPE) slope = 1.0f;
+    return z;
+  }
+}
 template <bool SLOPE>
 __device__ __forceinline__ float activate(int act, float z, float& slope) {
   switch (act) {
-    case kRelu:
-      if (SLOPE) slope = z > 0.0f ? 1.0f : 0.0f;
-      return z < 0.0f ? 0.0f : z;  // keeps NaN
-    case kGelu: {
-      const float cdf = 0.5f * erfcf(-0.70710678118654752f * z);
-      if (SLOPE) slope = cdf + z * 0.3989422804014327f * __expf(-0.5f * z * z);
-      return z * cdf;
-    }
-    case kGeluTanh: {  // 0.5 z (1 + tanh u) = z sigmoid(2u)
-      const float c = 0.7978845608028654f, z2 = z * z;
-      const float sig = 1.0f / (1.0f + __expf(-2.0f * c * z * (1.0f + 0.044715f * z2)));
-      if (SLOPE) slope = sig + z * sig * (1.0f - sig) * 2.0f * c * (1.0f + 3.0f * 0.044715f * z2);
-      return z * sig;
-    }
-    case kSilu: {
-      const float sig = 1.0f / (1.0f + __expf(-z));
-      if (SLOPE) slope = sig * (1.0f + z * (1.0f - sig));
-      return z * sig;
-    }
-    default:
-      if (SLOPE) slope = 1.0f;
-      return z;
+    case kRelu: return activate<kRelu, SLOPE>(z, slope);
+    case kGelu: return activate<kGelu, SLOPE>(z, slope);
+    case kGeluTanh: return activate<kGeluTanh, SLOPE>(z, slope);
+    case kSilu: return activate<kSilu, SLOPE>(z, slope);
+    default: return activate<kNone, SLOPE>(z, slope);
   }
 }
 
-// y = act(acc + bias) + residual, rounded once to 16 bits; the slope act'(z), which the backward
-// pass multiplies with, is rounded to 16 bits too (it is of order one, so its rounding is that of
-// the gradient it scales).
+// The derivative act'(z), kept for the backward pass as a 16-bit fixed-point number of step 2^-14
+// (every activation's lies in [-0.13, 1.13]): off by 2^-15 of a whole slope at most, an eighth of
+// a bf16 rounding, so the gradients are as exact as with a 32-bit slope.  -32768 stands for NaN.
+__device__ __forceinline__ int slope_code(float s) { return s != s ? -32768 : __float2int_rn(s * 16384.0f); }
+__device__ __forceinline__ float slope_value(int code) { return code == -32768 ? NAN : float(code) * (1.0f / 16384.0f); }
+
+// Per-warp staging: a thread holds 64 bytes (32 16-bit columns) of its own row; through shared
+// memory the warp writes them as 8 rows x 64 contiguous bytes per store.  The 16-byte chunks of a
+// row are permuted by the row, so that both sides touch every bank once.
+__device__ __forceinline__ uint4* stage_at(uint8_t* buf, int row, int chunk) {
+  return reinterpret_cast<uint4*>(buf + row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4));
+}
+// Rows m0 + r < M, columns n0 .. n0 + 31 < N of a 16-bit matrix from the warp's 16 words per thread.
+template <typename T>
+__device__ __forceinline__ void stage_rows(uint8_t* buf, const uint32_t* w, T* out, int64_t ld, int64_t m0, int64_t M,
+                                           int64_t n0, int64_t N, bool vec) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) *stage_at(buf, lane, i) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+  __syncwarp();
+  if (vec) {  // 16-byte aligned rows, N a multiple of 8
+    const int64_t n = n0 + 8 * (lane & 3);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = 8 * i + (lane >> 2);
+      if (m0 + r < M && n < N) *reinterpret_cast<uint4*>(out + (m0 + r) * ld + n) = *stage_at(buf, r, lane & 3);
+    }
+  } else if (n0 + lane < N) {
+    const int rows = int(min(int64_t(32), M - m0));
+    for (int r = 0; r < rows; ++r)
+      out[(m0 + r) * ld + n0 + lane] = reinterpret_cast<const T*>(stage_at(buf, r, lane >> 3))[lane & 7];
+  }
+  __syncwarp();
+}
+
+// y = act(acc + bias) + residual, rounded once to 16 bits, and (where asked for) the slopes.
 template <typename T>
 struct EpiLinear {
   const T* bias;  // or null
   const T* res;   // or null
   T* y;
-  T* slope;  // or null
+  int16_t* slope;  // or null
   int64_t ldr, ldy, M, N;
   int act;
-  bool vec;  // 16-byte accesses: every pointer and pitch allows them
-
-  __device__ __forceinline__ float2 pair(float a, float b, float2& sl) const {
-    if (slope) return make_float2(activate<true>(act, a, sl.x), activate<true>(act, b, sl.y));
-    return make_float2(activate<false>(act, a, sl.x), activate<false>(act, b, sl.y));
-  }
+  bool vec;  // 16-byte accesses: every pointer and pitch allows them, and N is a multiple of 8
 
   struct Row {
     int64_t m, n0;
-    __device__ __forceinline__ Row(const EpiLinear&, int64_t m_, int64_t n0_, int) : m(m_), n0(n0_) {}
-    __device__ __forceinline__ void cols(const EpiLinear& e, int c, const float* v) {
-      if (m >= e.M) return;
+    uint8_t* buf;
+    __device__ __forceinline__ Row(const EpiLinear&, int64_t m_, int64_t n0_, int, uint8_t* b) : m(m_), n0(n0_), buf(b) {}
+
+    template <int ACT, bool SLOPE>
+    __device__ __forceinline__ void run(const EpiLinear& e, int64_t n, float* v) {
+      uint32_t sw[16];
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int64_t n = n0 + c + 8 * g;
-        const float* w = v + 8 * g;
-        if (e.vec && n + 8 <= e.N) {
-          uint32_t bw[4] = {}, rw[4] = {}, yw[4], sw[4];
-          if (e.bias) load16(e.bias + n, bw);
-          if (e.res) load16(e.res + m * e.ldr + n, rw);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float2 sl;
-            float2 z = make_float2(w[2 * i], w[2 * i + 1]);
-            if (e.bias) z = make_float2(z.x + Num<T>::lo(bw[i]), z.y + Num<T>::hi(bw[i]));
-            z = e.pair(z.x, z.y, sl);
-            if (e.res) z = make_float2(z.x + Num<T>::lo(rw[i]), z.y + Num<T>::hi(rw[i]));
-            yw[i] = Num<T>::pack(z.x, z.y);
-            if (e.slope) sw[i] = Num<T>::pack(sl.x, sl.y);
-          }
-          *reinterpret_cast<uint4*>(e.y + m * e.ldy + n) = make_uint4(yw[0], yw[1], yw[2], yw[3]);
-          if (e.slope) *reinterpret_cast<uint4*>(e.slope + m * e.ldy + n) = make_uint4(sw[0], sw[1], sw[2], sw[3]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (n + i < e.N) {
-              float sl, z = w[i] + (e.bias ? Num<T>::to(e.bias[n + i]) : 0.0f);
-              z = e.slope ? activate<true>(e.act, z, sl) : activate<false>(e.act, z, sl);
-              if (e.res) z += Num<T>::to(e.res[m * e.ldr + n + i]);
-              e.y[m * e.ldy + n + i] = Num<T>::from(z);
-              if (e.slope) e.slope[m * e.ldy + n + i] = Num<T>::from(sl);
-            }
+      for (int i = 0; i < 16; ++i) {
+        float s0, s1;
+        v[2 * i] = activate<ACT, SLOPE>(v[2 * i], s0);
+        v[2 * i + 1] = activate<ACT, SLOPE>(v[2 * i + 1], s1);
+        if (SLOPE) sw[i] = (uint32_t(slope_code(s0)) & 0xFFFFu) | (uint32_t(slope_code(s1)) << 16);
+      }
+      if (SLOPE) stage_rows(buf, sw, e.slope, e.ldy, m - (threadIdx.x & 31), e.M, n, e.N, e.vec);
+    }
+
+    __device__ __forceinline__ void cols(const EpiLinear& e, int c, float* v) {
+      const int64_t n = n0 + c;
+      if (n >= e.N) return;
+      if (e.bias) add(e.bias, n, e, v);
+      if (e.slope) {
+        switch (e.act) {
+          case kRelu: run<kRelu, true>(e, n, v); break;
+          case kGelu: run<kGelu, true>(e, n, v); break;
+          case kGeluTanh: run<kGeluTanh, true>(e, n, v); break;
+          case kSilu: run<kSilu, true>(e, n, v); break;
+          default: run<kNone, true>(e, n, v);
+        }
+      } else {
+        switch (e.act) {
+          case kRelu: run<kRelu, false>(e, n, v); break;
+          case kGelu: run<kGelu, false>(e, n, v); break;
+          case kGeluTanh: run<kGeluTanh, false>(e, n, v); break;
+          case kSilu: run<kSilu, false>(e, n, v); break;
+          default: break;
         }
       }
+      if (e.res && m < e.M) add(e.res + m * e.ldr, n, e, v);
+      uint32_t w[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) w[i] = Num<T>::pack(v[2 * i], v[2 * i + 1]);
+      stage_rows(buf, w, e.y, e.ldy, m - (threadIdx.x & 31), e.M, n, e.N, e.vec);
     }
     __device__ __forceinline__ void end(const EpiLinear&) {}
-    static __device__ __forceinline__ void load16(const T* p, uint32_t* w) {
-      const uint4 q = *reinterpret_cast<const uint4*>(p);
-      w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w;
+
+    // v += row[n .. n + 31], as far as the columns go.
+    static __device__ __forceinline__ void add(const T* row, int64_t n, const EpiLinear& e, float* v) {
+      if (e.vec) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          if (n + 8 * g >= e.N) break;
+          const uint4 q = *reinterpret_cast<const uint4*>(row + n + 8 * g);
+          const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            v[8 * g + 2 * i] += Num<T>::lo(w[i]);
+            v[8 * g + 2 * i + 1] += Num<T>::hi(w[i]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (n + i < e.N) v[i] += Num<T>::to(row[n + i]);
+      }
     }
   };
 };
 
 // acc[split][m][n] (32 bits) = or += the tile: the parts of a contraction that is cut, across the
 // CTAs of one product or across the pieces of a weight.  finish_kernel adds the splits in order.
+// A thread's 128 bytes per 32 columns go through the staging buffer, so that the warp reads and
+// writes 4 rows of whole 128-byte lines at a time.
 struct EpiAccum {
   float* acc;
   int64_t M, N, ld;  // ld: a multiple of 4
@@ -162,21 +222,35 @@ struct EpiAccum {
   struct Row {
     int64_t m, n0;
     float* p;
-    __device__ __forceinline__ Row(const EpiAccum& e, int64_t m_, int64_t n0_, int split)
-        : m(m_), n0(n0_), p(e.acc + (int64_t(split) * e.M + m_) * e.ld + n0_) {}
+    uint8_t* buf;
+    __device__ __forceinline__ Row(const EpiAccum& e, int64_t m_, int64_t n0_, int split, uint8_t* b)
+        : m(m_), n0(n0_), p(e.acc + int64_t(split) * e.M * e.ld), buf(b) {}
+    __device__ __forceinline__ float4* at(int row, int chunk) const {
+      return reinterpret_cast<float4*>(buf + row * 128 + ((chunk ^ (row & 7)) << 4));
+    }
     __device__ __forceinline__ void cols(const EpiAccum& e, int c, const float* v) {
-      if (m >= e.M) return;
+      const int lane = threadIdx.x & 31;
+      if (n0 + c >= e.N) return;
 #pragma unroll
-      for (int g = 0; g < 8; ++g) {
-        if (n0 + c + 4 * g >= e.N) break;  // the pitch covers the last group of 4
-        float4* q = reinterpret_cast<float4*>(p + c + 4 * g);
-        float4 s = make_float4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
-        if (e.add) {
-          const float4 o = *q;
-          s = make_float4(s.x + o.x, s.y + o.y, s.z + o.z, s.w + o.w);
+      for (int g = 0; g < 8; ++g) *at(lane, g) = make_float4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
+      __syncwarp();
+      const int64_t n = n0 + c + 4 * (lane & 7), m0 = m - lane;
+      float4 s[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = 4 * i + (lane >> 3);
+        s[i] = *at(r, lane & 7);
+        if (e.add && m0 + r < e.M && n < e.N) {
+          const float4 o = *reinterpret_cast<const float4*>(p + (m0 + r) * e.ld + n);
+          s[i] = make_float4(s[i].x + o.x, s[i].y + o.y, s[i].z + o.z, s[i].w + o.w);
         }
-        *q = s;
       }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = 4 * i + (lane >> 3);
+        if (m0 + r < e.M && n < e.N) *reinterpret_cast<float4*>(p + (m0 + r) * e.ld + n) = s[i];
+      }
+      __syncwarp();
     }
     __device__ __forceinline__ void end(const EpiAccum&) {}
   };
@@ -232,7 +306,7 @@ struct EpiStats {
     const float* q;
     int at, count;
     int64_t next;  // column (of the piece) of the next id
-    __device__ __forceinline__ Row(const EpiStats& e, int64_t m_, int64_t n0_, int) : m(m_), n0(n0_) {
+    __device__ __forceinline__ Row(const EpiStats& e, int64_t m_, int64_t n0_, int, uint8_t*) : m(m_), n0(n0_) {
       st = {-INFINITY, 0.0f, 0.0f};
       at = count = 0;
       next = INT64_MAX;
@@ -298,7 +372,9 @@ struct EpiProb {
     float off;
     int at, count;
     int64_t next;
-    __device__ __forceinline__ Row(const EpiProb& e, int64_t m_, int64_t n0_, int) : m(m_), n0(n0_) {
+    uint8_t* buf;
+    __device__ __forceinline__ Row(const EpiProb& e, int64_t m_, int64_t n0_, int, uint8_t* b)
+        : m(m_), n0(n0_), buf(b) {
       at = count = 0;
       next = INT64_MAX;
       off = 0.0f;
@@ -314,7 +390,7 @@ struct EpiProb {
       }
     }
     __device__ __forceinline__ void cols(const EpiProb& e, int c, float* v) {
-      if (m >= e.M || n0 + c >= e.N) return;
+      if (n0 + c >= e.N) return;
 #pragma unroll
       for (int i = 0; i < 32; ++i) v[i] = count == 0 ? 0.0f : exp2f(v[i] * e.scale - off);
       if (next < n0 + c + 32) {
@@ -326,15 +402,11 @@ struct EpiProb {
             next = at < count ? ids[at] - e.v0 : INT64_MAX;
           }
       }
-      T* out = e.p + m * e.ld + n0 + c;
+      uint32_t w[16];
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        if (n0 + c + 8 * g >= e.N) break;  // the pitch covers the last group of 8
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = Num<T>::pack(v[8 * g + 2 * i] * e.gain, v[8 * g + 2 * i + 1] * e.gain);
-        *reinterpret_cast<uint4*>(out + 8 * g) = make_uint4(w[0], w[1], w[2], w[3]);
-      }
+      for (int i = 0; i < 16; ++i) w[i] = Num<T>::pack(v[2 * i] * e.gain, v[2 * i + 1] * e.gain);
+      // The pitch covers the last group of 8 columns.
+      stage_rows(buf, w, e.p, e.ld, m - (threadIdx.x & 31), e.M, n0 + c, e.ld, true);
     }
     __device__ __forceinline__ void end(const EpiProb&) {}
   };
@@ -404,7 +476,7 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Fin
     z = e.slope ? activate<true>(e.act, z, sl) : activate<false>(e.act, z, sl);
     if (e.res) z += Num<T>::to(e.res[m * e.ldr + n]);
     e.y[m * e.ldy + n] = Num<T>::from(z);
-    if (e.slope) e.slope[m * e.ldy + n] = Num<T>::from(sl);
+    if (e.slope) e.slope[m * e.ldy + n] = int16_t(slope_code(sl));
   }
 }
 
@@ -412,7 +484,7 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Fin
 // the unrounded products over kSumRows rows per block (part[row block][n], 32 bits).
 constexpr int kSumRows = 64;
 template <typename T>
-__global__ void __launch_bounds__(256) slope_kernel(const T* dy, int64_t ldy, const T* slope, T* dz, int64_t ldz,
+__global__ void __launch_bounds__(256) slope_kernel(const T* dy, int64_t ldy, const int16_t* slope, T* dz, int64_t ldz,
                                                     float* part, int64_t M, int64_t N) {
   const int64_t col_blocks = cdiv(N, 64), mb = blockIdx.x / col_blocks;
   const int64_t n = (blockIdx.x - mb * col_blocks) * 64 + 2 * (threadIdx.x & 31);
@@ -424,7 +496,7 @@ __global__ void __launch_bounds__(256) slope_kernel(const T* dy, int64_t ldy, co
     for (int i = 0; i < 2; ++i) {
       if (n + i >= N) break;
       float d = Num<T>::to(dy[m * ldy + n + i]);
-      if (slope) d *= Num<T>::to(slope[m * N + n + i]);
+      if (slope) d *= slope_value(slope[m * N + n + i]);
       if (dz) dz[m * ldz + n + i] = Num<T>::from(d);
       (i ? s.y : s.x) += d;
     }
@@ -740,18 +812,17 @@ int load_matrix(const void* p, int64_t rows, int64_t cols, int64_t pitch, void* 
   return copy_pitch(p, pitch, copy, round8(cols), rows, cols, s);
 }
 
-// How a product [M, K] x [N, K] is cut.  Tiles of 128 x 256 when they fill the GPU; else tiles of
-// 128 x 128, and the contraction is split until there is about one tile per SM (at least 4 blocks
-// of 64 per part).
+// How a product [M, K] x [N, K] is cut.  Pairs of CTAs with tiles of 256 x 256 when there are more
+// than 128 rows and the tiles fill the GPU; else single CTAs with tiles of 128 x 128, and the
+// contraction is split until there is about one tile per SM (at least 4 blocks of 64 per part).
 struct Cut {
-  int bn, splits;
+  int cg, splits;
 };
 Cut cut_of(int64_t M, int64_t N, int64_t K, int sms, bool split) {
-  const int64_t tm = cdiv(M, kBM);
-  if (tm * cdiv(N, 256) >= sms) return {256, 1};
-  const int64_t tiles = tm * cdiv(N, 128), kb = cdiv(K, kBK);
-  if (!split) return {128, 1};
-  return {128, int(std::max<int64_t>(1, std::min(sms / std::max<int64_t>(1, tiles), kb / 4)))};
+  if (M > 128 && cdiv(M, 256) * cdiv(N, 256) >= sms / 2) return {2, 1};
+  const int64_t tiles = cdiv(M, 128) * cdiv(N, 128), kb = cdiv(K, kBK);
+  if (!split) return {1, 1};
+  return {1, int(std::max<int64_t>(1, std::min(sms / std::max<int64_t>(1, tiles), kb / 4)))};
 }
 
 template <typename T, bool BMN, class Epi>
@@ -760,11 +831,11 @@ int product(const Matrix& a, const Matrix& b, const Cut& cut, const Epi& epi, in
   constexpr bool bf16 = Num<T>::kCode == 1;
   CUtensorMap ma, mb;
   if (int rc = make_map(&ma, a.p, a.rows, a.cols, a.pitch, kBM, bf16)) return rc;
-  if (int rc = make_map(&mb, b.p, b.rows, b.cols, b.pitch, BMN ? kBK : cut.bn, bf16)) return rc;
-  GemmShape g = gemm_shape(M, N, K, cut.bn, status);
+  if (int rc = make_map(&mb, b.p, b.rows, b.cols, b.pitch, BMN ? kBK : 128, bf16)) return rc;
+  GemmShape g = gemm_shape(M, N, K, cut.cg, status);
   g.splits = cut.splits;
-  if (cut.bn == 256) return launch_gemm<T, 256, BMN>(ma, mb, g, epi, s);
-  return launch_gemm<T, 128, BMN>(ma, mb, g, epi, s);
+  if (cut.cg == 2) return launch_gemm<T, 2, BMN>(ma, mb, g, epi, s);
+  return launch_gemm<T, 1, BMN>(ma, mb, g, epi, s);
 }
 
 template <typename T>
@@ -832,7 +903,7 @@ EpiLinear<T> linear_epilogue(const void* bias, const void* res, int64_t ldr, voi
   e.bias = bias ? static_cast<const T*>(bias) + r0 : nullptr;
   e.res = res ? static_cast<const T*>(res) + r0 : nullptr;
   e.y = static_cast<T*>(y) + r0;
-  e.slope = slope ? static_cast<T*>(slope) + r0 : nullptr;
+  e.slope = slope ? static_cast<int16_t*>(slope) + r0 : nullptr;
   e.ldr = ldr;
   e.ldy = ldy;
   e.M = M;
@@ -917,7 +988,7 @@ int run_linear_grad(const LinearGradPlan& p, const zn_weight* w, const void* dy,
     T* dz = slope ? static_cast<T*>(p.dz) : nullptr;
     const int64_t grid = cdiv(rows, 64) * p.sum_blocks;
     if (grid > 0x7FFFFFFF) return bad("zn_linear_grad");
-    slope_kernel<T><<<unsigned(grid), 256, 0, s>>>(g, ldy, static_cast<const T*>(slope), dz, p.ldz, p.part, tokens, rows);
+    slope_kernel<T><<<unsigned(grid), 256, 0, s>>>(g, ldy, static_cast<const int16_t*>(slope), dz, p.ldz, p.part, tokens, rows);
     count_launch();
     if (int rc = check_launch("slope_kernel")) return rc;
   }
@@ -1005,7 +1076,7 @@ int plan_loss(const zn_weight* w, const void* x, int64_t ldx, int64_t tokens, in
     if (int rc = plan_weight(w, 0, status, ar, &p->w)) return rc;
     p->cut = cut_of(tokens, p->w.piece_rows, w->cols, sms, false);
     // Every piece but the last is a multiple of 256 rows.
-    p->tiles = cdiv(w->rows, p->cut.bn);
+    p->tiles = cdiv(w->rows, 128 * p->cut.cg);
   }
   p->part = ar.take<float>(size_t(p->tiles) * 3 * tokens * 4);
   return ZN_OK;
@@ -1033,7 +1104,7 @@ int run_loss(const LossPlan& p, const void* x, int64_t ldx, int64_t tokens, cons
       const int64_t r1 = std::min(vocab, r0 + p.w.piece_rows);
       Matrix wm;
       if (int rc = load_piece(p.w, r0, r1, &wm, s)) return rc;
-      const EpiStats e{rows, p.part, tokens, r1 - r0, r0, r0 / p.cut.bn, p.cut.bn, kLog2e * inv_t};
+      const EpiStats e{rows, p.part, tokens, r1 - r0, r0, r0 / (128 * p.cut.cg), 128 * p.cut.cg, kLog2e * inv_t};
       if (int rc = product<T, false>(xm, wm, p.cut, e, p.w.status, s)) return rc;
     }
   }
