@@ -45,8 +45,9 @@ struct Geom {
 
 __host__ __device__ inline Geom geom_of(int64_t m, int t) {
   Geom g;
-  g.sc = cdiv(cdiv(m, int64_t(1) << t), kRound) * kRound;
-  g.nu = int(cdiv(m, g.sc));
+  g.sc = cdiv((m + (int64_t(1) << t) - 1) >> t, kRound) * kRound;
+  // A 32-bit division where the sizes allow it (every whole-tensor chunk): a fifth of the 64-bit one.
+  g.nu = m + g.sc <= 0xFFFFFFFFll ? int(uint32_t(m + g.sc - 1) / uint32_t(g.sc)) : int(cdiv(m, g.sc));
   g.lw = g.sc / kLanes < 65536 ? 2 : 4;  // a state emits at most one word per symbol
   return g;
 }

@@ -16,7 +16,6 @@ namespace {
 
 constexpr int kDecThreads = 128;  // 4 warps per chunk
 constexpr int kChains = 1;        // rANS states per lane (sub-chunks per lane)
-constexpr int kSym = 256 / kDecThreads;  // symbols per thread in table building
 constexpr int64_t kCodedBit = int64_t(1) << 62;
 constexpr int64_t kOffMask = kCodedBit - 1;
 
@@ -55,37 +54,24 @@ struct PlaneInfo {
 };
 
 struct DecSmem {
-  uint32_t f[256];
-  uint32_t cum[256];
-  uint32_t red[8];
+  uint32_t hi[256];            // per present symbol, ascending: f << 20 | symbol << 12
+  uint32_t cum[256];           // and its first slot
+  uint32_t start[kM / 32];     // bit z: a symbol's slots start at z
+  uint32_t sub[64];            // words of each sub-chunk's streams
+  uint32_t count[kDecThreads / 32], freq[kDecThreads / 32], starts[kDecThreads / 32];
   int err;
-  int t;
   PlaneInfo p[8];
 };
 
-__device__ __forceinline__ uint32_t block_sum(uint32_t v, uint32_t* red) {
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  uint32_t s = 0;
-  for (int w = 0; w < kDecThreads / 32; ++w) s += red[w];
-  return s;
-}
-
-__device__ __forceinline__ uint32_t block_excl(uint32_t v, uint32_t* red) {
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  uint32_t incl = v;
+// Inclusive sum over the lanes of a warp.
+__device__ __forceinline__ uint32_t warp_scan(uint32_t v) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    uint32_t u = __shfl_up_sync(0xFFFFFFFFu, incl, o);
-    if (lane >= o) incl += u;
+    const uint32_t u = __shfl_up_sync(0xFFFFFFFFu, v, o);
+    if (lane >= o) v += u;
   }
-  __syncthreads();
-  if (lane == 31) red[w] = incl;
-  __syncthreads();
-  uint32_t base = 0;
-  for (int q = 0; q < w; ++q) base += red[q];
-  return base + incl - v;
+  return v;
 }
 
 // Parse a ZNR2 payload header and build its decode table.  Entry of slot z (symbol s, cum c, freq
@@ -93,93 +79,119 @@ __device__ __forceinline__ uint32_t block_excl(uint32_t v, uint32_t* red) {
 // after the lookup.  A plane with a single symbol (f = M) needs no table: its state never changes
 // and it has no words; P.single holds that symbol.  Returns false (uniformly) if the payload is
 // malformed.
+//
+// A chunk's start is all latency, so the steps are few and wide: thread i owns symbols 2i and 2i + 1
+// (ballots number the present ones, one scan gives their first slots) and loads a stream length;
+// the table is filled 32 slots per warp step, a slot's symbol being the count of symbol starts up
+// to it (a bit mask of starts, popc and a scan over its words).
 __device__ bool build_plane(PlaneInfo& P, int64_t m, uint32_t* tab, DecSmem& S) {
-  const int tid = threadIdx.x;
+  static_assert(kDecThreads == 128 && kM / 32 == kDecThreads, "two symbols and one start word per thread");
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint8_t* pl = P.pl;
   const int64_t size = P.size;
-  bool ok = size >= 34 && pl[0] >= kMinSubLog2 && pl[0] <= kMaxSubLog2 && pl[1] == 0;
-  if (!__syncthreads_and(ok)) return false;
-  const int t = pl[0];
-  uint32_t pres[kSym], f4[kSym];
-  uint32_t npres = 0;
+  if (size < 34) return false;
+  const int t = pl[0], flag = pl[1];
+  const uint32_t bits = (pl[2 + (tid >> 2)] >> (2 * (tid & 3))) & 3;  // presence of symbols 2 tid, 2 tid + 1
+  if (t < kMinSubLog2 || t > kMaxSubLog2 || flag != 0) return false;
+  S.start[tid] = 0;
+  const uint32_t b0 = __ballot_sync(0xFFFFFFFFu, bits & 1), b1 = __ballot_sync(0xFFFFFFFFu, bits >> 1);
+  if (lane == 0) S.count[warp] = __popc(b0) + __popc(b1);
+  __syncthreads();
+  const uint32_t below = (1u << lane) - 1;
+  uint32_t np = 0, k = __popc(b0 & below) + __popc(b1 & below);
 #pragma unroll
-  for (int h = 0; h < kSym; ++h) {
-    const int s = kSym * tid + h;
-    pres[h] = (pl[2 + (s >> 3)] >> (s & 7)) & 1;
-    npres += pres[h];
+  for (int w = 0; w < kDecThreads / 32; ++w) {
+    if (w < warp) k += S.count[w];
+    np += S.count[w];
   }
-  const uint32_t np = block_sum(npres, S.red);
   const int64_t tb = table_bytes(int(np));
   const Geom g = geom_of(m, t);
   const int64_t mb = meta_bytes(int(np), g);
   if (np == 0 || mb > size) return false;
-  uint32_t k = block_excl(npres, S.red);
-  uint32_t fsum = 0;
+  uint32_t f[2];
 #pragma unroll
-  for (int h = 0; h < kSym; ++h) {
-    f4[h] = 0;
-    if (pres[h]) {
-      const uint32_t bit = 12 * k++;
+  for (int h = 0; h < 2; ++h) {
+    f[h] = 0;
+    if ((bits >> h) & 1) {
+      const uint32_t bit = 12 * (k + (h ? bits & 1 : 0));
       const uint8_t* q = pl + 34 + (bit >> 3);
       const uint32_t v = (uint32_t(q[0]) | (uint32_t(q[1]) << 8) | (uint32_t(q[2]) << 16)) >> (bit & 7);
-      f4[h] = (v & 0xFFF) + 1;
+      f[h] = (v & 0xFFF) + 1;
     }
-    fsum += f4[h];
   }
-  const uint32_t total = block_sum(fsum, S.red);
+  // Stream lengths, a field per thread; a sub-chunk's are 8 neighbouring lanes.
+  bool good = true;
+  const int fields = g.nu * kLanes;
+  for (int f0 = 0; f0 < fields; f0 += kDecThreads) {
+    const int fi = f0 + tid;
+    uint32_t nw = 0;
+    if (fi < fields)
+      nw = g.lw == 2 ? *reinterpret_cast<const uint16_t*>(pl + tb + 2 * fi)
+                     : *reinterpret_cast<const uint32_t*>(pl + tb + 4 * int64_t(fi));
+    good &= nw <= g.sc / kLanes;
+#pragma unroll
+    for (int o = 1; o < kLanes; o <<= 1) nw += __shfl_xor_sync(0xFFFFFFFFu, nw, o);
+    if (fi < fields && (lane & (kLanes - 1)) == 0) S.sub[fi / kLanes] = nw;
+  }
+  const uint32_t incl = warp_scan(f[0] + f[1]);
+  if (lane == 31) S.freq[warp] = incl;
+  __syncthreads();
+  uint32_t c = incl - f[0] - f[1], total = 0;
+#pragma unroll
+  for (int w = 0; w < kDecThreads / 32; ++w) {
+    if (w < warp) c += S.freq[w];
+    total += S.freq[w];
+  }
   if (total != kM) return false;
-  if (np == 1) {
 #pragma unroll
-    for (int h = 0; h < kSym; ++h)
-      if (pres[h]) P.single = kSym * tid + h;
-  }
-  uint32_t c0 = block_excl(fsum, S.red);
-#pragma unroll
-  for (int h = 0; h < kSym; ++h) {
-    S.f[kSym * tid + h] = f4[h];
-    S.cum[kSym * tid + h] = c0;
-    c0 += f4[h];
-  }
-  // Per-sub-chunk stream offsets (sum of its 8 lane lengths; one warp, one sub-chunk per lane).
-  if (tid < 32) {
-    int64_t pos = mb / 2;
-    bool good = true;
-    for (int g0 = 0; g0 < g.nu; g0 += 32) {
-      const int gi = g0 + tid;
-      int64_t sub = 0;
-      if (gi < g.nu)
-        for (int l = 0; l < kLanes; ++l) {
-          const int64_t fi = int64_t(gi) * kLanes + l;
-          const int64_t nw = g.lw == 2 ? int64_t(pl[tb + 2 * fi]) | (int64_t(pl[tb + 2 * fi + 1]) << 8)
-                                       : int64_t(*reinterpret_cast<const uint32_t*>(pl + tb + 4 * fi));
-          good &= nw <= g.sc / kLanes;
-          sub += nw;
-        }
-      int64_t incl = sub;
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t v = __shfl_up_sync(0xFFFFFFFFu, incl, o);
-        if (tid >= o) incl += v;
-      }
-      if (gi < g.nu) P.stream_off[gi] = int32_t(pos + incl - sub);
-      pos += __shfl_sync(0xFFFFFFFFu, incl, 31);
+  for (int h = 0; h < 2; ++h)
+    if (f[h]) {
+      const uint32_t s = 2 * tid + h;
+      S.hi[k] = (f[h] << 20) | (s << 12);  // f = M (one symbol) wraps: the table is unused
+      S.cum[k] = c;
+      atomicOr(&S.start[c >> 5], 1u << (c & 31));
+      if (np == 1) P.single = int(s);
+      ++k;
+      c += f[h];
     }
-    good = __all_sync(0xFFFFFFFFu, good);
+  if (warp == 0) {  // where each sub-chunk's streams start
+    int64_t pos = mb / 2;
+    for (int g0 = 0; g0 < g.nu; g0 += 32) {
+      const int gi = g0 + lane;
+      const int64_t sub = gi < g.nu ? S.sub[gi] : 0;
+      int64_t in = sub;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t v = __shfl_up_sync(0xFFFFFFFFu, in, o);
+        if (lane >= o) in += v;
+      }
+      if (gi < g.nu) P.stream_off[gi] = int32_t(pos + in - sub);
+      pos += __shfl_sync(0xFFFFFFFFu, in, 31);
+    }
+    good &= 2 * pos == size;
     if (tid == 0) {
       P.t = t;
       P.lens_off = tb;
       P.lw = g.lw;
       P.states_off = tb + lengths_bytes(g);
-      S.err = !(good && 2 * pos == size);
     }
   }
+  if (!__syncthreads_and(good)) return false;
+  // Warp w fills slots [1024 w, 1024 w + 1024): lane i holds start word 32 w + i.
+  const uint32_t word = S.start[tid];
+  const uint32_t in = warp_scan(__popc(word));
+  if (lane == 31) S.starts[warp] = in;
   __syncthreads();
-  if (S.err) return false;
-  // Fill the slot table, one symbol per warp iteration, 32 slots per step.
-  const int lane = tid & 31, warp = tid >> 5;
-  for (int s = warp; s < 256; s += kDecThreads / 32) {
-    const uint32_t f = S.f[s], c = S.cum[s];
-    const uint32_t hi = (f << 20) | (uint32_t(s) << 12);  // f = M (one symbol) wraps: the table is unused
-    for (uint32_t q = lane; q < f; q += 32) tab[c + q] = hi | q;
+  uint32_t before = in - __popc(word);
+#pragma unroll
+  for (int w = 0; w < kDecThreads / 32; ++w)
+    if (w < warp) before += S.starts[w];
+  const uint32_t upto = 0xFFFFFFFFu >> (31 - lane);
+#pragma unroll 8
+  for (int i = 0; i < 32; ++i) {
+    const uint32_t wi = __shfl_sync(0xFFFFFFFFu, word, i), bi = __shfl_sync(0xFFFFFFFFu, before, i);
+    const uint32_t q = bi + __popc(wi & upto) - 1, z = 1024 * warp + 32 * i + lane;
+    tab[z] = S.hi[q] | (z - S.cum[q]);
   }
   __syncthreads();
   return true;
@@ -640,17 +652,21 @@ __device__ __forceinline__ void decode_chunk(const DecArgs& a, int64_t j, bool o
         ring[q][c] = rings + (q * kChains + c) * kRing * kDecThreads + tid;
         cb.x = kL;
         cb.ptr = cb.end = cb.fill = cb.nload = 0;
-        if (q < ncoded && valid[c]) {
-          const PlaneInfo& P = S.p[pslot[q]];
-          const int64_t fbase = int64_t(gi[c]) * kLanes;
-          uint32_t before = 0, mine = 0;
-          for (int ll = 0; ll <= l; ++ll) {
-            const int64_t fi = fbase + ll;
-            const uint32_t nw = P.lw == 2 ? *reinterpret_cast<const uint16_t*>(P.pl + P.lens_off + 2 * fi)
-                                          : *reinterpret_cast<const uint32_t*>(P.pl + P.lens_off + 4 * fi);
-            if (ll < l) before += nw;
-            else mine = nw;
-          }
+        if (q >= ncoded) continue;
+        const PlaneInfo& P = S.p[pslot[q]];
+        const int64_t fbase = int64_t(gi[c]) * kLanes;
+        uint32_t mine = 0;
+        if (valid[c])
+          mine = P.lw == 2 ? *reinterpret_cast<const uint16_t*>(P.pl + P.lens_off + 2 * (fbase + l))
+                           : *reinterpret_cast<const uint32_t*>(P.pl + P.lens_off + 4 * (fbase + l));
+        uint32_t before = mine;  // words of the sub-chunk's lanes before this one
+#pragma unroll
+        for (int o = 1; o < kLanes; o <<= 1) {
+          const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, before, o, kLanes);
+          if (l >= o) before += v;
+        }
+        before -= mine;
+        if (valid[c]) {
           const uint32_t h0 = uint32_t((P.pl - gb[q]) >> 1) + uint32_t(P.stream_off[gi[c]]) + before;
           cb.x = *reinterpret_cast<const uint32_t*>(P.pl + P.states_off + 4 * (fbase + l));
           cb.ptr = h0;
