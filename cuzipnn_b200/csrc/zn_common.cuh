@@ -303,6 +303,32 @@ int upload_jobs(const T* host, int count, T* dev, int64_t total_chunks, cudaStre
                     : upload_batches<T, N>(host, count, dev, total_chunks, s);
 }
 
+// Programmatic dependent launch.  A kernel launched by launch_after may start while the kernel before
+// it in the stream still runs: it must call pdl_wait() before it touches memory, which returns once
+// that kernel has ended and its writes are visible.  (Every kernel of a chain of such launches
+// waits, so each also sees what came before.)  pdl_trigger() in the earlier kernel lets the later
+// one be placed as soon as all of the earlier one's blocks have called it.
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <class... P, class... A>
+int launch_after(void (*fn)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t s, const char* name,
+                 const A&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, fn, P(args)...);
+  count_launch();
+  return check_launch(name);
+}
+
 // An NVTX range over a scope of host code (entry points), visible to Nsight tools.
 struct NvtxScope {
   explicit NvtxScope(const char* name);

@@ -180,7 +180,7 @@ int launch_decode(const DecArgs* jobs, int njobs, int64_t grid, cudaStream_t s) 
 }  // namespace
 
 int weight_scan(const WeightBlob& w, void* temp, int32_t* status, cudaStream_t s) {
-  const DecArgs a = weight_args(w, temp, status);
+  const DecArgs a = weight_args(w, temp, status, kScanned);
   FirstJob<DecArgs> fj{};
   fj.job = a;
   fj.valid = 1;

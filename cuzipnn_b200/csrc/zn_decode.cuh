@@ -36,8 +36,14 @@ struct DecArgs {
   const int64_t* out_ptrs;
   const int64_t* out_cap;
   int32_t* statuses;
-  uint8_t* overflow;      // per chunk: more coded planes than the main pass holds
+  uint8_t* overflow;      // per chunk: more coded planes than the main pass holds (weights: its flags)
+  int mode;               // kJob, or for a weight kDirect / kScanned
 };
+
+// A weight's chunks report through one byte each (kChunkOver | error bits) instead of the status
+// word.  kScanned: dscan_kernel has filled `src`.  kDirect: every chunk finds its units itself.
+constexpr int kJob = 0, kScanned = 1, kDirect = 2;
+constexpr uint8_t kChunkOver = 128;
 
 struct PlaneInfo {
   const uint8_t* pl;  // payload (coded) or raw bytes of this unit's chunk
@@ -60,6 +66,8 @@ struct DecSmem {
   uint32_t sub[64];            // words of each sub-chunk's streams
   uint32_t count[kDecThreads / 32], freq[kDecThreads / 32], starts[kDecThreads / 32];
   int err;
+  int64_t sums[2][kDecThreads / 32];
+  int coded[2];
   PlaneInfo p[8];
 };
 
@@ -400,6 +408,7 @@ template <typename T, int MT>
 struct DotSink {
   static constexpr bool kDot = true;
   static constexpr int kRows = MT;
+  static constexpr bool kAhead = MT <= 2;  // x is loaded a round ahead (8 registers per row)
   using Elem = T;
   const T* x;
   int64_t ldx, cols, rows;
@@ -422,7 +431,22 @@ struct DotState {
   int64_t row;  // the segment's current row
   bool first;   // no row end met in this sub-chunk yet
   bool mid;     // the sub-chunk starts inside a row
+  uint4 x[MT][2];  // the next round's elements of x
 };
+
+// Loads the next round's elements of x (those of row 0 for rows past the last; lanes without
+// elements load valid ones too).  Called before the round is decoded, which hides the latency.
+template <class Sink>
+__device__ __forceinline__ void dot_load(const Sink& k, DotState<Sink::kRows>& st, int l) {
+  int col = st.col + kRound + l * kSteps;
+  if (col >= k.cols) col -= int(k.cols);
+#pragma unroll
+  for (int m = 0; m < Sink::kRows; ++m) {
+    const uint4* xp = reinterpret_cast<const uint4*>(k.x + (m < k.tokens ? m * k.ldx : 0) + col);
+    st.x[m][0] = __ldg(xp);
+    st.x[m][1] = __ldg(xp + 1);
+  }
+}
 
 template <int MT>
 __device__ __forceinline__ void segment_sum(float* v, uint32_t mask) {
@@ -437,19 +461,16 @@ template <class Sink>
 __device__ __forceinline__ void dot_round(const Sink& k, DotState<Sink::kRows>& st, const uint32_t* e, bool active,
                                           int l, uint32_t mask, float* slot0) {
   constexpr int MT = Sink::kRows;
+  if constexpr (!Sink::kAhead) dot_load(k, st, l);
   st.col += kRound;
-  int col = st.col + l * kSteps;
-  const bool wrapped = active && col >= k.cols;  // the lane's elements lie in the next row
-  if (wrapped) col -= int(k.cols);
+  const bool wrapped = active && st.col + l * kSteps >= k.cols;  // the lane's elements lie in the next row
   float d[MT];
 #pragma unroll
   for (int m = 0; m < MT; ++m) d[m] = 0.0f;
   if (active) {
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      if (m >= k.tokens) break;
-      const uint4* xp = reinterpret_cast<const uint4*>(k.x + m * k.ldx + col);
-      const uint4 a = __ldg(xp), b = __ldg(xp + 1);
+      const uint4 a = st.x[m][0], b = st.x[m][1];
       const uint32_t xw[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -515,12 +536,71 @@ __device__ __forceinline__ void dot_finish_chunk(const Sink& k, int64_t j, int64
   }
 }
 
+// Offset (with kCodedBit, or -1) of the units of chunk j of a weight, by the whole CTA from the blob's
+// tables: what dscan_kernel computes for all units at once, with the same checks.  It reads the
+// tables up to the chunk's second unit (12 bytes per chunk of the blob, from L2 but for the first
+// CTA), so it pays for weights of up to kDirectChunks chunks, whose launch it saves.
+__device__ __forceinline__ void find_units(const DecArgs& a, int64_t j, DecSmem& S, int64_t* unit, bool* bad) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid < 2) S.coded[tid] = 0;
+  __syncthreads();
+  const int64_t n_comp = *reinterpret_cast<const uint32_t*>(a.blob + 12);
+  const int64_t data_off = align8(a.idx_off + 4 * n_comp);
+  bool wrong = false;
+  *bad = false;
+  if (n_comp > a.units || data_off > a.blob_bytes) {  // uniform
+    unit[0] = unit[1] = -1;
+    *bad = true;
+    return;
+  }
+  const int32_t* stored = reinterpret_cast<const int32_t*>(a.blob + a.sizes_off);
+  const int32_t* idx = reinterpret_cast<const int32_t*>(a.blob + a.idx_off);
+  const int nch = int(a.nch), end = nch + int(j);
+  int64_t s0 = 0, s1 = 0;
+#pragma unroll 4
+  for (int i = tid; i < end; i += kDecThreads) {
+    const int32_t s = stored[i];
+    wrong |= s < 0;
+    const int64_t v = s < 0 ? 0 : align8(s);
+    s1 += v;
+    if (i < j) s0 += v;
+  }
+#pragma unroll 4
+  for (int i = tid; i < int(n_comp); i += kDecThreads) {
+    const int32_t u = idx[i];
+    wrong |= u < 0 || u >= a.units;
+    if (u == j) S.coded[0] = 1;
+    if (u == end) S.coded[1] = 1;
+  }
+  for (int o = 16; o; o >>= 1) {
+    s0 += __shfl_xor_sync(0xFFFFFFFFu, s0, o);
+    s1 += __shfl_xor_sync(0xFFFFFFFFu, s1, o);
+  }
+  if (lane == 0) {
+    S.sums[0][warp] = s0;
+    S.sums[1][warp] = s1;
+  }
+  wrong = __syncthreads_or(wrong);
+  const int64_t raw = j == a.nch - 1 ? a.n - j * a.C : a.C;
+#pragma unroll
+  for (int b = 0; b < 2; ++b) {
+    int64_t off = data_off;
+#pragma unroll
+    for (int w = 0; w < kDecThreads / 32; ++w) off += S.sums[b][w];
+    const int64_t st = stored[b * a.nch + j];
+    const bool coded = S.coded[b] != 0;
+    unit[b] = st < 0 || off + st > a.blob_bytes || (!coded && st != raw) ? -1 : off | (coded ? kCodedBit : 0);
+  }
+  *bad = wrong;
+}
+
 // Decode chunk j of a job with the whole CTA.  KC: coded planes per chunk held in shared memory.
 // The main pass (KC = 1 for K > 1) flags chunks with more coded planes; a second pass with KC = K
 // decodes only those.  Every return is taken by all threads of the CTA together.
 // Work split: a warp item is 8 sub-chunks; lane l of 8-lane segment g runs chain c on sub-chunk
 // 8 * item + 4 * c + g.
-template <int K, bool REORDER, int KC, class Sink>
+// WEIGHT: a chunk of a weight (DecArgs::mode).
+template <int K, bool REORDER, int KC, bool WEIGHT = false, class Sink>
 __device__ __forceinline__ void decode_chunk(const DecArgs& a, int64_t j, bool overflow_pass, const Sink& sink) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
   using Slot = RingSlot<KC>;
@@ -543,7 +623,16 @@ __device__ __forceinline__ void decode_chunk(const DecArgs& a, int64_t j, bool o
   }
   if constexpr (Sink::kDot)
     for (int i = tid; i < 64 * 2 * Sink::kRows; i += kDecThreads) slots[i] = 0.0f;
+  int flags = 0;  // weights: error bits of this chunk
+  [[maybe_unused]] int64_t unit[2] = {-1, -1};
+  if constexpr (WEIGHT)
+    if (a.mode == kDirect) {
+      bool wrong;
+      find_units(a, j, S, unit, &wrong);
+      if (wrong) flags |= kErrTable;
+    }
   if (tid == 0) S.err = 0;
+  if constexpr (WEIGHT) __syncthreads();
   if (tid < K) {
     PlaneInfo& P = S.p[tid];
     if (batched) {
@@ -554,7 +643,9 @@ __device__ __forceinline__ void decode_chunk(const DecArgs& a, int64_t j, bool o
       P.hi = P.pl + P.size;
     } else {
       const int64_t u = int64_t(tid) * a.nch + j;
-      const int64_t s = a.src[u];
+      int64_t s;
+      if constexpr (WEIGHT) s = a.mode != kDirect ? a.src[u] : tid == 0 ? unit[0] : unit[1];
+      else s = a.src[u];
       // dscan_kernel has checked that the tables lie inside the blob for every unit with s >= 0.
       const int64_t stored = s >= 0 ? *reinterpret_cast<const int32_t*>(a.blob + a.sizes_off + 4 * u) : 0;
       P.coded = s >= 0 && (s & kCodedBit);
@@ -579,8 +670,15 @@ __device__ __forceinline__ void decode_chunk(const DecArgs& a, int64_t j, bool o
     }
   if (KC < K && !overflow_pass) {
     const bool over = ncoded > KC;
-    if (tid == 0) a.overflow[j] = over;
-    if (over) return;
+    if constexpr (WEIGHT) {
+      if (over) {
+        if (tid == 0) a.overflow[j] = uint8_t(kChunkOver | flags);
+        return;
+      }
+    } else {
+      if (tid == 0) a.overflow[j] = over;
+      if (over) return;
+    }
   }
   bool bad = S.err != 0 || m <= 0;
   for (int q = 0; q < KC && q < ncoded && !bad; ++q)
@@ -594,7 +692,8 @@ __device__ __forceinline__ void decode_chunk(const DecArgs& a, int64_t j, bool o
   }
   if (bad) {
     if (tid == 0) {
-      if (batched) a.statuses[j] = kErrPayload;
+      if (WEIGHT) a.overflow[j] = uint8_t((overflow_pass ? kChunkOver : 0) | flags | kErrPayload);
+      else if (batched) a.statuses[j] = kErrPayload;
       else atomicOr(a.status, kErrPayload);
     }
     if constexpr (Sink::kDot) {
@@ -739,6 +838,8 @@ __device__ __forceinline__ void decode_chunk(const DecArgs& a, int64_t j, bool o
               if (cb.nload) cb.r0 = block(cb.fill / 8);
             }
           }
+          if constexpr (Sink::kDot)
+            if constexpr (Sink::kAhead) dot_load(sink, dot, l);
           uint32_t p[kChains][K][4];
 #pragma unroll
           for (int c = 0; c < kChains; ++c)
@@ -826,6 +927,8 @@ __device__ __forceinline__ void decode_chunk(const DecArgs& a, int64_t j, bool o
 #pragma unroll
           for (int i = 0; i < 4; ++i) p[c][b][i] = pn[c][b][i];
       if (r + 1 < rounds) load_raw_round<K, kChains>(src, coded, base, len, r + 1, l, pn);
+      if constexpr (Sink::kDot)
+        if constexpr (Sink::kAhead) dot_load(sink, dot, l);
       const bool full = nact[0] == kSteps && nact[kChains - 1] == kSteps;
 #pragma unroll
       for (int q = 0; q < KC; ++q) {
@@ -899,6 +1002,10 @@ __device__ __forceinline__ void decode_chunk(const DecArgs& a, int64_t j, bool o
   }
   const bool any_err = __syncthreads_or(err);
   if constexpr (Sink::kDot) dot_finish_chunk(sink, j, j * a.C, j * a.C + m, g.sc, slots, any_err);
+  if constexpr (WEIGHT) {
+    if (tid == 0) a.overflow[j] = uint8_t((overflow_pass ? kChunkOver : 0) | flags | (any_err ? kErrStream : 0));
+    return;
+  }
   if (any_err && tid == 0) {
     if (batched) a.statuses[j] = kErrStream;
     else atomicOr(a.status, kErrStream);
@@ -917,8 +1024,9 @@ inline size_t dec_job_bytes(int64_t n, int k, int64_t chunk_bytes) {
 }
 
 // The decoder's job for a weight, with its scratch in `temp`.
-inline DecArgs weight_args(const WeightBlob& w, void* temp, int32_t* status) {
+inline DecArgs weight_args(const WeightBlob& w, void* temp, int32_t* status, int mode) {
   DecArgs a{};
+  a.mode = mode;
   a.blob = w.blob;
   a.blob_bytes = w.blob_bytes;
   a.n = w.rows * w.cols;

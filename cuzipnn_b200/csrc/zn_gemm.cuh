@@ -266,6 +266,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
   __syncthreads();
   if constexpr (CG == 2) group_sync<2>();
   tc_fence_after();
+  pdl_wait();
   const uint32_t tmem = s_tmem;
   volatile int* abort_flag = &s_abort;
 
@@ -437,12 +438,14 @@ int launch_gemm(const CUtensorMap& a, const CUtensorMap& b, const GemmShape& g, 
   cfg.blockDim = dim3(kGemmThreads);
   cfg.dynamicSmemBytes = GemmCfg<CG>::kSmem;
   cfg.stream = s;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = CG;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = CG > 1 ? 1 : 0;
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = CG;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = CG > 1 ? 2 : 1;
   TimedLaunch tl("gemm", s);
   cudaLaunchKernelEx(&cfg, fn, a, b, g, epi);
   count_launch();

@@ -1,0 +1,220 @@
+// The linear layer's epilogue, on a tile of a product (EpiLinear) or element by element (Finish).
+#pragma once
+
+#include "zn_gemm.cuh"
+#include "zn_weight.cuh"
+
+namespace zn {
+
+constexpr int kNone = 0, kRelu = 1, kGelu = 2, kGeluTanh = 3, kSilu = 4;
+
+// act(z) and its derivative (where asked for), in 32 bits.
+template <int ACT, bool SLOPE>
+__device__ __forceinline__ float activate(float z, float& slope) {
+  if constexpr (ACT == kRelu) {
+    if (SLOPE) slope = z > 0.0f ? 1.0f : 0.0f;
+    return z < 0.0f ? 0.0f : z;  // keeps NaN
+  } else if constexpr (ACT == kGelu) {
+    const float cdf = 0.5f * erfcf(-0.70710678118654752f * z);
+    if (SLOPE) slope = cdf + z * 0.3989422804014327f * __expf(-0.5f * z * z);
+    return z * cdf;
+  } else if constexpr (ACT == kGeluTanh) {  // 0.5 z (1 + tanh u) = z sigmoid(2u)
+    const float c = 0.7978845608028654f, z2 = z * z;
+    const float sig = __fdividef(1.0f, 1.0f + __expf(-2.0f * c * z * (1.0f + 0.044715f * z2)));
+    if (SLOPE) slope = sig + z * sig * (1.0f - sig) * 2.0f * c * (1.0f + 3.0f * 0.044715f * z2);
+    return z * sig;
+  } else if constexpr (ACT == kSilu) {
+    const float sig = __fdividef(1.0f, 1.0f + __expf(-z));
+    if (SLOPE) slope = sig * (1.0f + z * (1.0f - sig));
+    return z * sig;
+  } else {
+    if (SLOPE) slope = 1.0f;
+    return z;
+  }
+}
+template <bool SLOPE>
+__device__ __forceinline__ float activate(int act, float z, float& slope) {
+  switch (act) {
+    case kRelu: return activate<kRelu, SLOPE>(z, slope);
+    case kGelu: return activate<kGelu, SLOPE>(z, slope);
+    case kGeluTanh: return activate<kGeluTanh, SLOPE>(z, slope);
+    case kSilu: return activate<kSilu, SLOPE>(z, slope);
+    default: return activate<kNone, SLOPE>(z, slope);
+  }
+}
+
+// The derivative act'(z), kept for the backward pass as a 16-bit fixed-point number of step 2^-14
+// (every activation's lies in [-0.13, 1.13]): off by 2^-15 of a whole slope at most, an eighth of
+// a bf16 rounding, so the gradients are as exact as with a 32-bit slope.  -32768 stands for NaN.
+__device__ __forceinline__ int slope_code(float s) { return s != s ? -32768 : __float2int_rn(s * 16384.0f); }
+__device__ __forceinline__ float slope_value(int code) { return code == -32768 ? NAN : float(code) * (1.0f / 16384.0f); }
+
+// Per-warp staging: a thread holds 64 bytes (32 16-bit columns) of its own row; through shared
+// memory the warp writes them as 8 rows x 64 contiguous bytes per store.  The 16-byte chunks of a
+// row are permuted by the row, so that both sides touch every bank once.
+__device__ __forceinline__ uint4* stage_at(uint8_t* buf, int row, int chunk) {
+  return reinterpret_cast<uint4*>(buf + row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4));
+}
+// Rows m0 + r < M, columns n0 .. n0 + 31 < N of a 16-bit matrix from the warp's 16 words per thread.
+template <typename T>
+__device__ __forceinline__ void stage_rows(uint8_t* buf, const uint32_t* w, T* out, int64_t ld, int64_t m0, int64_t M,
+                                           int64_t n0, int64_t N, bool vec) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) *stage_at(buf, lane, i) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+  __syncwarp();
+  if (vec) {  // 16-byte aligned rows, N a multiple of 8
+    const int64_t n = n0 + 8 * (lane & 3);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = 8 * i + (lane >> 2);
+      if (m0 + r < M && n < N) *reinterpret_cast<uint4*>(out + (m0 + r) * ld + n) = *stage_at(buf, r, lane & 3);
+    }
+  } else if (n0 + lane < N) {
+    const int rows = int(min(int64_t(32), M - m0));
+    for (int r = 0; r < rows; ++r)
+      out[(m0 + r) * ld + n0 + lane] = reinterpret_cast<const T*>(stage_at(buf, r, lane >> 3))[lane & 7];
+  }
+  __syncwarp();
+}
+
+// y = act(acc + bias) + residual, rounded once to 16 bits, and (where asked for) the slopes.
+template <typename T>
+struct EpiLinear {
+  const T* bias;  // or null
+  const T* res;   // or null
+  T* y;
+  int16_t* slope;  // or null
+  int64_t ldr, ldy, M, N;
+  int act;
+  bool vec;  // 16-byte accesses: every pointer and pitch allows them, and N is a multiple of 8
+
+  struct Row {
+    int64_t m, n0;
+    uint8_t* buf;
+    __device__ __forceinline__ Row(const EpiLinear&, int64_t m_, int64_t n0_, int, uint8_t* b) : m(m_), n0(n0_), buf(b) {}
+
+    template <int ACT, bool SLOPE>
+    __device__ __forceinline__ void run(const EpiLinear& e, int64_t n, float* v) {
+      uint32_t sw[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        float s0, s1;
+        v[2 * i] = activate<ACT, SLOPE>(v[2 * i], s0);
+        v[2 * i + 1] = activate<ACT, SLOPE>(v[2 * i + 1], s1);
+        if (SLOPE) sw[i] = (uint32_t(slope_code(s0)) & 0xFFFFu) | (uint32_t(slope_code(s1)) << 16);
+      }
+      if (SLOPE) stage_rows(buf, sw, e.slope, e.ldy, m - (threadIdx.x & 31), e.M, n, e.N, e.vec);
+    }
+
+    __device__ __forceinline__ void cols(const EpiLinear& e, int c, float* v) {
+      const int64_t n = n0 + c;
+      if (n >= e.N) return;
+      if (e.bias) add(e.bias, n, e, v);
+      if (e.slope) {
+        switch (e.act) {
+          case kRelu: run<kRelu, true>(e, n, v); break;
+          case kGelu: run<kGelu, true>(e, n, v); break;
+          case kGeluTanh: run<kGeluTanh, true>(e, n, v); break;
+          case kSilu: run<kSilu, true>(e, n, v); break;
+          default: run<kNone, true>(e, n, v);
+        }
+      } else {
+        switch (e.act) {
+          case kRelu: run<kRelu, false>(e, n, v); break;
+          case kGelu: run<kGelu, false>(e, n, v); break;
+          case kGeluTanh: run<kGeluTanh, false>(e, n, v); break;
+          case kSilu: run<kSilu, false>(e, n, v); break;
+          default: break;
+        }
+      }
+      if (e.res && m < e.M) add(e.res + m * e.ldr, n, e, v);
+      uint32_t w[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) w[i] = Num<T>::pack(v[2 * i], v[2 * i + 1]);
+      stage_rows(buf, w, e.y, e.ldy, m - (threadIdx.x & 31), e.M, n, e.N, e.vec);
+    }
+    __device__ __forceinline__ void end(const EpiLinear&) {}
+
+    // v += row[n .. n + 31], as far as the columns go.
+    static __device__ __forceinline__ void add(const T* row, int64_t n, const EpiLinear& e, float* v) {
+      if (e.vec) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          if (n + 8 * g >= e.N) break;
+          const uint4 q = *reinterpret_cast<const uint4*>(row + n + 8 * g);
+          const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            v[8 * g + 2 * i] += Num<T>::lo(w[i]);
+            v[8 * g + 2 * i + 1] += Num<T>::hi(w[i]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (n + i < e.N) v[i] += Num<T>::to(row[n + i]);
+      }
+    }
+  };
+};
+
+// z[t, r] of weight_dot: from z, or the parts of a row that spans chunks, in order.
+struct DotValue {
+  const float* z;
+  const float* part;
+  int64_t rows, cols, chunk;
+  __device__ __forceinline__ float get(int64_t t, int64_t r) const {
+    const int64_t c0 = r * cols / chunk, c1 = ((r + 1) * cols - 1) / chunk;
+    if (c0 == c1) return z[t * rows + r];
+    float v = part[(2 * c0 + 1) * kDotRows + t];
+    for (int64_t c = c0 + 1; c <= c1; ++c) v += part[2 * c * kDotRows + t];
+    return v;
+  }
+};
+
+// y = act(z + bias) + residual from z = sum of the splits of acc, or from weight_dot; or
+// y = z * (a scale per row) for the gradient of a loss.
+template <typename T>
+struct Finish {
+  const float* acc;  // [splits][M][ld], or null: dot
+  int64_t M, N, ld;
+  int splits;
+  DotValue dot;
+  EpiLinear<T> lin;
+  // gradient of a loss: row m is scaled by T * grad / (rows that count for a mean) / gain
+  const float* grad;  // or null
+  int64_t grad_step;
+  const int32_t* count;
+  const float* mean_rows;  // or null
+  float factor;
+};
+
+template <typename T>
+__device__ __forceinline__ void finish_element(const Finish<T>& f, int64_t i) {
+  const int64_t m = i / f.N, n = i - m * f.N;
+  float z = 0.0f;
+  if (f.acc)
+    for (int s = 0; s < f.splits; ++s) z += f.acc[(s * f.M + m) * f.ld + n];
+  else z = f.dot.get(m, n);
+  const EpiLinear<T>& e = f.lin;
+  if (f.grad) {
+    if (f.count[m] == 0) z = 0.0f;
+    else z *= f.factor * f.grad[m * f.grad_step] / (f.mean_rows ? *f.mean_rows : 1.0f);
+    e.y[m * e.ldy + n] = Num<T>::from(z);
+    return;
+  }
+  if (e.bias) z += Num<T>::to(e.bias[n]);
+  float sl;
+  z = e.slope ? activate<true>(e.act, z, sl) : activate<false>(e.act, z, sl);
+  if (e.res) z += Num<T>::to(e.res[m * e.ldr + n]);
+  e.y[m * e.ldy + n] = Num<T>::from(z);
+  if (e.slope) e.slope[m * e.ldy + n] = int16_t(slope_code(sl));
+}
+
+// weight_dot, then f (whose dot it fills in) on every element.
+template <typename T>
+int weight_linear(const WeightBlob& w, void* temp, const void* x, int64_t ldx, int tokens, float* z, float* part,
+                  const Finish<T>& f, int32_t* status, cudaStream_t s);
+
+}  // namespace zn

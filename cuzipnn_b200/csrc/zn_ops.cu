@@ -16,8 +16,7 @@
 // backward pass computes a piece of them again.
 #include <algorithm>
 
-#include "zn_gemm.cuh"
-#include "zn_weight.cuh"
+#include "zn_linear.cuh"
 
 namespace zn {
 
@@ -54,162 +53,10 @@ int sm_count(int* sms) {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr int kNone = 0, kRelu = 1, kGelu = 2, kGeluTanh = 3, kSilu = 4;
 constexpr int kMean = 0, kRows = 2;  // reductions (1: sum)
 constexpr int kMaxTop = 256;
 
 // ---- epilogues ------------------------------------------------------------------------------
-
-// act(z) and its derivative (where asked for), in 32 bits.
-template <int ACT, bool SLOPE>
-__device__ __forceinline__ float activate(float z, float& slope) {
-  if constexpr (ACT == kRelu) {
-    if (SLOPE) slope = z > 0.0f ? 1.0f : 0.0f;
-    return z < 0.0f ? 0.0f : z;  // keeps NaN
-  } else if constexpr (ACT == kGelu) {
-    const float cdf = 0.5f * erfcf(-0.70710678118654752f * z);
-    if (SLOPE) slope = cdf + z * 0.3989422804014327f * __expf(-0.5f * z * z);
-    return z * cdf;
-  } else if constexpr (ACT == kGeluTanh) {  // 0.5 z (1 + tanh u) = z sigmoid(2u)
-    const float c = 0.7978845608028654f, z2 = z * z;
-    const float sig = __fdividef(1.0f, 1.0f + __expf(-2.0f * c * z * (1.0f + 0.044715f * z2)));
-    if (SLOPE) slope = sig + z * sig * (1.0f - sig) * 2.0f * c * (1.0f + 3.0f * 0.044715f * z2);
-    return z * sig;
-  } else if constexpr (ACT == kSilu) {
-    const float sig = __fdividef(1.0f, 1.0f + __expf(-z));
-    if (SLOPE) slope = sig * (1.0f + z * (1.0f - sig));
-    return z * sig;
-  } else {
-    if (SLOPE) slope = 1.0f;
-    return z;
-  }
-}
-template <bool SLOPE>
-__device__ __forceinline__ float activate(int act, float z, float& slope) {
-  switch (act) {
-    case kRelu: return activate<kRelu, SLOPE>(z, slope);
-    case kGelu: return activate<kGelu, SLOPE>(z, slope);
-    case kGeluTanh: return activate<kGeluTanh, SLOPE>(z, slope);
-    case kSilu: return activate<kSilu, SLOPE>(z, slope);
-    default: return activate<kNone, SLOPE>(z, slope);
-  }
-}
-
-// The derivative act'(z), kept for the backward pass as a 16-bit fixed-point number of step 2^-14
-// (every activation's lies in [-0.13, 1.13]): off by 2^-15 of a whole slope at most, an eighth of
-// a bf16 rounding, so the gradients are as exact as with a 32-bit slope.  -32768 stands for NaN.
-__device__ __forceinline__ int slope_code(float s) { return s != s ? -32768 : __float2int_rn(s * 16384.0f); }
-__device__ __forceinline__ float slope_value(int code) { return code == -32768 ? NAN : float(code) * (1.0f / 16384.0f); }
-
-// Per-warp staging: a thread holds 64 bytes (32 16-bit columns) of its own row; through shared
-// memory the warp writes them as 8 rows x 64 contiguous bytes per store.  The 16-byte chunks of a
-// row are permuted by the row, so that both sides touch every bank once.
-__device__ __forceinline__ uint4* stage_at(uint8_t* buf, int row, int chunk) {
-  return reinterpret_cast<uint4*>(buf + row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4));
-}
-// Rows m0 + r < M, columns n0 .. n0 + 31 < N of a 16-bit matrix from the warp's 16 words per thread.
-template <typename T>
-__device__ __forceinline__ void stage_rows(uint8_t* buf, const uint32_t* w, T* out, int64_t ld, int64_t m0, int64_t M,
-                                           int64_t n0, int64_t N, bool vec) {
-  const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) *stage_at(buf, lane, i) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-  __syncwarp();
-  if (vec) {  // 16-byte aligned rows, N a multiple of 8
-    const int64_t n = n0 + 8 * (lane & 3);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = 8 * i + (lane >> 2);
-      if (m0 + r < M && n < N) *reinterpret_cast<uint4*>(out + (m0 + r) * ld + n) = *stage_at(buf, r, lane & 3);
-    }
-  } else if (n0 + lane < N) {
-    const int rows = int(min(int64_t(32), M - m0));
-    for (int r = 0; r < rows; ++r)
-      out[(m0 + r) * ld + n0 + lane] = reinterpret_cast<const T*>(stage_at(buf, r, lane >> 3))[lane & 7];
-  }
-  __syncwarp();
-}
-
-// y = act(acc + bias) + residual, rounded once to 16 bits, and (where asked for) the slopes.
-template <typename T>
-struct EpiLinear {
-  const T* bias;  // or null
-  const T* res;   // or null
-  T* y;
-  int16_t* slope;  // or null
-  int64_t ldr, ldy, M, N;
-  int act;
-  bool vec;  // 16-byte accesses: every pointer and pitch allows them, and N is a multiple of 8
-
-  struct Row {
-    int64_t m, n0;
-    uint8_t* buf;
-    __device__ __forceinline__ Row(const EpiLinear&, int64_t m_, int64_t n0_, int, uint8_t* b) : m(m_), n0(n0_), buf(b) {}
-
-    template <int ACT, bool SLOPE>
-    __device__ __forceinline__ void run(const EpiLinear& e, int64_t n, float* v) {
-      uint32_t sw[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float s0, s1;
-        v[2 * i] = activate<ACT, SLOPE>(v[2 * i], s0);
-        v[2 * i + 1] = activate<ACT, SLOPE>(v[2 * i + 1], s1);
-        if (SLOPE) sw[i] = (uint32_t(slope_code(s0)) & 0xFFFFu) | (uint32_t(slope_code(s1)) << 16);
-      }
-      if (SLOPE) stage_rows(buf, sw, e.slope, e.ldy, m - (threadIdx.x & 31), e.M, n, e.N, e.vec);
-    }
-
-    __device__ __forceinline__ void cols(const EpiLinear& e, int c, float* v) {
-      const int64_t n = n0 + c;
-      if (n >= e.N) return;
-      if (e.bias) add(e.bias, n, e, v);
-      if (e.slope) {
-        switch (e.act) {
-          case kRelu: run<kRelu, true>(e, n, v); break;
-          case kGelu: run<kGelu, true>(e, n, v); break;
-          case kGeluTanh: run<kGeluTanh, true>(e, n, v); break;
-          case kSilu: run<kSilu, true>(e, n, v); break;
-          default: run<kNone, true>(e, n, v);
-        }
-      } else {
-        switch (e.act) {
-          case kRelu: run<kRelu, false>(e, n, v); break;
-          case kGelu: run<kGelu, false>(e, n, v); break;
-          case kGeluTanh: run<kGeluTanh, false>(e, n, v); break;
-          case kSilu: run<kSilu, false>(e, n, v); break;
-          default: break;
-        }
-      }
-      if (e.res && m < e.M) add(e.res + m * e.ldr, n, e, v);
-      uint32_t w[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) w[i] = Num<T>::pack(v[2 * i], v[2 * i + 1]);
-      stage_rows(buf, w, e.y, e.ldy, m - (threadIdx.x & 31), e.M, n, e.N, e.vec);
-    }
-    __device__ __forceinline__ void end(const EpiLinear&) {}
-
-    // v += row[n .. n + 31], as far as the columns go.
-    static __device__ __forceinline__ void add(const T* row, int64_t n, const EpiLinear& e, float* v) {
-      if (e.vec) {
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          if (n + 8 * g >= e.N) break;
-          const uint4 q = *reinterpret_cast<const uint4*>(row + n + 8 * g);
-          const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            v[8 * g + 2 * i] += Num<T>::lo(w[i]);
-            v[8 * g + 2 * i + 1] += Num<T>::hi(w[i]);
-          }
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (n + i < e.N) v[i] += Num<T>::to(row[n + i]);
-      }
-    }
-  };
-};
 
 // acc[split][m][n] (32 bits) = or += the tile: the parts of a contraction that is cut, across the
 // CTAs of one product or across the pieces of a weight.  finish_kernel adds the splits in order.
@@ -424,60 +271,11 @@ __global__ void __launch_bounds__(256) pitch_kernel(const uint16_t* src, int64_t
   }
 }
 
-// z[t, r] of weight_dot: from z, or the parts of a row that spans chunks, in order.
-struct DotValue {
-  const float* z;
-  const float* part;
-  int64_t rows, cols, chunk;
-  __device__ __forceinline__ float get(int64_t t, int64_t r) const {
-    const int64_t c0 = r * cols / chunk, c1 = ((r + 1) * cols - 1) / chunk;
-    if (c0 == c1) return z[t * rows + r];
-    float v = part[(2 * c0 + 1) * kDotRows + t];
-    for (int64_t c = c0 + 1; c <= c1; ++c) v += part[2 * c * kDotRows + t];
-    return v;
-  }
-};
-
-// y = act(z + bias) + residual from z = sum of the splits of acc, or from weight_dot; or
-// y = z * (a scale per row) for the gradient of a loss.
-template <typename T>
-struct Finish {
-  const float* acc;  // [splits][M][ld], or null: dot
-  int64_t M, N, ld;
-  int splits;
-  DotValue dot;
-  EpiLinear<T> lin;
-  // gradient of a loss: row m is scaled by T * grad / (rows that count for a mean) / gain
-  const float* grad;  // or null
-  int64_t grad_step;
-  const int32_t* count;
-  const float* mean_rows;  // or null
-  float factor;
-};
-
 template <typename T>
 __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Finish<T> f) {
+  pdl_wait();
   const int64_t total = f.M * f.N, step = int64_t(gridDim.x) * blockDim.x;
-  for (int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += step) {
-    const int64_t m = i / f.N, n = i - m * f.N;
-    float z = 0.0f;
-    if (f.acc)
-      for (int s = 0; s < f.splits; ++s) z += f.acc[(s * f.M + m) * f.ld + n];
-    else z = f.dot.get(m, n);
-    const EpiLinear<T>& e = f.lin;
-    if (f.grad) {
-      if (f.count[m] == 0) z = 0.0f;
-      else z *= f.factor * f.grad[m * f.grad_step] / (f.mean_rows ? *f.mean_rows : 1.0f);
-      e.y[m * e.ldy + n] = Num<T>::from(z);
-      continue;
-    }
-    if (e.bias) z += Num<T>::to(e.bias[n]);
-    float sl;
-    z = e.slope ? activate<true>(e.act, z, sl) : activate<false>(e.act, z, sl);
-    if (e.res) z += Num<T>::to(e.res[m * e.ldr + n]);
-    e.y[m * e.ldy + n] = Num<T>::from(z);
-    if (e.slope) e.slope[m * e.ldy + n] = int16_t(slope_code(sl));
-  }
+  for (int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += step) finish_element(f, i);
 }
 
 // dz = dy * slope in 16 bits (the operand of dx = dz W; dz null: not wanted) and the column sums of
@@ -612,6 +410,7 @@ __global__ void __launch_bounds__(128) loss_prep_kernel(const int64_t* ids, cons
 constexpr int kStatCols = 2048;
 __global__ void __launch_bounds__(256) dot_stats_kernel(DotValue v, LossRows rows, float* part, int64_t tokens,
                                                         float scale) {
+  pdl_wait();
   const int64_t m = blockIdx.y, n0 = int64_t(blockIdx.x) * kStatCols;
   const int64_t n1 = min(v.rows, n0 + kStatCols);
   const int count = rows.count[m];
@@ -655,6 +454,7 @@ __global__ void __launch_bounds__(256) dot_stats_kernel(DotValue v, LossRows row
 // Joins the tiles' statistics of 32 rows per block (in a fixed order) into lse and the rows' losses.
 __global__ void __launch_bounds__(1024) loss_rows_kernel(const float* part, int64_t tiles, int64_t tokens,
                                                          float temperature, LossRows rows, float* loss) {
+  pdl_wait();
   const int64_t m = int64_t(blockIdx.x) * 32 + (threadIdx.x & 31);
   const int sub = threadIdx.x >> 5;
   RowStats st{-INFINITY, 0.0f, 0.0f};
@@ -677,6 +477,7 @@ __global__ void __launch_bounds__(1024) loss_rows_kernel(const float* part, int6
 // Sum or mean over the rows that count, added in 64 bits by one block in a fixed order.
 __global__ void __launch_bounds__(1024) loss_reduce_kernel(const float* row_loss, LossRows rows, int64_t tokens,
                                                            bool mean, float* loss) {
+  pdl_wait();
   double s = 0.0;
   int64_t n = 0;
   for (int64_t m = threadIdx.x; m < tokens; m += 1024) {
@@ -769,6 +570,7 @@ int plan_weight(const zn_weight* w, int64_t rows_cap, int32_t* status, Arena& ar
   if (rows < w->rows) rows = std::max<int64_t>(256, rows / 256 * 256);
   out->piece_rows = std::min(rows, w->rows);
   out->pieces = cdiv(w->rows, out->piece_rows);
+  out->b.direct = !out->stored && weight_direct(out->b, out->pieces);
   if (!out->stored) {
     out->temp = ar.take(weight_temp_bytes(out->b));
     const int64_t chunks = std::min(cdiv(n, w->chunk_bytes), cdiv(out->piece_rows * w->cols, w->chunk_bytes) + 1);
@@ -779,7 +581,7 @@ int plan_weight(const zn_weight* w, int64_t rows_cap, int32_t* status, Arena& ar
 }
 
 int start_weight(const Weight& w, cudaStream_t s) {
-  if (!w.stored) return weight_scan(w.b, w.temp, w.status, s);
+  if (!w.stored) return w.b.direct ? ZN_OK : weight_scan(w.b, w.temp, w.status, s);
   const cudaError_t e = cudaMemsetAsync(w.status, 0, sizeof(int32_t), s);
   return e == cudaSuccess ? ZN_OK : set_error(ZN_ERR_CUDA, "status: %s", cudaGetErrorString(e));
 }
@@ -841,9 +643,7 @@ int product(const Matrix& a, const Matrix& b, const Cut& cut, const Epi& epi, in
 template <typename T>
 int run_finish(const Finish<T>& f, cudaStream_t s) {
   TimedLaunch tl("finish", s);
-  finish_kernel<T><<<grid_1d(f.M * f.N, 1024, 148 * 16), 256, 0, s>>>(f);
-  count_launch();
-  return check_launch("finish_kernel");
+  return launch_after(finish_kernel<T>, dim3(grid_1d(f.M * f.N, 256, 148 * 16)), 256, 0, s, "finish_kernel", f);
 }
 
 int bad(const char* what) { return set_error(ZN_ERR_INVALID, "%s: bad arguments", what); }
@@ -881,6 +681,7 @@ int plan_linear(const zn_weight* w, const void* x, int64_t ldx, int64_t tokens, 
   p->x_copy = plan_matrix(x, tokens, w->cols, ldx, ar);
   if (p->dot) {
     p->w.b = {static_cast<const uint8_t*>(w->blob), w->blob_bytes, w->rows, w->cols, w->chunk_bytes, w->dtype == 8};
+    p->w.b.direct = weight_direct(p->w.b, 1);
     p->w.status = status;
     p->w.temp = ar.take(weight_temp_bytes(p->w.b));
     p->acc = ar.take<float>(size_t(tokens) * w->rows * 4);
@@ -924,11 +725,9 @@ int run_linear(const LinearPlan& p, const void* x, int64_t ldx, int64_t tokens, 
   Finish<T> f{};
   f.M = tokens;
   if (p.dot) {
-    if (int rc = weight_dot(p.w.b, p.w.temp, xm.p, xm.pitch, int(tokens), p.acc, p.part, p.w.status, s)) return rc;
     f.N = rows;
-    f.dot = {p.acc, p.part, rows, cols, p.w.b.chunk};
     f.lin = linear_epilogue<T>(bias, res, ldr, y, slope, rows, tokens, 0, rows, act);
-    return run_finish(f, s);
+    return weight_linear<T>(p.w.b, p.w.temp, xm.p, xm.pitch, int(tokens), p.acc, p.part, f, p.w.status, s);
   }
   for (int64_t r0 = 0; r0 < rows; r0 += p.w.piece_rows) {
     const int64_t r1 = std::min(rows, r0 + p.w.piece_rows);
@@ -1067,6 +866,7 @@ int plan_loss(const zn_weight* w, const void* x, int64_t ldx, int64_t tokens, in
   p->dot = w->chunk_bytes > 0 && dot_shape(tokens, w->cols, w->chunk_bytes);
   if (p->dot) {
     p->w.b = {static_cast<const uint8_t*>(w->blob), w->blob_bytes, w->rows, w->cols, w->chunk_bytes, w->dtype == 8};
+    p->w.b.direct = weight_direct(p->w.b, 1);
     p->w.status = status;
     p->w.temp = ar.take(weight_temp_bytes(p->w.b));
     p->z = ar.take<float>(size_t(tokens) * w->rows * 4);
@@ -1096,9 +896,9 @@ int run_loss(const LossPlan& p, const void* x, int64_t ldx, int64_t tokens, cons
   if (p.dot) {
     if (int rc = weight_dot(p.w.b, p.w.temp, xm.p, xm.pitch, int(tokens), p.z, p.z_part, p.w.status, s)) return rc;
     const DotValue v{p.z, p.z_part, vocab, cols, p.w.b.chunk};
-    dot_stats_kernel<<<dim3(unsigned(p.tiles), unsigned(tokens)), 256, 0, s>>>(v, rows, p.part, tokens, kLog2e * inv_t);
-    count_launch();
-    if (int rc = check_launch("dot_stats_kernel")) return rc;
+    if (int rc = launch_after(dot_stats_kernel, dim3(unsigned(p.tiles), unsigned(tokens)), 256, 0, s, "dot_stats_kernel",
+                              v, rows, p.part, tokens, kLog2e * inv_t))
+      return rc;
   } else {
     for (int64_t r0 = 0; r0 < vocab; r0 += p.w.piece_rows) {
       const int64_t r1 = std::min(vocab, r0 + p.w.piece_rows);
@@ -1109,13 +909,12 @@ int run_loss(const LossPlan& p, const void* x, int64_t ldx, int64_t tokens, cons
     }
   }
   float* row_loss = reduction == kRows ? loss : p.row_loss;
-  loss_rows_kernel<<<unsigned(cdiv(tokens, 32)), 1024, 0, s>>>(p.part, p.tiles, tokens, temperature, rows, row_loss);
-  count_launch();
-  if (int rc = check_launch("loss_rows_kernel")) return rc;
+  if (int rc = launch_after(loss_rows_kernel, dim3(unsigned(cdiv(tokens, 32))), 1024, 0, s, "loss_rows_kernel",
+                            static_cast<const float*>(p.part), p.tiles, tokens, temperature, rows, row_loss))
+    return rc;
   if (reduction == kRows) return ZN_OK;
-  loss_reduce_kernel<<<1, 1024, 0, s>>>(row_loss, rows, tokens, reduction == kMean, loss);
-  count_launch();
-  return check_launch("loss_reduce_kernel");
+  return launch_after(loss_reduce_kernel, dim3(1), 1024, 0, s, "loss_reduce_kernel", static_cast<const float*>(row_loss),
+                      rows, tokens, reduction == kMean, loss);
 }
 
 // The backward pass's pieces are bounded so that P [tokens, piece] stays within 512 MB too.

@@ -1,6 +1,7 @@
 // Weights as operands (zn_weight.cuh): ranges of a blob's chunks decoded into a buffer, or multiplied
 // with a few vectors inside the decoder.
 #include "zn_decode.cuh"
+#include "zn_linear.cuh"
 
 namespace zn {
 namespace {
@@ -10,30 +11,86 @@ namespace {
 // Chunks [c0, c0 + gridDim.x) of one weight.
 template <bool REORDER, class Sink>
 __global__ void __launch_bounds__(kDecThreads) weight_kernel(const __grid_constant__ DecArgs a, int64_t c0,
-                                                             const __grid_constant__ Sink sink) {
-  decode_chunk<2, REORDER, 1>(a, c0 + blockIdx.x, false, sink);
+                                                             const __grid_constant__ Sink sink, uint32_t* counter) {
+  pdl_wait();
+  pdl_trigger();
+  if (blockIdx.x == 0 && threadIdx.x == 0) *counter = 0;
+  decode_chunk<2, REORDER, 1, true>(a, c0 + blockIdx.x, false, sink);
 }
 
-// The chunks of [c0, c1) with both planes coded.  Their flags were set by weight_kernel.
-template <bool REORDER, class Sink>
-__global__ void __launch_bounds__(kDecThreads) weight_overflow_kernel(const __grid_constant__ DecArgs a, int64_t c0,
-                                                                      int64_t c1, const __grid_constant__ Sink sink) {
-  __shared__ int64_t flagged[kDecThreads];
-  __shared__ int nflagged;
-  const int64_t stride = gridDim.x;
-  for (int64_t first = c0 + blockIdx.x; first < c1; first += stride * kDecThreads) {
-    const int64_t c = first + stride * threadIdx.x;
-    if (threadIdx.x == 0) nflagged = 0;
-    __syncthreads();
-    if (c < c1 && a.overflow[c]) flagged[atomicAdd(&nflagged, 1)] = c;
-    __syncthreads();
-    const int nf = nflagged;
-    for (int q = 0; q < nf; ++q) {
-      decode_chunk<2, REORDER, 2>(a, flagged[q], true, sink);
-      __syncthreads();
+// What the tail does once the weight's chunks are done (elements split over `n` threads).
+struct NoFin {
+  __device__ __forceinline__ void run(int64_t, int64_t) const {}
+};
+template <typename T>
+struct LinearFin {
+  Finish<T> f;
+  __device__ __forceinline__ void run(int64_t i, int64_t n) const {
+    for (; i < f.M * f.N; i += n) finish_element(f, i);
+  }
+};
+
+// After weight_kernel: the status from the chunks' flags, the chunks with both planes coded (whose
+// flags weight_kernel set), and `fin`.  Usually no chunk is left: every CTA sees that from the flags
+// and does its share of `fin` at once.  Otherwise the CTAs decode the flagged chunks, and the last
+// one to finish does all of `fin`.
+template <bool REORDER, class Sink, class Fin>
+__global__ void __launch_bounds__(kDecThreads) weight_tail_kernel(const __grid_constant__ DecArgs a, int64_t c0,
+                                                                  int64_t c1, const __grid_constant__ Sink sink,
+                                                                  const __grid_constant__ Fin fin, uint32_t* counter) {
+  __shared__ uint32_t s_any[kDecThreads / 32];
+  __shared__ uint32_t s_last;
+  pdl_wait();
+  pdl_trigger();
+  const int tid = threadIdx.x;
+  auto all_flags = [&] {  // OR of the chunks' flags, on every thread
+    uint32_t any = 0;
+    // Whole words in the middle (the array starts on an 8-byte boundary), bytes at the ends.
+    const int64_t w0 = (c0 + 3) / 4, w1 = c1 / 4;
+    const volatile uint32_t* words = reinterpret_cast<const volatile uint32_t*>(a.overflow);
+    const volatile uint8_t* bytes = a.overflow;
+#pragma unroll 4
+    for (int64_t i = w0 + tid; i < w1; i += kDecThreads) any |= words[i];
+    any |= any >> 16;
+    any |= any >> 8;
+    if (w0 <= w1) {
+      if (c0 + tid < 4 * w0) any |= bytes[c0 + tid];
+      if (4 * w1 + tid < c1) any |= bytes[4 * w1 + tid];
+    } else if (c0 + tid < c1) {
+      any |= bytes[c0 + tid];
     }
+    any = __reduce_or_sync(0xFFFFFFFFu, any & 0xFF);
+    __syncthreads();
+    if ((tid & 31) == 0) s_any[tid >> 5] = any;
+    __syncthreads();
+    any = 0;
+#pragma unroll
+    for (int w = 0; w < kDecThreads / 32; ++w) any |= s_any[w];
+    return any;
+  };
+  const uint32_t any = all_flags();
+  auto report = [&](uint32_t flags) {
+    if (tid == 0) *a.status = (a.mode == kDirect ? 0 : *a.status) | int32_t(flags & ~uint32_t(kChunkOver));
+  };
+  if (!(any & kChunkOver)) {
+    if (blockIdx.x == 0) report(any);
+    fin.run(int64_t(blockIdx.x) * kDecThreads + tid, int64_t(gridDim.x) * kDecThreads);
+    return;
+  }
+  for (int64_t c = c0 + blockIdx.x; c < c1; c += gridDim.x) {
+    if (!(a.overflow[c] & kChunkOver)) continue;  // uniform: this CTA alone changes the flag's other bits
+    __syncthreads();
+    decode_chunk<2, REORDER, 2, true>(a, c, true, sink);
     __syncthreads();
   }
+  __threadfence();
+  __syncthreads();
+  if (tid == 0) s_last = atomicAdd(counter, 1) == gridDim.x - 1;
+  __syncthreads();
+  if (!s_last) return;
+  __threadfence();
+  report(all_flags());
+  fin.run(tid, kDecThreads);
 }
 
 template <class Sink>
@@ -42,38 +99,37 @@ constexpr size_t sink_smem() {
   else return 0;
 }
 
-template <bool REORDER, class Sink>
-int launch_weight(const DecArgs& a, int64_t c0, int64_t c1, const Sink& sink, cudaStream_t s) {
+// `work`: elements of `fin`.
+template <bool REORDER, class Sink, class Fin>
+int launch_weight(const DecArgs& a, int64_t c0, int64_t c1, const Sink& sink, const Fin& fin, int64_t work,
+                  cudaStream_t s) {
   if (c1 <= c0) return ZN_OK;
+  uint32_t* counter = reinterpret_cast<uint32_t*>(a.overflow + ((a.nch + 3) & ~int64_t(3)));
   {
     auto fn = weight_kernel<REORDER, Sink>;
     const size_t sm = dec_smem(1) + sink_smem<Sink>();
     if (int rc = set_max_smem(reinterpret_cast<const void*>(fn), int(sm))) return rc;
     TimedLaunch tl("decode", s);
-    fn<<<unsigned(c1 - c0), kDecThreads, sm, s>>>(a, c0, sink);
+    if (int rc = launch_after(fn, dim3(unsigned(c1 - c0)), kDecThreads, sm, s, "weight_kernel", a, c0, sink, counter))
+      return rc;
   }
-  count_launch();
-  if (int rc = check_launch("weight_kernel")) return rc;
-  auto fn = weight_overflow_kernel<REORDER, Sink>;
+  auto fn = weight_tail_kernel<REORDER, Sink, Fin>;
   const size_t sm = dec_smem(2) + sink_smem<Sink>();
   if (int rc = set_max_smem(reinterpret_cast<const void*>(fn), int(sm))) return rc;
-  int dev = 0, sms = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  if (e != cudaSuccess) return set_error(ZN_ERR_CUDA, "weight_overflow_kernel: %s", cudaGetErrorString(e));
+  int sms = 0;
+  if (int rc = sm_count(&sms)) return rc;
+  const int64_t grid = min(max(c1 - c0, cdiv(work, kDecThreads)), int64_t(2 * sms));
   TimedLaunch tl("decode_overflow", s);
-  fn<<<unsigned(min(c1 - c0, int64_t(2 * sms))), kDecThreads, sm, s>>>(a, c0, c1, sink);
-  count_launch();
-  return check_launch("weight_overflow_kernel");
+  return launch_after(fn, dim3(unsigned(grid)), kDecThreads, sm, s, "weight_tail_kernel", a, c0, c1, sink, fin, counter);
 }
 
-template <typename T, bool REORDER>
+template <typename T, bool REORDER, class Fin>
 int launch_dot(const DecArgs& a, const WeightBlob& w, const void* x, int64_t ldx, int tokens, float* z, float* part,
-               cudaStream_t s) {
+               const Fin& fin, int64_t work, cudaStream_t s) {
   auto go = [&](auto mt) {
     constexpr int MT = decltype(mt)::value;
     DotSink<T, MT> k{static_cast<const T*>(x), ldx, w.cols, w.rows, tokens, z, part};
-    return launch_weight<REORDER>(a, 0, a.nch, k, s);
+    return launch_weight<REORDER>(a, 0, a.nch, k, fin, work, s);
   };
   if (tokens == 1) return go(std::integral_constant<int, 1>());
   if (tokens == 2) return go(std::integral_constant<int, 2>());
@@ -84,13 +140,14 @@ int launch_dot(const DecArgs& a, const WeightBlob& w, const void* x, int64_t ldx
 }  // namespace
 
 size_t weight_temp_bytes(const WeightBlob& w) {
-  return job_structs_bytes<DecArgs>(1) + dec_job_bytes(w.rows * w.cols, 2, w.chunk);
+  return job_structs_bytes<DecArgs>(1) + dec_job_bytes(w.rows * w.cols, 2, w.chunk) + 256;  // + the counter
 }
 
 int weight_decode(const WeightBlob& w, void* temp, int64_t c0, int64_t c1, void* out, int32_t* status, cudaStream_t s) {
-  DecArgs a = weight_args(w, temp, status);
+  DecArgs a = weight_args(w, temp, status, w.direct ? kDirect : kScanned);
   a.out = static_cast<uint8_t*>(out) - c0 * w.chunk * 2;
-  return w.bf16 ? launch_weight<true>(a, c0, c1, StoreSink(), s) : launch_weight<false>(a, c0, c1, StoreSink(), s);
+  return w.bf16 ? launch_weight<true>(a, c0, c1, StoreSink(), NoFin(), 0, s)
+                : launch_weight<false>(a, c0, c1, StoreSink(), NoFin(), 0, s);
 }
 
 int weight_wave(const WeightBlob& w, int64_t* chunks) {
@@ -109,9 +166,22 @@ size_t dot_part_bytes(const WeightBlob& w) { return size_t(weight_chunks(w)) * 2
 
 int weight_dot(const WeightBlob& w, void* temp, const void* x, int64_t ldx, int tokens, float* z, float* part,
                int32_t* status, cudaStream_t s) {
-  const DecArgs a = weight_args(w, temp, status);
-  return w.bf16 ? launch_dot<__nv_bfloat16, true>(a, w, x, ldx, tokens, z, part, s)
-                : launch_dot<__half, false>(a, w, x, ldx, tokens, z, part, s);
+  const DecArgs a = weight_args(w, temp, status, w.direct ? kDirect : kScanned);
+  return w.bf16 ? launch_dot<__nv_bfloat16, true>(a, w, x, ldx, tokens, z, part, NoFin(), 0, s)
+                : launch_dot<__half, false>(a, w, x, ldx, tokens, z, part, NoFin(), 0, s);
 }
+
+template <typename T>
+int weight_linear(const WeightBlob& w, void* temp, const void* x, int64_t ldx, int tokens, float* z, float* part,
+                  const Finish<T>& f, int32_t* status, cudaStream_t s) {
+  const DecArgs a = weight_args(w, temp, status, w.direct ? kDirect : kScanned);
+  LinearFin<T> fin{f};
+  fin.f.dot = {z, part, w.rows, w.cols, w.chunk};
+  return launch_dot<T, Num<T>::kCode == 1>(a, w, x, ldx, tokens, z, part, fin, f.M * f.N, s);
+}
+template int weight_linear<__nv_bfloat16>(const WeightBlob&, void*, const void*, int64_t, int, float*, float*,
+                                          const Finish<__nv_bfloat16>&, int32_t*, cudaStream_t);
+template int weight_linear<__half>(const WeightBlob&, void*, const void*, int64_t, int, float*, float*,
+                                   const Finish<__half>&, int32_t*, cudaStream_t);
 
 }  // namespace zn

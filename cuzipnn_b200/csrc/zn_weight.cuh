@@ -13,6 +13,7 @@ struct WeightBlob {
   int64_t rows, cols;
   int64_t chunk;  // elements per chunk
   bool bf16;      // else fp16
+  bool direct;    // every chunk finds its units itself, without weight_scan (weight_direct)
 };
 
 // Rows of one product inside the decoder, and the shape rule of that path (see DotSink).
@@ -23,11 +24,16 @@ inline bool dot_shape(int64_t tokens, int64_t cols, int64_t chunk) {
 }
 
 inline int64_t weight_chunks(const WeightBlob& w) { return cdiv(w.rows * w.cols, w.chunk); }
-// Scratch of one weight (unit offsets, overflow flags), filled by weight_scan.
+// Scratch of one weight (unit offsets, the chunks' flags, a counter).
 size_t weight_temp_bytes(const WeightBlob& w);
-// First step of every call: the offsets of the blob's units; sets the status word to 0 or errors.
+// Whether a weight decoded by one call is better off without the scan of its tables: up to 2048
+// chunks, where the 24 KB of tables that a chunk's CTA then reads cost it about 2 us, against 6 us
+// or more of a kernel before all others.
+inline bool weight_direct(const WeightBlob& w, int64_t pieces) { return pieces == 1 && weight_chunks(w) <= 2048; }
+// First step of a call unless w.direct: the offsets of the blob's units; sets the status word.
 int weight_scan(const WeightBlob& w, void* temp, int32_t* status, cudaStream_t s);
-// Decode chunks [c0, c1) to `out` (the address of chunk c0's first element, 16-byte aligned).
+// Decode chunks [c0, c1) to `out` (the address of chunk c0's first element, 16-byte aligned).  Sets
+// the status word (w.direct) or adds to it.
 int weight_decode(const WeightBlob& w, void* temp, int64_t c0, int64_t c1, void* out, int32_t* status, cudaStream_t s);
 // Chunks that the decoder works on at once on this device (its resident blocks).
 int weight_wave(const WeightBlob& w, int64_t* chunks);
@@ -37,6 +43,7 @@ int weight_wave(const WeightBlob& w, int64_t* chunks);
 // w.rows); the parts of rows that span chunks go to `part` ([chunk][2][kDotRows], dot_part_bytes):
 // slot 1 holds the part of a row that starts in the chunk, slot 0 of one that started before it.
 size_t dot_part_bytes(const WeightBlob& w);
+// Without w.direct, weight_scan comes first.
 int weight_dot(const WeightBlob& w, void* temp, const void* x, int64_t ldx, int tokens, float* z, float* part,
                int32_t* status, cudaStream_t s);
 
