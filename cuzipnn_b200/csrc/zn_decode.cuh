@@ -299,7 +299,7 @@ __device__ __forceinline__ void decode_round(Cursor* cb, const uint32_t* __restr
 __device__ __forceinline__ void decode_round_fast(Cursor* cb, const uint32_t* __restrict__ tab, const uint8_t* rows,
                                                   int tid, uint32_t (*acc)[4]) {
   constexpr uint32_t kRowBytes = kDecThreads * 4, kRingBytes = kRing * kRowBytes;
-  uint32_t xv[kChains], ro[kChains], ro0[kChains], wn[kChains];
+  uint32_t xv[kChains], ro[kChains], ro0[kChains], wn[kChains], pair[kChains];
 #pragma unroll
   for (int c = 0; c < kChains; ++c) {
     xv[c] = cb[c].x;
@@ -311,13 +311,16 @@ __device__ __forceinline__ void decode_round_fast(Cursor* cb, const uint32_t* __
   _Pragma("unroll") for (int c = 0; c < kChains; ++c) {                                               \
     const uint32_t e = tab[xv[c] & (kM - 1)];                                                         \
     const uint32_t xn = (e >> 20) * (xv[c] >> kScaleBits) + (e & 0xFFFu);                             \
-    acc[c][(I) >> 2] = __byte_perm(acc[c][(I) >> 2], e >> 12,                                         \
-                                   (0x3210 & ~(0xF << (4 * ((I) & 3)))) | (4 << (4 * ((I) & 3))));    \
     const bool need = xn < kL;                                                                        \
     const uint32_t w = wn[c];                                                                         \
     ro[c] = need ? ((ro[c] + kRowBytes) & (kRingBytes - 1)) : ro[c];                                  \
     wn[c] = *reinterpret_cast<const uint32_t*>(rows + c * kRingBytes + ro[c]);                        \
     xv[c] = need ? __byte_perm(w, xn, 0x5410) : xn;                                                   \
+    /* Symbols (bits 12-19 of the entries) four at a time: two entries' middle bytes side by side,  \
+       shifted to the byte boundary, then one byte of each. */                                        \
+    if (((I) & 1) == 0) pair[c] = e;                                                                  \
+    else if (((I) & 3) == 1) acc[c][(I) >> 2] = __byte_perm(pair[c], e, 0x6521) >> 4;                 \
+    else acc[c][(I) >> 2] = __byte_perm(acc[c][(I) >> 2], __byte_perm(pair[c], e, 0x6521) >> 4, 0x6420); \
   }
   ZN_FSTEP(0) ZN_FSTEP(1) ZN_FSTEP(2) ZN_FSTEP(3) ZN_FSTEP(4) ZN_FSTEP(5) ZN_FSTEP(6) ZN_FSTEP(7)
   ZN_FSTEP(8) ZN_FSTEP(9) ZN_FSTEP(10) ZN_FSTEP(11) ZN_FSTEP(12) ZN_FSTEP(13) ZN_FSTEP(14) ZN_FSTEP(15)
@@ -398,96 +401,125 @@ struct StoreSink {
 //
 // A lane's 16 elements of a round lie in one row (cols and the chunk size are multiples of 16), and
 // a row is at least one round (128 elements) long, so a segment (8 lanes, one sub-chunk) crosses at
-// most one row end per round.  Each lane sums its own products in 32 bits; at a row end the 8 sums
-// are added by a fixed tree.  A row inside one sub-chunk is complete then and goes to z.  Parts of
-// rows that span sub-chunks go to shared slots (per sub-chunk: 0 = the row started before it, 1 =
-// it starts here and goes on), which the CTA adds in order at the end; rows that span chunks leave
-// their parts in `part` with the same rule per chunk.  No atomics: the result does not depend on
-// the order in which chunks are decoded.
+// most one row end per round.  The products are taken by mma.m16n8k16 with 32-bit sums, although
+// every lane has its own place in W and x: with a lane's words of W as its part of A's rows 0-7 and
+// the matching words of x as its part of B, the diagonal element D[r, r] is the sum of the own
+// products of lanes 4r .. 4r + 3, whatever these are (the other elements mean nothing and are
+// dropped).  4 such steps take the lane's 16 elements as they are packed; with scalar arithmetic
+// their 32 conversions and 16 dependent additions made one token's product 30 % slower than the
+// decoding alone.  At a row end the segment's two diagonal elements are added, and lanes beyond it
+// start the next row.
+//
+// A row inside one sub-chunk is complete then and goes to z.  Parts of rows that span sub-chunks go
+// to shared slots (per sub-chunk: 0 = the row started before it, 1 = it starts here and goes on),
+// which the CTA adds in order at the end; rows that span chunks leave their parts in `part` with the
+// same rule per chunk.  No atomics: the result does not depend on the order in which chunks are
+// decoded.
 template <typename T, int MT>
 struct DotSink {
   static constexpr bool kDot = true;
   static constexpr int kRows = MT;
-  static constexpr bool kAhead = MT <= 2;  // x is loaded a round ahead (8 registers per row)
+  static constexpr bool kAhead = MT == 1;  // x is loaded before the round is decoded (8 registers)
   using Elem = T;
   const T* x;
-  int64_t ldx, cols, rows;
-  int tokens;
+  int64_t ldx, rows;
+  int cols, tokens;
   float* z;     // [tokens][rows]
   float* part;  // [chunk][2][kDotRows]
 };
 
-__device__ __forceinline__ float2 unpack2(uint32_t w, __nv_bfloat16) {
-  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
-}
-__device__ __forceinline__ float2 unpack2(uint32_t w, __half) {
-  return __half22float2(*reinterpret_cast<const __half2*>(&w));
-}
-
 template <int MT>
 struct DotState {
-  float acc[MT];
-  int col;      // of the segment's first element in its current row (of the round before)
-  int64_t row;  // the segment's current row
-  bool first;   // no row end met in this sub-chunk yet
-  bool mid;     // the sub-chunk starts inside a row
-  uint4 x[MT][2];  // the next round's elements of x
+  float c[MT][2];  // row lane / 4, columns 2 (lane % 4) and + 1 of each accumulator
+  int col;         // of the segment's first element in its current row (of the round before)
+  int row;         // the segment's current row
+  bool first;      // no row end met in this sub-chunk yet
+  bool mid;        // the sub-chunk starts inside a row
+  uint4 x[2];      // kAhead: the round's elements of x
 };
 
-// Loads the next round's elements of x (those of row 0 for rows past the last; lanes without
-// elements load valid ones too).  Called before the round is decoded, which hides the latency.
+// Column of the next round's elements (lanes without elements get a valid one too).
 template <class Sink>
-__device__ __forceinline__ void dot_load(const Sink& k, DotState<Sink::kRows>& st, int l) {
-  int col = st.col + kRound + l * kSteps;
-  if (col >= k.cols) col -= int(k.cols);
+__device__ __forceinline__ int dot_col(const Sink& k, const DotState<Sink::kRows>& st, int l) {
+  const int col = st.col + kRound + l * kSteps;
+  return col >= k.cols ? col - k.cols : col;
+}
+template <class Sink>
+__device__ __forceinline__ void dot_load(const Sink& k, int m, int col, uint4* x) {
+  const uint4* xp = reinterpret_cast<const uint4*>(k.x + m * k.ldx + col);
+  x[0] = __ldg(xp);
+  x[1] = __ldg(xp + 1);
+}
+
+// One step of the products: rows 0-7 of A from a0, a2, rows 8-15 zero.
+__device__ __forceinline__ void dot_mma(float* c, uint32_t a0, uint32_t a2, uint32_t b0, uint32_t b1, __nv_bfloat16) {
+  [[maybe_unused]] float d2, d3;
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %5}, {%7, %8}, {%9, %10, %11, %11};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(d2), "=f"(d3)
+      : "r"(a0), "r"(0u), "r"(a2), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(0.0f));
+}
+__device__ __forceinline__ void dot_mma(float* c, uint32_t a0, uint32_t a2, uint32_t b0, uint32_t b1, __half) {
+  [[maybe_unused]] float d2, d3;
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %5}, {%7, %8}, {%9, %10, %11, %11};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(d2), "=f"(d3)
+      : "r"(a0), "r"(0u), "r"(a2), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(0.0f));
+}
+// Lanes with `use` add their products, the others nothing (both factors are zeroed: 0 * inf is NaN).
+template <class Sink, bool MASKED>
+__device__ __forceinline__ void dot_products(const Sink& k, DotState<Sink::kRows>& st, const uint32_t* e, int col,
+                                             bool use) {
+  uint32_t w[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = !MASKED || use ? e[i] : 0u;
 #pragma unroll
   for (int m = 0; m < Sink::kRows; ++m) {
-    const uint4* xp = reinterpret_cast<const uint4*>(k.x + (m < k.tokens ? m * k.ldx : 0) + col);
-    st.x[m][0] = __ldg(xp);
-    st.x[m][1] = __ldg(xp + 1);
+    uint4 q[2];
+    if constexpr (Sink::kAhead) {
+      q[0] = st.x[0];
+      q[1] = st.x[1];
+    } else {
+      dot_load(k, m < k.tokens ? m : 0, col, q);
+    }
+    uint32_t x[8] = {q[0].x, q[0].y, q[0].z, q[0].w, q[1].x, q[1].y, q[1].z, q[1].w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (MASKED && !use) x[i] = 0u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) dot_mma(st.c[m], w[2 * i], w[2 * i + 1], x[2 * i], x[2 * i + 1], typename Sink::Elem());
   }
 }
 
+// The segment's sums (on all its lanes): its two quads' diagonal elements.
 template <int MT>
-__device__ __forceinline__ void segment_sum(float* v, uint32_t mask) {
+__device__ __forceinline__ void segment_sum(const DotState<MT>& st, float* v) {
+  const int lane = threadIdx.x & 31, quad = lane >> 2;
+  const bool mine = (lane & 3) == (quad >> 1);
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
+  for (int m = 0; m < MT; ++m) {
+    v[m] = mine ? ((quad & 1) ? st.c[m][1] : st.c[m][0]) : 0.0f;
 #pragma unroll
-    for (int o = 4; o; o >>= 1) v[m] += __shfl_xor_sync(mask, v[m], o);
+    for (int o = 4; o; o >>= 1) v[m] += __shfl_xor_sync(0xFFFFFFFFu, v[m], o);
+  }
 }
 
-// One round of a segment: 16 elements per lane (8 words), none for inactive lanes.
-template <class Sink>
+// One round of a warp's segments: 16 elements per lane (8 words), none for inactive lanes.  Called
+// by whole warps.
+template <class Sink, bool ALL>
 __device__ __forceinline__ void dot_round(const Sink& k, DotState<Sink::kRows>& st, const uint32_t* e, bool active,
-                                          int l, uint32_t mask, float* slot0) {
+                                          int l, int seg, float* slot0) {
   constexpr int MT = Sink::kRows;
-  if constexpr (!Sink::kAhead) dot_load(k, st, l);
+  const int col = dot_col(k, st, l);
   st.col += kRound;
   const bool wrapped = active && st.col + l * kSteps >= k.cols;  // the lane's elements lie in the next row
-  float d[MT];
-#pragma unroll
-  for (int m = 0; m < MT; ++m) d[m] = 0.0f;
-  if (active) {
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const uint4 a = st.x[m][0], b = st.x[m][1];
-      const uint32_t xw[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float2 w2 = unpack2(e[i], typename Sink::Elem()), x2 = unpack2(xw[i], typename Sink::Elem());
-        d[m] = fmaf(w2.x, x2.x, d[m]);
-        d[m] = fmaf(w2.y, x2.y, d[m]);
-      }
-    }
+  const uint32_t over = __ballot_sync(0xFFFFFFFFu, wrapped);
+  if (!over) {
+    dot_products<Sink, !ALL>(k, st, e, col, active);
+    return;
   }
-  if (__any_sync(mask, wrapped)) {
-    float v[MT];
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      v[m] = st.acc[m] + (wrapped ? 0.0f : d[m]);
-      st.acc[m] = wrapped ? d[m] : 0.0f;
-    }
-    segment_sum<MT>(v, mask);
+  dot_products<Sink, true>(k, st, e, col, active && !wrapped);
+  float v[MT];
+  segment_sum<MT>(st, v);
+  if ((over >> (8 * seg)) & 0xFF) {
     if (l == 0) {
 #pragma unroll
       for (int m = 0; m < MT; ++m)
@@ -496,13 +528,13 @@ __device__ __forceinline__ void dot_round(const Sink& k, DotState<Sink::kRows>& 
           else k.z[m * k.rows + st.row] = v[m];
         }
     }
+#pragma unroll
+    for (int m = 0; m < MT; ++m) st.c[m][0] = st.c[m][1] = 0.0f;
     st.first = false;
     ++st.row;
-    st.col -= int(k.cols);  // below 0 when the row ended inside the round
-  } else {
-#pragma unroll
-    for (int m = 0; m < MT; ++m) st.acc[m] += d[m];
+    st.col -= k.cols;  // below 0 when the row ended inside the round
   }
+  dot_products<Sink, true>(k, st, e, col, wrapped);
 }
 
 // The rows of chunk j (elements [g0, g1)) that no single sub-chunk completed: the sums of their
@@ -777,13 +809,12 @@ __device__ __forceinline__ void decode_chunk(const DecArgs& a, int64_t j, bool o
     uint32_t pn[kChains][K][4];
     load_raw_round<K, kChains>(src, coded, base, len, 0, l, pn);
     int r = 0;
-    [[maybe_unused]] const uint32_t seg_mask = 0xFFu << (8 * seg);
     [[maybe_unused]] auto dot = [&] {
       if constexpr (Sink::kDot) {
         DotState<Sink::kRows> st{};
         const int64_t e0 = j * a.C + base[0];
-        st.row = e0 / sink.cols;
-        const int c0 = int(e0 - st.row * sink.cols);
+        st.row = int(e0 / sink.cols);
+        const int c0 = int(e0 - int64_t(st.row) * sink.cols);
         st.col = c0 - kRound;  // dot_round advances it by a round first
         st.first = true;
         st.mid = c0 != 0;
@@ -803,8 +834,8 @@ __device__ __forceinline__ void decode_chunk(const DecArgs& a, int64_t j, bool o
       uint32_t end8[kChains], off[kChains];  // off: element offset of the lane's round r in the chunk
 #pragma unroll
       for (int c = 0; c < kChains; ++c) {
-        // A product's segments need all 8 lanes in every round of this loop.
-        if constexpr (Sink::kDot) rfull = int(len[c] / kRound);
+        // Products are taken by whole warps: rounds that are full for all lanes of all segments.
+        if constexpr (Sink::kDot) rfull = int(__reduce_min_sync(0xFFFFFFFFu, uint32_t(len[c] / kRound)));
         else rfull = min(rfull, len[c] >= l16 + kSteps ? int((len[c] - l16 - kSteps) / kRound) + 1 : 0);
         end8[c] = (cur[0][c].end + 7) & ~7u;
         off[c] = uint32_t(base[c] + l16);
@@ -839,7 +870,7 @@ __device__ __forceinline__ void decode_chunk(const DecArgs& a, int64_t j, bool o
             }
           }
           if constexpr (Sink::kDot)
-            if constexpr (Sink::kAhead) dot_load(sink, dot, l);
+            if constexpr (Sink::kAhead) dot_load(sink, 0, dot_col(sink, dot, l), dot.x);
           uint32_t p[kChains][K][4];
 #pragma unroll
           for (int c = 0; c < kChains; ++c)
@@ -881,7 +912,7 @@ __device__ __forceinline__ void decode_chunk(const DecArgs& a, int64_t j, bool o
           for (int c = 0; c < kChains; ++c) {
             uint32_t e[4 * K];
             assemble_elements<K, REORDER>(p[c], e);
-            if constexpr (Sink::kDot) dot_round(sink, dot, e, true, l, seg_mask, slot0);
+            if constexpr (Sink::kDot) dot_round<Sink, true>(sink, dot, e, true, l, seg, slot0);
             else store_words(outc + size_t(off[c]) * K, e, 4 * K, out16);  // 16-byte aligned when outc is
             off[c] += kRound;
           }
@@ -928,7 +959,7 @@ __device__ __forceinline__ void decode_chunk(const DecArgs& a, int64_t j, bool o
           for (int i = 0; i < 4; ++i) p[c][b][i] = pn[c][b][i];
       if (r + 1 < rounds) load_raw_round<K, kChains>(src, coded, base, len, r + 1, l, pn);
       if constexpr (Sink::kDot)
-        if constexpr (Sink::kAhead) dot_load(sink, dot, l);
+        if constexpr (Sink::kAhead) dot_load(sink, 0, dot_col(sink, dot, l), dot.x);
       const bool full = nact[0] == kSteps && nact[kChains - 1] == kSteps;
 #pragma unroll
       for (int q = 0; q < KC; ++q) {
@@ -964,7 +995,7 @@ __device__ __forceinline__ void decode_chunk(const DecArgs& a, int64_t j, bool o
         uint32_t e[4 * K];
         assemble_elements<K, REORDER>(p[c], e);
         if constexpr (Sink::kDot) {
-          dot_round(sink, dot, e, nact[c] == kSteps, l, seg_mask, slot0);
+          dot_round<Sink, false>(sink, dot, e, nact[c] == kSteps, l, seg, slot0);
           continue;
         }
         uint8_t* dst = outc + (base[c] + off[c]) * K;
@@ -985,16 +1016,17 @@ __device__ __forceinline__ void decode_chunk(const DecArgs& a, int64_t j, bool o
       for (int c = 0; c < kChains; ++c)
         if (q < ncoded && valid[c]) err |= (cur[q][c].x != kL) || (cur[q][c].ptr != cur[q][c].end);
     if constexpr (Sink::kDot) {
+      float sum[Sink::kRows];
+      segment_sum<Sink::kRows>(dot, sum);
       if (valid[0]) {  // the row that the sub-chunk ends in
-        segment_sum<Sink::kRows>(dot.acc, seg_mask);
         const int64_t e1 = j * a.C + base[0] + len[0];
         const bool ended = e1 % sink.cols == 0, here = !(dot.first && dot.mid);
         if (l == 0) {
 #pragma unroll
           for (int mm = 0; mm < Sink::kRows; ++mm)
             if (mm < sink.tokens) {
-              if (ended && here) sink.z[mm * sink.rows + dot.row] = dot.acc[mm];
-              else slot0[(here ? Sink::kRows : 0) + mm] = dot.acc[mm];
+              if (ended && here) sink.z[mm * sink.rows + dot.row] = sum[mm];
+              else slot0[(here ? Sink::kRows : 0) + mm] = sum[mm];
             }
         }
       }

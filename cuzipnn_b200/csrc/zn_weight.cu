@@ -8,9 +8,16 @@ namespace {
 
 // ---- a weight's chunks (zn_weight.cuh) -------------------------------------------------------
 
+// CTAs per SM that the registers have to allow.
+template <class Sink>
+constexpr int weight_blocks() {
+  if constexpr (Sink::kDot) return Sink::kRows <= 1 ? 5 : 4;
+  else return 5;
+}
+
 // Chunks [c0, c0 + gridDim.x) of one weight.
 template <bool REORDER, class Sink>
-__global__ void __launch_bounds__(kDecThreads) weight_kernel(const __grid_constant__ DecArgs a, int64_t c0,
+__global__ void __launch_bounds__(kDecThreads, weight_blocks<Sink>()) weight_kernel(const __grid_constant__ DecArgs a, int64_t c0,
                                                              const __grid_constant__ Sink sink, uint32_t* counter) {
   pdl_wait();
   pdl_trigger();
@@ -128,12 +135,11 @@ int launch_dot(const DecArgs& a, const WeightBlob& w, const void* x, int64_t ldx
                const Fin& fin, int64_t work, cudaStream_t s) {
   auto go = [&](auto mt) {
     constexpr int MT = decltype(mt)::value;
-    DotSink<T, MT> k{static_cast<const T*>(x), ldx, w.cols, w.rows, tokens, z, part};
+    DotSink<T, MT> k{static_cast<const T*>(x), ldx, w.rows, int(w.cols), tokens, z, part};
     return launch_weight<REORDER>(a, 0, a.nch, k, fin, work, s);
   };
   if (tokens == 1) return go(std::integral_constant<int, 1>());
   if (tokens == 2) return go(std::integral_constant<int, 2>());
-  if (tokens <= 4) return go(std::integral_constant<int, 4>());
   return go(std::integral_constant<int, kDotRows>());
 }
 
