@@ -28,6 +28,8 @@ _ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 _REDUCTIONS = {"mean": 0, "sum": 1, "none": 2}
 _MAX_TOP = 256
 _MAX_DIM = 1 << 31
+_ENTRIES = {name: (getattr(_lib.lib, name + "_temp_bytes"), getattr(_lib.lib, name))
+            for name in ("zn_linear", "zn_linear_grad", "zn_loss", "zn_loss_grad")}
 
 
 def upload_blob(blob: torch.Tensor, *, compute_device: torch.device | str | None = None) -> torch.Tensor:
@@ -117,15 +119,20 @@ class _Weight:
         """Run entry point `name` on the device's current stream: scratch from <name>_temp_bytes
         (with the `query` arguments), then (weight, *args, status, scratch, stream)."""
         w = ctypes.byref(self.desc)
-        nbytes = int(getattr(_lib.lib, name + "_temp_bytes")(w, *query))
-        temp = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=self.device)
-        _lib.check(getattr(_lib.lib, name)(w, *args, status.data_ptr(), temp.data_ptr(), nbytes,
-                                           _stream(self.device)), name)
+        temp_bytes, run = _ENTRIES[name]
+        nbytes = temp_bytes(w, *query)
+        temp = torch.empty(nbytes or 1, dtype=torch.uint8, device=self.device)
+        status_code = run(w, *args, status.data_ptr(), temp.data_ptr(), nbytes, _stream(self.device))
+        if status_code:
+            _lib.check(status_code, name)
 
 
 def _rows(t: torch.Tensor, cols: int) -> tuple[torch.Tensor, int]:
     """`t` as rows of `cols` adjacent elements, and the pitch between them (a copy if it must be)."""
-    t = t.detach().reshape(-1, cols)
+    if t.dim() != 2:
+        t = t.reshape(-1, cols)
+    if t.is_contiguous() and t.shape[0] > 1:
+        return t, cols
     if (cols > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < cols):
         t = t.contiguous()
     # One row has any pitch: the next multiple of 8, which the kernels read in place.
@@ -142,7 +149,7 @@ def _linear_forward(w: _Weight, x, bias, act: int, residual, want_slope: bool, s
     slope = torch.empty(shape, dtype=torch.int16, device=w.device) if want_slope else None
     x2, ldx = _rows(x, w.cols)
     r2, ldr = (None, 0) if residual is None else _rows(residual, w.rows)
-    b = None if bias is None else bias.detach().contiguous()
+    b = None if bias is None else bias.contiguous()
     tokens = x2.shape[0]
     if tokens:
         w.call("zn_linear", (x2.data_ptr(), ldx, tokens),
@@ -170,8 +177,10 @@ class _Linear(torch.autograd.Function):
         _, slope = ctx.saved_tensors
         need_x, _, need_b, need_r = ctx.needs_input_grad[:4]
         dx = torch.empty(ctx.x_shape, dtype=w.dtype, device=w.device) if need_x else None
-        db = torch.zeros(w.rows, dtype=w.dtype, device=w.device) if need_b else None
-        if (need_x or need_b) and dy.numel():
+        db = torch.empty(w.rows, dtype=w.dtype, device=w.device) if need_b else None
+        if not dy.numel():
+            return dx, None, db.zero_() if need_b else None, dy if need_r else None, None, None
+        if need_x or need_b:
             with _on(w.device):
                 g, ldy = _rows(dy, w.rows)
                 w.call("zn_linear_grad",
@@ -213,7 +222,8 @@ def blob_linear(
     w.place("x")
     act = _ACTIVATIONS[activation]
     with _on(w.device):
-        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, bias, residual)):
+        if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)
+                                        or (residual is not None and residual.requires_grad)):
             return _Linear.apply(x, blob, bias, residual, w, act)
         status = torch.empty(1, dtype=torch.int32, device=w.device)
         y, _ = _linear_forward(w, x, bias, act, residual, False, status)

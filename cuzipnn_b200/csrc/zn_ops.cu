@@ -264,57 +264,109 @@ struct EpiProb {
 // Rows of `cols` 16-bit elements to another pitch (a multiple of 8; the padding is not read).
 __global__ void __launch_bounds__(256) pitch_kernel(const uint16_t* src, int64_t lds, uint16_t* dst, int64_t ldd,
                                                     int64_t rows, int64_t cols) {
-  const int64_t total = rows * cols, step = int64_t(gridDim.x) * blockDim.x;
-  for (int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += step) {
-    const int64_t r = i / cols, c = i - r * cols;
-    dst[r * ldd + c] = src[r * lds + c];
+  pdl_wait();
+  pdl_trigger();
+  // A warp per 256 columns of a row at a time: no division per element.
+  const int64_t per_row = cdiv(cols, 256), total = rows * per_row;
+  const int lane = threadIdx.x & 31;
+  for (int64_t i = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5); i < total; i += int64_t(gridDim.x) * 8) {
+    const int64_t r = i / per_row, c0 = (i - r * per_row) * 256 + lane;
+    uint16_t v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (c0 + 32 * k < cols) v[k] = src[r * lds + c0 + 32 * k];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (c0 + 32 * k < cols) dst[r * ldd + c0 + 32 * k] = v[k];
   }
 }
 
 template <typename T>
 __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Finish<T> f) {
   pdl_wait();
+  pdl_trigger();
   const int64_t total = f.M * f.N, step = int64_t(gridDim.x) * blockDim.x;
   for (int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += step) finish_element(f, i);
 }
 
 // dz = dy * slope in 16 bits (the operand of dx = dz W; dz null: not wanted) and the column sums of
-// the unrounded products over kSumRows rows per block (part[row block][n], 32 bits).
-constexpr int kSumRows = 64;
-template <typename T>
-__global__ void __launch_bounds__(256) slope_kernel(const T* dy, int64_t ldy, const int16_t* slope, T* dz, int64_t ldz,
-                                                    float* part, int64_t M, int64_t N) {
-  const int64_t col_blocks = cdiv(N, 64), mb = blockIdx.x / col_blocks;
-  const int64_t n = (blockIdx.x - mb * col_blocks) * 64 + 2 * (threadIdx.x & 31);
-  const int sub = threadIdx.x >> 5;
-  float2 s = make_float2(0.0f, 0.0f);
-  const int64_t m1 = min(M, (mb + 1) * kSumRows);
-  for (int64_t m = mb * kSumRows + sub; m < m1; m += 8) {
+// the unrounded products over `per` rows per block: to dbias when that is all rows (one launch less
+// for a few tokens), else to part[row block][n] (32 bits), which column_sum_kernel adds in order.
+// V columns per thread: 8 in 16-byte accesses, four rows in flight, where the matrices allow it (72 us
+// for 4096 x 18944, the bandwidth of its 465 MB), else 1.
+constexpr int kSumRows = 64, kSumAll = 512;
+template <typename T, int V>
+__global__ void __launch_bounds__(256) slope_kernel(const T* __restrict__ dy, int64_t ldy,
+                                                    const int16_t* __restrict__ slope, T* __restrict__ dz, int64_t ldz,
+                                                    float* __restrict__ part, T* __restrict__ dbias, int64_t M,
+                                                    int64_t N, int64_t per) {
+  pdl_wait();
+  pdl_trigger();
+  const int64_t col_blocks = cdiv(N, 32 * V), mb = blockIdx.x / col_blocks;
+  const int lane = threadIdx.x & 31, sub = threadIdx.x >> 5;
+  const int64_t n = (blockIdx.x - mb * col_blocks) * 32 * V + V * lane;
+  const int64_t m1 = min(M, (mb + 1) * per);
+  float s[V];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      if (n + i >= N) break;
-      float d = Num<T>::to(dy[m * ldy + n + i]);
-      if (slope) d *= slope_value(slope[m * N + n + i]);
-      if (dz) dz[m * ldz + n + i] = Num<T>::from(d);
-      (i ? s.y : s.x) += d;
+  for (int i = 0; i < V; ++i) s[i] = 0.0f;
+  if (n < N) {
+    if constexpr (V == 8) {
+      constexpr int kDeep = 4;
+      for (int64_t m = mb * per + sub; m < m1; m += 8 * kDeep) {
+        uint4 g[kDeep], w[kDeep];
+#pragma unroll
+        for (int q = 0; q < kDeep; ++q)
+          if (m + 8 * q < m1) {
+            g[q] = *reinterpret_cast<const uint4*>(dy + (m + 8 * q) * ldy + n);
+            if (slope) w[q] = *reinterpret_cast<const uint4*>(slope + (m + 8 * q) * N + n);
+          }
+#pragma unroll
+        for (int q = 0; q < kDeep; ++q)
+          if (m + 8 * q < m1) {
+            const uint32_t gw[4] = {g[q].x, g[q].y, g[q].z, g[q].w}, ww[4] = {w[q].x, w[q].y, w[q].z, w[q].w};
+            uint32_t z[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              float a = Num<T>::lo(gw[i]), b = Num<T>::hi(gw[i]);
+              if (slope) {
+                a *= slope_value(int16_t(ww[i]));
+                b *= slope_value(int16_t(ww[i] >> 16));
+              }
+              z[i] = Num<T>::pack(a, b);
+              s[2 * i] += a;
+              s[2 * i + 1] += b;
+            }
+            if (dz) *reinterpret_cast<uint4*>(dz + (m + 8 * q) * ldz + n) = make_uint4(z[0], z[1], z[2], z[3]);
+          }
+      }
+    } else {
+      for (int64_t m = mb * per + sub; m < m1; m += 8) {
+        float d = Num<T>::to(dy[m * ldy + n]);
+        if (slope) d *= slope_value(slope[m * N + n]);
+        if (dz) dz[m * ldz + n] = Num<T>::from(d);
+        s[0] += d;
+      }
     }
   }
-  if (!part) return;
-  __shared__ float2 sm[8][32];
-  sm[sub][threadIdx.x & 31] = s;
+  if (!part && !dbias) return;
+  __shared__ float sm[8][32 * V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) sm[sub][V * lane + i] = s[i];
   __syncthreads();
-  if (sub == 0) {
-    for (int i = 1; i < 8; ++i) {
-      s.x += sm[i][threadIdx.x].x;
-      s.y += sm[i][threadIdx.x].y;
-    }
-    if (n < N) part[mb * N + n] = s.x;
-    if (n + 1 < N) part[mb * N + n + 1] = s.y;
+  const int64_t c0 = n - V * lane;
+  for (int c = threadIdx.x; c < 32 * V; c += 256) {
+    if (c0 + c >= N) continue;
+    float v = 0.0f;
+    for (int i = 0; i < 8; ++i) v += sm[i][c];
+    if (dbias) dbias[c0 + c] = Num<T>::from(v);
+    else part[mb * N + c0 + c] = v;
   }
 }
 
 template <typename T>
 __global__ void __launch_bounds__(256) column_sum_kernel(const float* part, int64_t blocks, int64_t N, T* out) {
+  pdl_wait();
+  pdl_trigger();
   const int64_t n = int64_t(blockIdx.x) * 32 + (threadIdx.x & 31);
   const int sub = threadIdx.x >> 5;
   float s = 0.0f;
@@ -335,6 +387,8 @@ __global__ void __launch_bounds__(256) column_sum_kernel(const float* part, int6
 // an entry is counted against all others (top <= 256), so no sort network is needed.
 __global__ void __launch_bounds__(128) loss_prep_kernel(const int64_t* ids, const float* logits, int64_t tokens,
                                                         int64_t vocab, int64_t ignore, float inv_t, LossRows out) {
+  pdl_wait();
+  pdl_trigger();
   const int64_t m = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   if (m >= tokens) return;
@@ -411,6 +465,7 @@ constexpr int kStatCols = 2048;
 __global__ void __launch_bounds__(256) dot_stats_kernel(DotValue v, LossRows rows, float* part, int64_t tokens,
                                                         float scale) {
   pdl_wait();
+  pdl_trigger();
   const int64_t m = blockIdx.y, n0 = int64_t(blockIdx.x) * kStatCols;
   const int64_t n1 = min(v.rows, n0 + kStatCols);
   const int count = rows.count[m];
@@ -455,6 +510,7 @@ __global__ void __launch_bounds__(256) dot_stats_kernel(DotValue v, LossRows row
 __global__ void __launch_bounds__(1024) loss_rows_kernel(const float* part, int64_t tiles, int64_t tokens,
                                                          float temperature, LossRows rows, float* loss) {
   pdl_wait();
+  pdl_trigger();
   const int64_t m = int64_t(blockIdx.x) * 32 + (threadIdx.x & 31);
   const int sub = threadIdx.x >> 5;
   RowStats st{-INFINITY, 0.0f, 0.0f};
@@ -531,10 +587,8 @@ bool tma_ready(const void* p, int64_t pitch) { return (reinterpret_cast<uintptr_
 
 int copy_pitch(const void* src, int64_t lds, void* dst, int64_t ldd, int64_t rows, int64_t cols, cudaStream_t s) {
   if (rows * cols == 0) return ZN_OK;
-  pitch_kernel<<<grid_1d(rows * cols, 1024, 148 * 16), 256, 0, s>>>(static_cast<const uint16_t*>(src), lds,
-                                                                    static_cast<uint16_t*>(dst), ldd, rows, cols);
-  count_launch();
-  return check_launch("pitch_kernel");
+  return launch_after(pitch_kernel, dim3(grid_1d(rows * cdiv(cols, 256), 8, 148 * 8)), 256, 0, s, "pitch_kernel",
+                      static_cast<const uint16_t*>(src), lds, static_cast<uint16_t*>(dst), ldd, rows, cols);
 }
 
 // A weight and the scratch that its pieces are decoded into.
@@ -616,7 +670,8 @@ int load_matrix(const void* p, int64_t rows, int64_t cols, int64_t pitch, void* 
 
 // How a product [M, K] x [N, K] is cut.  Pairs of CTAs with tiles of 256 x 256 when there are more
 // than 128 rows and the tiles fill the GPU; else single CTAs with tiles of 128 x 128, and the
-// contraction is split until there is about one tile per SM (at least 4 blocks of 64 per part).
+// contraction is split until there is about one tile per SM, with at least 8 blocks of 64 per part (a
+// part of 8 blocks takes about 2 us, the pass that adds the parts 4).
 struct Cut {
   int cg, splits;
 };
@@ -624,7 +679,7 @@ Cut cut_of(int64_t M, int64_t N, int64_t K, int sms, bool split) {
   if (M > 128 && cdiv(M, 256) * cdiv(N, 256) >= sms / 2) return {2, 1};
   const int64_t tiles = cdiv(M, 128) * cdiv(N, 128), kb = cdiv(K, kBK);
   if (!split) return {1, 1};
-  return {1, int(std::max<int64_t>(1, std::min(sms / std::max<int64_t>(1, tiles), kb / 4)))};
+  return {1, int(std::max<int64_t>(1, std::min(sms / std::max<int64_t>(1, tiles), kb / 8)))};
 }
 
 template <typename T, bool BMN, class Epi>
@@ -757,7 +812,7 @@ struct LinearGradPlan {
   int64_t ldz;
   float* acc;
   float* part;
-  int64_t ld, sum_blocks;
+  int64_t ld, sum_rows, sum_blocks;
 };
 
 int plan_linear_grad(const zn_weight* w, const void* dy, int64_t ldy, int64_t tokens, bool slope, bool dx, bool dbias,
@@ -765,8 +820,9 @@ int plan_linear_grad(const zn_weight* w, const void* dy, int64_t ldy, int64_t to
   *p = {};
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
-  p->sum_blocks = cdiv(tokens, kSumRows);
-  if (dbias) p->part = ar.take<float>(size_t(p->sum_blocks) * w->rows * 4);
+  p->sum_rows = tokens <= kSumAll ? kSumAll : kSumRows;
+  p->sum_blocks = cdiv(tokens, p->sum_rows);
+  if (dbias && p->sum_blocks > 1) p->part = ar.take<float>(size_t(p->sum_blocks) * w->rows * 4);
   p->w.status = status;
   if (!dx) return ZN_OK;
   p->ldz = round8(w->rows);
@@ -785,17 +841,19 @@ int run_linear_grad(const LinearGradPlan& p, const zn_weight* w, const void* dy,
   const T* g = static_cast<const T*>(dy);
   if (slope || dbias) {
     T* dz = slope ? static_cast<T*>(p.dz) : nullptr;
-    const int64_t grid = cdiv(rows, 64) * p.sum_blocks;
+    const bool vec = rows % 8 == 0 && tma_ready(g, ldy) && tma_ready(slope, 0) && tma_ready(dz, p.ldz);
+    const int64_t grid = cdiv(rows, vec ? 256 : 32) * p.sum_blocks;
     if (grid > 0x7FFFFFFF) return bad("zn_linear_grad");
-    slope_kernel<T><<<unsigned(grid), 256, 0, s>>>(g, ldy, static_cast<const int16_t*>(slope), dz, p.ldz, p.part, tokens, rows);
-    count_launch();
-    if (int rc = check_launch("slope_kernel")) return rc;
+    auto fn = vec ? slope_kernel<T, 8> : slope_kernel<T, 1>;
+    if (int rc = launch_after(fn, dim3(unsigned(grid)), 256, 0, s, "slope_kernel", g, ldy,
+                              static_cast<const int16_t*>(slope), dz, p.ldz, p.part,
+                              dbias && !p.part ? static_cast<T*>(dbias) : nullptr, tokens, rows, p.sum_rows))
+      return rc;
   }
-  if (dbias) {
-    column_sum_kernel<T><<<unsigned(cdiv(rows, 32)), 256, 0, s>>>(p.part, p.sum_blocks, rows, static_cast<T*>(dbias));
-    count_launch();
-    if (int rc = check_launch("column_sum_kernel")) return rc;
-  }
+  if (p.part)
+    if (int rc = launch_after(column_sum_kernel<T>, dim3(unsigned(cdiv(rows, 32))), 256, 0, s, "column_sum_kernel",
+                              static_cast<const float*>(p.part), p.sum_blocks, rows, static_cast<T*>(dbias)))
+      return rc;
   if (!dx) {
     const cudaError_t e = cudaMemsetAsync(p.w.status, 0, sizeof(int32_t), s);
     return e == cudaSuccess ? ZN_OK : set_error(ZN_ERR_CUDA, "status: %s", cudaGetErrorString(e));
@@ -887,9 +945,9 @@ int run_loss(const LossPlan& p, const void* x, int64_t ldx, int64_t tokens, cons
              int64_t ignore, float temperature, int reduction, float* loss, const LossRows& rows, cudaStream_t s) {
   const int64_t vocab = p.w.b.rows, cols = p.w.b.cols;
   const float inv_t = 1.0f / temperature;
-  loss_prep_kernel<<<unsigned(cdiv(tokens, 4)), 128, 0, s>>>(ids, logits, tokens, vocab, ignore, inv_t, rows);
-  count_launch();
-  if (int rc = check_launch("loss_prep_kernel")) return rc;
+  if (int rc = launch_after(loss_prep_kernel, dim3(unsigned(cdiv(tokens, 4))), 128, 0, s, "loss_prep_kernel", ids,
+                            logits, tokens, vocab, ignore, inv_t, rows))
+    return rc;
   if (int rc = start_weight(p.w, s)) return rc;
   Matrix xm;
   if (int rc = load_matrix(x, tokens, cols, ldx, p.x_copy, &xm, s)) return rc;

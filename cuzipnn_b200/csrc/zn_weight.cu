@@ -157,14 +157,10 @@ int weight_decode(const WeightBlob& w, void* temp, int64_t c0, int64_t c1, void*
 }
 
 int weight_wave(const WeightBlob& w, int64_t* chunks) {
-  int dev = 0, sms = 0, per_sm = 0;
-  const void* fn = w.bf16 ? reinterpret_cast<const void*>(weight_kernel<true, StoreSink>)
-                          : reinterpret_cast<const void*>(weight_kernel<false, StoreSink>);
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, fn, kDecThreads, dec_smem(1));
-  if (e != cudaSuccess) return set_error(ZN_ERR_CUDA, "weight_kernel occupancy: %s", cudaGetErrorString(e));
-  *chunks = int64_t(sms) * max(1, per_sm);
+  // The register bound of weight_kernel; a query of the occupancy costs a microsecond of every call.
+  int sms = 0;
+  if (int rc = sm_count(&sms)) return rc;
+  *chunks = int64_t(sms) * weight_blocks<StoreSink>();
   return ZN_OK;
 }
 
