@@ -10,8 +10,9 @@
 // holds its 128 rows of the result, so that a byte loaded is used twice as often.  Warp 0 loads
 // 64-wide blocks with TMA (128-byte swizzle) into a ring of shared-memory stages, one thread of warp
 // 1 (of the pair's first CTA) issues tcgen05.mma into one of two accumulators in tensor memory, and
-// warps 4-7 read the other accumulator (a thread owns a row of the tile) and run the epilogue
-// meanwhile.
+// warps 4-11 read the other accumulator (a thread owns a row of one half of the tile's columns) and
+// run the epilogue meanwhile.  Two warps per scheduler: an activation's dependent arithmetic leaves
+// one warp idle most of the time.
 //
 // Every wait has an iteration limit.  A wait that gives up sets kErrWait in the status word and the
 // abort flag, upon which all warps leave their loops, the loads in flight are waited for (again
@@ -30,7 +31,8 @@ constexpr int32_t kErrWait = 16;  // a bounded wait inside a product kernel gave
 
 constexpr int kBM = 128;          // rows of a tile per CTA (tensor memory lanes)
 constexpr int kBK = 64;           // contraction block: 128 bytes of a 16-bit type, one swizzle row
-constexpr int kGemmThreads = 256;
+constexpr int kGemmThreads = 384;  // TMA, MMA, allocation, an idle warp, and 8 epilogue warps
+constexpr int kEpiWarps = 8;
 constexpr uint32_t kWaitLimit = 1u << 24;  // polls of up to kPollNs each (about 4 s at most)
 constexpr uint32_t kPollNs = 256;
 
@@ -216,7 +218,7 @@ struct GemmCfg {
   static constexpr int kStageBytes = 2 * kOperand;
   static constexpr int kStages = 5;
   static constexpr int kWarpBuf = 4096;  // per epilogue warp, to turn rows into whole sectors
-  static constexpr int kSmem = kStages * kStageBytes + 4 * kWarpBuf + 1024;  // + alignment of the first stage
+  static constexpr int kSmem = kStages * kStageBytes + kEpiWarps * kWarpBuf + 1024;  // + alignment of the first stage
 };
 
 // Instruction descriptor: f32 accumulator, 16-bit operands of one type, B's major-ness, N and M.
@@ -226,7 +228,7 @@ __device__ constexpr uint32_t instr_desc() {
          (uint32_t(GemmCfg<CG>::kBN / 8) << 17) | (uint32_t(kBM * CG / 16) << 24);
 }
 
-// Epilogue interface.  Epi::Row row(epi, m, n0, split, buf) at the start of a thread's tile row (the
+// Epilogue interface.  Epi::Row row(epi, m, n0, split, buf) at the start of a thread's half row (the
 // warp holds rows m - lane .. m - lane + 31; m may be past the last row: nothing may be accessed
 // then), row.cols(epi, c, v) for each 32 columns n0 + c .. n0 + c + 31, by whole warps, row.end(epi)
 // after the last.  buf: kWarpBuf bytes of the warp's own shared memory.
@@ -254,7 +256,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(accfull0 + 8 * i, 1);
-      mbar_init(accempty0 + 8 * i, 4 * CG);  // one arrival per epilogue warp
+      mbar_init(accempty0 + 8 * i, kEpiWarps * CG);  // one arrival per epilogue warp
     }
     mbar_init(drain, 1);
     s_abort = 0;
@@ -366,8 +368,9 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     }
     __syncwarp();
   } else if (warp >= 4) {
-    const int quarter = warp & 3;
-    uint8_t* buf = smem_dyn + (stage0 - smem_addr(smem_dyn)) + kStages * Cfg::kStageBytes + quarter * Cfg::kWarpBuf;
+    constexpr int kHalf = BN / 2;
+    const int quarter = warp & 3, half = (warp - 4) >> 2;
+    uint8_t* buf = smem_dyn + (stage0 - smem_addr(smem_dyn)) + kStages * Cfg::kStageBytes + (warp - 4) * Cfg::kWarpBuf;
     int64_t n = 0;
     for (int64_t t = first; t < total; t += step, ++n) {
       int tm, tn, ks;
@@ -376,14 +379,15 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
       const bool ok = mbar_wait(accfull0 + 8 * acc, uint32_t((n / 2) & 1), abort_flag);
       if (!__all_sync(0xFFFFFFFFu, ok)) break;
       tc_fence_after();
-      const uint32_t src = tmem + (uint32_t(quarter * 32) << 16) + acc * BN;
-      typename Epi::Row row(epi, (int64_t(tm) * CG + rank) * kBM + quarter * 32 + lane, int64_t(tn) * BN, ks, buf);
+      const uint32_t src = tmem + (uint32_t(quarter * 32) << 16) + acc * BN + half * kHalf;
+      typename Epi::Row row(epi, (int64_t(tm) * CG + rank) * kBM + quarter * 32 + lane,
+                             int64_t(tn) * BN + half * kHalf, ks, buf);
 #pragma unroll 1
-      for (int c = 0; c < BN; c += 32) {
+      for (int c = 0; c < kHalf; c += 32) {
         float v[32];
         tc_load32(src + c, v);
         tc_wait_load();
-        if (c + 32 >= BN) {  // the accumulator is read: hand it back before the last columns' work
+        if (c + 32 >= kHalf) {  // the accumulator is read: hand it back before the last columns' work
           tc_fence_before();
           __syncwarp();
           if (lane == 0) {

@@ -15,7 +15,7 @@ __device__ __forceinline__ float activate(float z, float& slope) {
     if (SLOPE) slope = z > 0.0f ? 1.0f : 0.0f;
     return z < 0.0f ? 0.0f : z;  // keeps NaN
   } else if constexpr (ACT == kGelu) {
-    const float cdf = 0.5f * erfcf(-0.70710678118654752f * z);
+    const float cdf = 0.5f + 0.5f * erff(0.70710678118654752f * z);
     if (SLOPE) slope = cdf + z * 0.3989422804014327f * __expf(-0.5f * z * z);
     return z * cdf;
   } else if constexpr (ACT == kGeluTanh) {  // 0.5 z (1 + tanh u) = z sigmoid(2u)
@@ -46,7 +46,10 @@ __device__ __forceinline__ float activate(int act, float z, float& slope) {
 // The derivative act'(z), kept for the backward pass as a 16-bit fixed-point number of step 2^-14
 // (every activation's lies in [-0.13, 1.13]): off by 2^-15 of a whole slope at most, an eighth of
 // a bf16 rounding, so the gradients are as exact as with a 32-bit slope.  -32768 stands for NaN.
-__device__ __forceinline__ int slope_code(float s) { return s != s ? -32768 : __float2int_rn(s * 16384.0f); }
+// (The sum's low 16 bits are the rounded product: 1.5 * 2^23 leaves no fraction bits.)
+__device__ __forceinline__ uint32_t slope_code(float s) {
+  return s != s ? 0x8000u : __float_as_uint(fmaf(s, 16384.0f, 12582912.0f)) & 0xFFFFu;
+}
 __device__ __forceinline__ float slope_value(int code) { return code == -32768 ? NAN : float(code) * (1.0f / 16384.0f); }
 
 // Per-warp staging: a thread holds 64 bytes (32 16-bit columns) of its own row; through shared
@@ -102,7 +105,7 @@ struct EpiLinear {
         float s0, s1;
         v[2 * i] = activate<ACT, SLOPE>(v[2 * i], s0);
         v[2 * i + 1] = activate<ACT, SLOPE>(v[2 * i + 1], s1);
-        if (SLOPE) sw[i] = (uint32_t(slope_code(s0)) & 0xFFFFu) | (uint32_t(slope_code(s1)) << 16);
+        if (SLOPE) sw[i] = slope_code(s0) | (slope_code(s1) << 16);
       }
       if (SLOPE) stage_rows(buf, sw, e.slope, e.ldy, m - (threadIdx.x & 31), e.M, n, e.N, e.vec);
     }

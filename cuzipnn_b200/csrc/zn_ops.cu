@@ -140,11 +140,11 @@ __device__ __forceinline__ void stats_join(RowStats& a, float mx, float sum, flo
 
 struct EpiStats {
   LossRows rows;
-  float* part;    // [tile][3][M]: max, sum, hit
+  float* part;    // [half tile][3][M]: max, sum, hit
   int64_t M, N;   // N: columns of this piece
   int64_t v0;     // first vocabulary row of this piece
-  int64_t tile0;  // its first column tile
-  int tile_cols;
+  int64_t tile0;  // its first half tile
+  int tile_cols;  // columns of a half tile
   float scale;    // log2(e) / T
   struct Row {
     int64_t m, n0;
@@ -934,7 +934,7 @@ int plan_loss(const zn_weight* w, const void* x, int64_t ldx, int64_t tokens, in
     if (int rc = plan_weight(w, 0, status, ar, &p->w)) return rc;
     p->cut = cut_of(tokens, p->w.piece_rows, w->cols, sms, false);
     // Every piece but the last is a multiple of 256 rows.
-    p->tiles = cdiv(w->rows, 128 * p->cut.cg);
+    p->tiles = cdiv(w->rows, 64 * p->cut.cg);
   }
   p->part = ar.take<float>(size_t(p->tiles) * 3 * tokens * 4);
   return ZN_OK;
@@ -962,7 +962,7 @@ int run_loss(const LossPlan& p, const void* x, int64_t ldx, int64_t tokens, cons
       const int64_t r1 = std::min(vocab, r0 + p.w.piece_rows);
       Matrix wm;
       if (int rc = load_piece(p.w, r0, r1, &wm, s)) return rc;
-      const EpiStats e{rows, p.part, tokens, r1 - r0, r0, r0 / (128 * p.cut.cg), 128 * p.cut.cg, kLog2e * inv_t};
+      const EpiStats e{rows, p.part, tokens, r1 - r0, r0, r0 / (64 * p.cut.cg), 64 * p.cut.cg, kLog2e * inv_t};
       if (int rc = product<T, false>(xm, wm, p.cut, e, p.w.status, s)) return rc;
     }
   }
