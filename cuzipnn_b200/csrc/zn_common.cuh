@@ -203,6 +203,16 @@ __device__ __forceinline__ void store_words(uint8_t* p, const uint32_t* w, int n
   }
 }
 
+// NW words (a multiple of 8) in 32-byte stores, 32-byte aligned.
+template <int NW>
+__device__ __forceinline__ void store_sectors(uint8_t* p, const uint32_t* w) {
+#pragma unroll
+  for (int i = 0; i + 8 <= NW; i += 8)
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p + 4 * i), "r"(w[i]), "r"(w[i + 1]),
+                 "r"(w[i + 2]), "r"(w[i + 3]), "r"(w[i + 4]), "r"(w[i + 5]), "r"(w[i + 6]), "r"(w[i + 7])
+                 : "memory");
+}
+
 // A batch's job table in device memory: njobs structs, then (for more than one job) a map from
 // global chunk index to job index, so that a CTA finds its job with one load instead of a binary
 // search through the job structs (a chain of dependent loads at the start of every CTA).

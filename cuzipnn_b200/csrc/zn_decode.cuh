@@ -741,6 +741,9 @@ __device__ __forceinline__ void decode_chunk(const DecArgs& a, int64_t j, bool o
   const int seg = lane >> 3, l = lane & 7;
   const int rounds = int(g.sc / kRound);
   const bool out16 = (reinterpret_cast<uintptr_t>(outc) & 15) == 0;
+  // A lane's 16 elements as whole 32-byte sectors per store instruction (two 16-byte stores at a
+  // 32-byte stride use half of every sector they touch).
+  [[maybe_unused]] const bool out32 = (reinterpret_cast<uintptr_t>(outc) & 31) == 0;
   bool coded[K];
   const uint8_t* src[K];
 #pragma unroll
@@ -748,6 +751,10 @@ __device__ __forceinline__ void decode_chunk(const DecArgs& a, int64_t j, bool o
     coded[b] = S.p[b].coded;
     src[b] = S.p[b].pl;
   }
+  bool raw16 = true;  // every raw plane starts on a 16-byte boundary (units are aligned to 8)
+#pragma unroll
+  for (int b = 0; b < K; ++b)
+    if (!coded[b]) raw16 &= (reinterpret_cast<uintptr_t>(src[b]) & 15) == 0;
   const uint8_t* gb[KC];
   const uint8_t* lo[KC];
   const uint8_t* hi[KC];
@@ -884,9 +891,14 @@ __device__ __forceinline__ void decode_chunk(const DecArgs& a, int64_t j, bool o
 #pragma unroll
               for (int b = 0; b < K; ++b) {
                 if (LAST ? b == K - 1 : coded[b]) continue;
-                const uint2* sp = reinterpret_cast<const uint2*>(src[b] + off[c] + kRound);
-                const uint2 v0 = sp[0], v1 = sp[1];
-                pn[c][b][0] = v0.x; pn[c][b][1] = v0.y; pn[c][b][2] = v1.x; pn[c][b][3] = v1.y;
+                const uint8_t* sp = src[b] + off[c] + kRound;
+                if (raw16) {
+                  const uint4 v = *reinterpret_cast<const uint4*>(sp);
+                  pn[c][b][0] = v.x; pn[c][b][1] = v.y; pn[c][b][2] = v.z; pn[c][b][3] = v.w;
+                } else {
+                  const uint2 v0 = reinterpret_cast<const uint2*>(sp)[0], v1 = reinterpret_cast<const uint2*>(sp)[1];
+                  pn[c][b][0] = v0.x; pn[c][b][1] = v0.y; pn[c][b][2] = v1.x; pn[c][b][3] = v1.y;
+                }
               }
           } else if (r + 1 < rounds) {
             load_raw_round<K, kChains>(src, coded, base, len, r + 1, l, pn);
@@ -913,6 +925,7 @@ __device__ __forceinline__ void decode_chunk(const DecArgs& a, int64_t j, bool o
             uint32_t e[4 * K];
             assemble_elements<K, REORDER>(p[c], e);
             if constexpr (Sink::kDot) dot_round<Sink, true>(sink, dot, e, true, l, seg, slot0);
+            else if (K >= 2 && out32) store_sectors<4 * K>(outc + size_t(off[c]) * K, e);
             else store_words(outc + size_t(off[c]) * K, e, 4 * K, out16);  // 16-byte aligned when outc is
             off[c] += kRound;
           }
