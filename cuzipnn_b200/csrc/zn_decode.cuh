@@ -856,8 +856,9 @@ __device__ __forceinline__ void decode_chunk(const DecArgs& a, int64_t j, bool o
         return q >= qbeg && q < qend ? __ldg(gb4 + q) : load_block(gb[0], q, lo[0], hi[0]);
       };
       const uint8_t* rows = reinterpret_cast<const uint8_t*>(rings);
-      // LAST: the one coded plane is plane K - 1 (the exponent plane of every float type), so the
-      // raw planes and the decoded symbols have fixed places (no per-round plane selection).
+      // LAST: the one coded plane is plane K - 1 (the exponent plane of every float type) and has more
+      // than one symbol, so the raw planes and the decoded symbols have fixed places (no per-round
+      // plane selection).
       auto full_rounds = [&](auto last) {
         constexpr bool LAST = decltype(last)::value;
         for (; r < rfull; ++r) {
@@ -905,16 +906,25 @@ __device__ __forceinline__ void decode_chunk(const DecArgs& a, int64_t j, bool o
           }
           if (LAST || ncoded > 0) {
             uint32_t acc[kChains][4] = {};
-            if (single[0] < 0) decode_round_fast(cur[0], tabs, rows, tid, acc);
+            if (LAST || single[0] < 0) decode_round_fast(cur[0], tabs, rows, tid, acc);
             else fill_single(acc, single[0]);
 #pragma unroll
-            for (int c = 0; c < kChains; ++c) {
+            for (int c = 0; c < kChains; ++c)
 #pragma unroll
               for (int b = 0; b < K; ++b)
                 if (LAST ? b == K - 1 : b == pslot[0]) {
 #pragma unroll
                   for (int i = 0; i < 4; ++i) p[c][b][i] = acc[c][i];
                 }
+          }
+          // (No branch lies between the 16 steps and this: four elements can be put together while
+          // the next four symbols wait for their lookups.)
+          uint32_t e[kChains][4 * K];
+#pragma unroll
+          for (int c = 0; c < kChains; ++c) assemble_elements<K, REORDER>(p[c], e[c]);
+          if (LAST || ncoded > 0) {
+#pragma unroll
+            for (int c = 0; c < kChains; ++c) {
               Cursor& cb = cur[0][c];
               if (cb.nload) ring_put(ring[0][c], cb.fill, cb.r0);
               cb.fill += 8 * cb.nload;
@@ -922,16 +932,14 @@ __device__ __forceinline__ void decode_chunk(const DecArgs& a, int64_t j, bool o
           }
 #pragma unroll
           for (int c = 0; c < kChains; ++c) {
-            uint32_t e[4 * K];
-            assemble_elements<K, REORDER>(p[c], e);
-            if constexpr (Sink::kDot) dot_round<Sink, true>(sink, dot, e, true, l, seg, slot0);
-            else if (K >= 2 && out32) store_sectors<4 * K>(outc + size_t(off[c]) * K, e);
-            else store_words(outc + size_t(off[c]) * K, e, 4 * K, out16);  // 16-byte aligned when outc is
+            if constexpr (Sink::kDot) dot_round<Sink, true>(sink, dot, e[c], true, l, seg, slot0);
+            else if (K >= 2 && out32) store_sectors<4 * K>(outc + size_t(off[c]) * K, e[c]);
+            else store_words(outc + size_t(off[c]) * K, e[c], 4 * K, out16);  // 16-byte aligned when outc is
             off[c] += kRound;
           }
         }
       };
-      if (ncoded == 1 && pslot[0] == K - 1) full_rounds(std::true_type{});
+      if (ncoded == 1 && pslot[0] == K - 1 && single[0] < 0) full_rounds(std::true_type{});
       else full_rounds(std::false_type{});
     }
     for (; r < rounds; ++r) {
