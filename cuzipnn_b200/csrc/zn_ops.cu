@@ -261,24 +261,10 @@ struct EpiProb {
 
 // ---- small kernels --------------------------------------------------------------------------
 
-// Rows of `cols` 16-bit elements to another pitch (a multiple of 8; the padding is not read).
-__global__ void __launch_bounds__(256) pitch_kernel(const uint16_t* src, int64_t lds, uint16_t* dst, int64_t ldd,
-                                                    int64_t rows, int64_t cols) {
+__global__ void __launch_bounds__(256) pitch_kernel(const __grid_constant__ PitchCopy p) {
   pdl_wait();
   pdl_trigger();
-  // A warp per 256 columns of a row at a time: no division per element.
-  const int64_t per_row = cdiv(cols, 256), total = rows * per_row;
-  const int lane = threadIdx.x & 31;
-  for (int64_t i = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5); i < total; i += int64_t(gridDim.x) * 8) {
-    const int64_t r = i / per_row, c0 = (i - r * per_row) * 256 + lane;
-    uint16_t v[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (c0 + 32 * k < cols) v[k] = src[r * lds + c0 + 32 * k];
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (c0 + 32 * k < cols) dst[r * ldd + c0 + 32 * k] = v[k];
-  }
+  pitch_rows(p, int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5), int64_t(gridDim.x) * 8);
 }
 
 template <typename T>
@@ -585,10 +571,9 @@ struct Matrix {
 };
 bool tma_ready(const void* p, int64_t pitch) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && pitch % 8 == 0; }
 
-int copy_pitch(const void* src, int64_t lds, void* dst, int64_t ldd, int64_t rows, int64_t cols, cudaStream_t s) {
-  if (rows * cols == 0) return ZN_OK;
-  return launch_after(pitch_kernel, dim3(grid_1d(rows * cdiv(cols, 256), 8, 148 * 8)), 256, 0, s, "pitch_kernel",
-                      static_cast<const uint16_t*>(src), lds, static_cast<uint16_t*>(dst), ldd, rows, cols);
+int copy_pitch(const PitchCopy& p, cudaStream_t s) {
+  if (p.rows * p.cols == 0) return ZN_OK;
+  return launch_after(pitch_kernel, dim3(grid_1d(p.rows * cdiv(p.cols, 256), 8, 148 * 8)), 256, 0, s, "pitch_kernel", p);
 }
 
 // A weight and the scratch that its pieces are decoded into.
@@ -640,32 +625,32 @@ int start_weight(const Weight& w, cudaStream_t s) {
   return e == cudaSuccess ? ZN_OK : set_error(ZN_ERR_CUDA, "status: %s", cudaGetErrorString(e));
 }
 
-// Rows [r0, r1) as a matrix in memory.
-int load_piece(const Weight& w, int64_t r0, int64_t r1, Matrix* out, cudaStream_t s) {
-  const int64_t cols = w.b.cols;
-  const uint8_t* src;
-  if (w.stored) {
-    src = w.b.blob + 24 + 8 * 2 + r0 * cols * 2;
-  } else {
-    const int64_t c0 = r0 * cols / w.b.chunk, c1 = cdiv(r1 * cols, w.b.chunk);
-    if (int rc = weight_decode(w.b, w.temp, c0, c1, w.flat, w.status, s)) return rc;
-    src = w.flat + (r0 * cols - c0 * w.b.chunk) * 2;
-  }
+// Rows [r0, r1) as a matrix in memory.  With the first rows goes the copy of the other operand.
+int load_piece(const Weight& w, int64_t r0, int64_t r1, const PitchCopy& other, Matrix* out, cudaStream_t s) {
+  const int64_t cols = w.b.cols, c0 = w.stored ? 0 : r0 * cols / w.b.chunk;
+  const uint8_t* src = w.stored ? w.b.blob + 24 + 8 * 2 + r0 * cols * 2 : w.flat + (r0 * cols - c0 * w.b.chunk) * 2;
+  const PitchCopy second = r0 == 0 ? other : PitchCopy{};
+  PitchCopy first{};
   *out = {src, r1 - r0, cols, cols};
-  if (!w.padded) return ZN_OK;  // cols and the chunk size are multiples of 8: the rows are aligned
-  *out = {w.padded, r1 - r0, cols, w.pitch};
-  return copy_pitch(src, cols, w.padded, w.pitch, r1 - r0, cols, s);
+  if (w.padded) {  // else cols and the chunk size are multiples of 8: the rows are aligned
+    first = {reinterpret_cast<const uint16_t*>(src), reinterpret_cast<uint16_t*>(w.padded), cols, w.pitch, r1 - r0, cols};
+    *out = {w.padded, r1 - r0, cols, w.pitch};
+  }
+  if (!w.stored) return weight_decode(w.b, w.temp, c0, cdiv(r1 * cols, w.b.chunk), w.flat, first, second, w.status, s);
+  if (int rc = copy_pitch(first, s)) return rc;
+  return copy_pitch(second, s);
 }
 
-// A caller's matrix, copied to an aligned pitch when TMA cannot read it as it lies.
+// A caller's matrix, copied to an aligned pitch when TMA cannot read it as it lies; the copy is left
+// to the caller (PitchCopy).
 void* plan_matrix(const void* p, int64_t rows, int64_t cols, int64_t pitch, Arena& ar) {
   return tma_ready(p, pitch) ? nullptr : ar.take(size_t(rows) * round8(cols) * 2);
 }
-int load_matrix(const void* p, int64_t rows, int64_t cols, int64_t pitch, void* copy, Matrix* out, cudaStream_t s) {
-  *out = {p, rows, cols, pitch};
-  if (!copy) return ZN_OK;
-  *out = {copy, rows, cols, round8(cols)};
-  return copy_pitch(p, pitch, copy, round8(cols), rows, cols, s);
+Matrix load_matrix(const void* p, int64_t rows, int64_t cols, int64_t pitch, void* copy, PitchCopy* job) {
+  *job = {};
+  if (!copy) return {p, rows, cols, pitch};
+  *job = {static_cast<const uint16_t*>(p), static_cast<uint16_t*>(copy), pitch, round8(cols), rows, cols};
+  return {copy, rows, cols, round8(cols)};
 }
 
 // How a product [M, K] x [N, K] is cut.  Pairs of CTAs with tiles of 256 x 256 when there are more
@@ -775,11 +760,12 @@ int run_linear(const LinearPlan& p, const void* x, int64_t ldx, int64_t tokens, 
                const void* res, int64_t ldr, void* y, void* slope, cudaStream_t s) {
   const int64_t rows = p.w.b.rows, cols = p.w.b.cols;
   if (int rc = start_weight(p.w, s)) return rc;
-  Matrix xm;
-  if (int rc = load_matrix(x, tokens, cols, ldx, p.x_copy, &xm, s)) return rc;
+  PitchCopy x_job;
+  const Matrix xm = load_matrix(x, tokens, cols, ldx, p.x_copy, &x_job);
   Finish<T> f{};
   f.M = tokens;
   if (p.dot) {
+    if (int rc = copy_pitch(x_job, s)) return rc;
     f.N = rows;
     f.lin = linear_epilogue<T>(bias, res, ldr, y, slope, rows, tokens, 0, rows, act);
     return weight_linear<T>(p.w.b, p.w.temp, xm.p, xm.pitch, int(tokens), p.acc, p.part, f, p.w.status, s);
@@ -787,7 +773,7 @@ int run_linear(const LinearPlan& p, const void* x, int64_t ldx, int64_t tokens, 
   for (int64_t r0 = 0; r0 < rows; r0 += p.w.piece_rows) {
     const int64_t r1 = std::min(rows, r0 + p.w.piece_rows);
     Matrix wm;
-    if (int rc = load_piece(p.w, r0, r1, &wm, s)) return rc;
+    if (int rc = load_piece(p.w, r0, r1, x_job, &wm, s)) return rc;
     const EpiLinear<T> e = linear_epilogue<T>(bias, res, ldr, y, slope, rows, tokens, r0, r1, act);
     if (p.cut.splits == 1) {
       if (int rc = product<T, false>(xm, wm, p.cut, e, p.w.status, s)) return rc;
@@ -859,14 +845,14 @@ int run_linear_grad(const LinearGradPlan& p, const zn_weight* w, const void* dy,
     return e == cudaSuccess ? ZN_OK : set_error(ZN_ERR_CUDA, "status: %s", cudaGetErrorString(e));
   }
   if (int rc = start_weight(p.w, s)) return rc;
+  PitchCopy dy_job{};
   Matrix dzm{p.dz, tokens, rows, p.ldz};
-  if (!slope)
-    if (int rc = load_matrix(dy, tokens, rows, ldy, p.dz, &dzm, s)) return rc;
+  if (!slope) dzm = load_matrix(dy, tokens, rows, ldy, p.dz, &dy_job);
   const EpiLinear<T> e = linear_epilogue<T>(nullptr, nullptr, 0, dx, nullptr, cols, tokens, 0, cols, kNone);
   for (int64_t r0 = 0; r0 < rows; r0 += p.w.piece_rows) {
     const int64_t r1 = std::min(rows, r0 + p.w.piece_rows);
     Matrix wm;
-    if (int rc = load_piece(p.w, r0, r1, &wm, s)) return rc;
+    if (int rc = load_piece(p.w, r0, r1, dy_job, &wm, s)) return rc;
     // Columns [r0, r1) of dz (r0 is a multiple of 256: the rows stay 16-byte aligned).
     const Matrix a{static_cast<const T*>(dzm.p) + r0, tokens, r1 - r0, dzm.pitch};
     if (!p.acc) {
@@ -949,9 +935,10 @@ int run_loss(const LossPlan& p, const void* x, int64_t ldx, int64_t tokens, cons
                             logits, tokens, vocab, ignore, inv_t, rows))
     return rc;
   if (int rc = start_weight(p.w, s)) return rc;
-  Matrix xm;
-  if (int rc = load_matrix(x, tokens, cols, ldx, p.x_copy, &xm, s)) return rc;
+  PitchCopy x_job;
+  const Matrix xm = load_matrix(x, tokens, cols, ldx, p.x_copy, &x_job);
   if (p.dot) {
+    if (int rc = copy_pitch(x_job, s)) return rc;
     if (int rc = weight_dot(p.w.b, p.w.temp, xm.p, xm.pitch, int(tokens), p.z, p.z_part, p.w.status, s)) return rc;
     const DotValue v{p.z, p.z_part, vocab, cols, p.w.b.chunk};
     if (int rc = launch_after(dot_stats_kernel, dim3(unsigned(p.tiles), unsigned(tokens)), 256, 0, s, "dot_stats_kernel",
@@ -961,7 +948,7 @@ int run_loss(const LossPlan& p, const void* x, int64_t ldx, int64_t tokens, cons
     for (int64_t r0 = 0; r0 < vocab; r0 += p.w.piece_rows) {
       const int64_t r1 = std::min(vocab, r0 + p.w.piece_rows);
       Matrix wm;
-      if (int rc = load_piece(p.w, r0, r1, &wm, s)) return rc;
+      if (int rc = load_piece(p.w, r0, r1, x_job, &wm, s)) return rc;
       const EpiStats e{rows, p.part, tokens, r1 - r0, r0, r0 / (64 * p.cut.cg), 64 * p.cut.cg, kLog2e * inv_t};
       if (int rc = product<T, false>(xm, wm, p.cut, e, p.w.status, s)) return rc;
     }
@@ -1009,12 +996,12 @@ int run_loss_grad(const LossGradPlan& p, const void* x, int64_t ldx, int64_t tok
   const int64_t vocab = p.w.b.rows, cols = p.w.b.cols;
   const float gain = Num<T>::kCode == 1 ? 1.0f : 32768.0f;
   if (int rc = start_weight(p.w, s)) return rc;
-  Matrix xm;
-  if (int rc = load_matrix(x, tokens, cols, ldx, p.x_copy, &xm, s)) return rc;
+  PitchCopy x_job;
+  const Matrix xm = load_matrix(x, tokens, cols, ldx, p.x_copy, &x_job);
   for (int64_t r0 = 0; r0 < vocab; r0 += p.w.piece_rows) {
     const int64_t r1 = std::min(vocab, r0 + p.w.piece_rows);
     Matrix wm;
-    if (int rc = load_piece(p.w, r0, r1, &wm, s)) return rc;
+    if (int rc = load_piece(p.w, r0, r1, x_job, &wm, s)) return rc;
     const EpiProb<T> e{rows, static_cast<T*>(p.prob), tokens, r1 - r0, p.ldp, r0, kLog2e / temperature, gain};
     if (int rc = product<T, false>(xm, wm, p.cut, e, p.w.status, s)) return rc;
     const Matrix pm{p.prob, tokens, r1 - r0, p.ldp};

@@ -29,6 +29,13 @@ __global__ void __launch_bounds__(kDecThreads, weight_blocks<Sink>()) weight_ker
 struct NoFin {
   __device__ __forceinline__ void run(int64_t, int64_t) const {}
 };
+struct PitchFin {
+  PitchCopy copy[2];
+  __device__ __forceinline__ void run(int64_t i, int64_t n) const {
+    pitch_rows(copy[0], i / 32, n / 32);
+    pitch_rows(copy[1], i / 32, n / 32);
+  }
+};
 template <typename T>
 struct LinearFin {
   Finish<T> f;
@@ -149,11 +156,14 @@ size_t weight_temp_bytes(const WeightBlob& w) {
   return job_structs_bytes<DecArgs>(1) + dec_job_bytes(w.rows * w.cols, 2, w.chunk) + 256;  // + the counter
 }
 
-int weight_decode(const WeightBlob& w, void* temp, int64_t c0, int64_t c1, void* out, int32_t* status, cudaStream_t s) {
+int weight_decode(const WeightBlob& w, void* temp, int64_t c0, int64_t c1, void* out, const PitchCopy& copy0,
+                  const PitchCopy& copy1, int32_t* status, cudaStream_t s) {
   DecArgs a = weight_args(w, temp, status, w.direct ? kDirect : kScanned);
   a.out = static_cast<uint8_t*>(out) - c0 * w.chunk * 2;
-  return w.bf16 ? launch_weight<true>(a, c0, c1, StoreSink(), NoFin(), 0, s)
-                : launch_weight<false>(a, c0, c1, StoreSink(), NoFin(), 0, s);
+  const PitchFin fin{{copy0, copy1}};
+  const int64_t work = copy0.rows * copy0.cols + copy1.rows * copy1.cols;
+  return w.bf16 ? launch_weight<true>(a, c0, c1, StoreSink(), fin, work, s)
+                : launch_weight<false>(a, c0, c1, StoreSink(), fin, work, s);
 }
 
 int weight_wave(const WeightBlob& w, int64_t* chunks) {

@@ -34,9 +34,35 @@ size_t weight_temp_bytes(const WeightBlob& w);
 inline bool weight_direct(const WeightBlob& w, int64_t pieces) { return pieces == 1 && weight_chunks(w) <= 2048; }
 // First step of a call unless w.direct: the offsets of the blob's units; sets the status word.
 int weight_scan(const WeightBlob& w, void* temp, int32_t* status, cudaStream_t s);
-// Decode chunks [c0, c1) to `out` (the address of chunk c0's first element, 16-byte aligned).  Sets
-// the status word (w.direct) or adds to it.
-int weight_decode(const WeightBlob& w, void* temp, int64_t c0, int64_t c1, void* out, int32_t* status, cudaStream_t s);
+// A copy of `rows` rows of `cols` 16-bit elements to another pitch (rows = 0: none).
+struct PitchCopy {
+  const uint16_t* src;
+  uint16_t* dst;
+  int64_t lds, ldd, rows, cols;
+};
+#ifdef __CUDACC__
+// Its share of warp `w` of `n`: 256 columns of a row at a time.
+__device__ __forceinline__ void pitch_rows(const PitchCopy& p, int64_t w, int64_t n) {
+  const int64_t per_row = cdiv(p.cols, 256), total = p.rows * per_row;
+  const int lane = threadIdx.x & 31;
+  for (int64_t i = w; i < total; i += n) {
+    const int64_t r = i / per_row, c0 = (i - r * per_row) * 256 + lane;
+    uint16_t v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (c0 + 32 * k < p.cols) v[k] = p.src[r * p.lds + c0 + 32 * k];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (c0 + 32 * k < p.cols) p.dst[r * p.ldd + c0 + 32 * k] = v[k];
+  }
+}
+#endif
+
+// Decode chunks [c0, c1) to `out` (the address of chunk c0's first element, 16-byte aligned), then make
+// the two copies (of the decoded rows, and of another operand: in the same kernel as the check of the
+// chunks, so that odd sizes cost no launches).  Sets the status word (w.direct) or adds to it.
+int weight_decode(const WeightBlob& w, void* temp, int64_t c0, int64_t c1, void* out, const PitchCopy& copy0,
+                  const PitchCopy& copy1, int32_t* status, cudaStream_t s);
 // Chunks that the decoder works on at once on this device (its resident blocks).
 int weight_wave(const WeightBlob& w, int64_t* chunks);
 
