@@ -28,6 +28,7 @@ _ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 _REDUCTIONS = {"mean": 0, "sum": 1, "none": 2}
 _MAX_TOP = 256
 _MAX_DIM = 1 << 31
+_MIN_TEMPERATURE, _MAX_TEMPERATURE = 2.0**-20, 2.0**20  # its square and inverse stay far inside float32
 _ENTRIES = {name: (getattr(_lib.lib, name + "_temp_bytes"), getattr(_lib.lib, name))
             for name in ("zn_linear", "zn_linear_grad", "zn_loss", "zn_loss_grad")}
 
@@ -354,8 +355,8 @@ def blob_distillation(
     blob_cross_entropy; the teacher is a constant."""
     _check_reduction(reduction)
     temperature = float(temperature)
-    if not 0.0 < temperature < math.inf:
-        raise ValueError("temperature must be positive and finite")
+    if not _MIN_TEMPERATURE <= temperature <= _MAX_TEMPERATURE:
+        raise ValueError(f"temperature must be between {_MIN_TEMPERATURE} and {_MAX_TEMPERATURE}, not {temperature}")
     w = _Weight(blob, hidden, "hidden")
     if teacher_ids.dim() < 1 or not 1 <= teacher_ids.shape[-1] <= _MAX_TOP:
         raise ValueError(f"teacher_ids must have between 1 and {_MAX_TOP} entries per row")

@@ -216,7 +216,7 @@ struct GemmCfg {
   static constexpr int kBN = 128 * CG;
   static constexpr int kOperand = 128 * kBK * 2;  // bytes of A, and of B, that a CTA holds per stage
   static constexpr int kStageBytes = 2 * kOperand;
-  static constexpr int kStages = 5;
+  static constexpr int kStages = 6;
   static constexpr int kWarpBuf = 4096;  // per epilogue warp, to turn rows into whole sectors
   static constexpr int kSmem = kStages * kStageBytes + kEpiWarps * kWarpBuf + 1024;  // + alignment of the first stage
 };

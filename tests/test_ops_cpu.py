@@ -78,7 +78,7 @@ def test_loss_refusals():
     with pytest.raises(ValueError, match="targets has shape"):
         z.blob_cross_entropy(X, W, t[:4])
     ids, logits = torch.zeros(5, 3, dtype=torch.int64), torch.zeros(5, 3)
-    for temperature in (0.0, -1.0, float("inf"), float("nan")):
+    for temperature in (0.0, -1.0, 1e-30, 1e30, float("inf"), float("nan")):
         with pytest.raises(ValueError, match="temperature"):
             z.blob_distillation(X, W, logits, ids, temperature=temperature)
     with pytest.raises(ValueError, match="between 1 and 256"):

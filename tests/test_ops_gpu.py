@@ -515,6 +515,129 @@ def test_upload_blob():
         z.blob_linear(rnd(2, 144), host)
 
 
+@pytest.mark.parametrize("tokens,rows,cols", [(2, 64, 256), (40, 64, 256), (300, 4100, 256)])
+def test_unaligned_operands(tokens, rows, cols):
+    """Operands that start 2 bytes past an aligned address, and pitches that no 16-byte access fits."""
+    w, blob = weight(rows, cols, BF)
+    x = torch.zeros(tokens * cols + 1, dtype=BF, device=DEV)[1:].view(tokens, cols).copy_(rnd(tokens, cols))
+    bias = torch.zeros(rows + 1, dtype=BF, device=DEV)[1:].copy_(rnd(rows))
+    res = torch.zeros(tokens, rows + 1, dtype=BF, device=DEV)[:, 1:].copy_(rnd(tokens, rows, seed=4))
+    check_linear(x, w, blob, bias=bias, act="silu", res=res)
+    xg = x.clone().requires_grad_()
+    g = torch.zeros(tokens, rows + 3, dtype=BF, device=DEV)[:, 3:].copy_(rnd(tokens, rows, seed=5))
+    dx, = grads(z.blob_linear(xg, blob), [xg], g)
+    want = g.double() @ w.double()
+    assert_within(dx, want, u_of(BF) * want.abs() + sum_bound(rows) * (g.double().abs() @ w.double().abs()))
+
+
+@pytest.mark.parametrize("tokens", [1, 4, 50, 300])
+def test_special_values_stay_in_their_rows(tokens):
+    """Infinities and NaN of the weight reach only their own output columns, those of x only their rows."""
+    w = rnd(3000, 272, scale=0.05)
+    clean_blob = z.compress_tensor(w, chunk_bytes=4096, min_compress_bytes=0, readback_to_cpu=False)
+    w2 = w.clone()
+    w2[5], w2[7, 100], w2[2048, 271], w2[2999, 0] = math.inf, math.nan, -math.inf, math.nan
+    blob = z.compress_tensor(w2, chunk_bytes=4096, min_compress_bytes=0, readback_to_cpu=False)
+    x = rnd(tokens, 272).abs() + 0.5
+    y, clean = z.blob_linear(x, blob), z.blob_linear(x, clean_blob)
+    bad = torch.zeros(3000, dtype=torch.bool, device=DEV)
+    bad[[5, 7, 2048, 2999]] = True
+    assert torch.equal(y[:, ~bad], clean[:, ~bad])
+    assert bool((y[:, 5] == math.inf).all()) and bool((y[:, 2048] == -math.inf).all()) and bool(y[:, [7, 2999]].isnan().all())
+    x2 = x.clone()
+    x2[-1, 3] = math.nan
+    y = z.blob_linear(x2, clean_blob, activation="relu")
+    assert torch.equal(y[:-1], z.blob_linear(x, clean_blob, activation="relu")[:-1]) and bool(y[-1].isnan().all())
+
+
+def test_threads_on_their_own_streams():
+    """Calls from several threads at once: each keeps its results and its own decode status."""
+    import threading
+
+    ws, blobs, x, bias, ids, t, logits = model_inputs()
+    want = small_model(x, blobs, bias, ids, t, logits)
+    bad = z.upload_blob(blobs[0].clone())
+    bad[40:44] = 255  # a negative unit size
+    bad = z.upload_blob(bad.clone())
+    torch.cuda.synchronize()
+    out, errors = {}, []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(10):
+                    out[i] = small_model(x, blobs, bias, ids, t, logits)
+                    ok = z.last_decode_status()
+                    if i % 2:
+                        z.blob_linear(x, bad)
+                    status = z.last_decode_status()
+                    assert ok == 0 and (status != 0) == bool(i % 2)
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not errors, errors
+    assert all(torch.equal(o, want) for o in out.values())
+
+
+def test_backward_twice_and_captured_afterwards():
+    """The same graph twice; then a captured training step of the same leaf, once the eager graph is
+    gone (while it lives, PyTorch itself refuses to capture a backward pass of its leaves: their
+    gradient nodes belong to the eager stream)."""
+    ws, blobs, x, bias, ids, t, logits = model_inputs()
+    x = x.requires_grad_()
+    loss = small_model(x, blobs, bias, ids, t, logits)
+    one, = torch.autograd.grad(loss, [x], retain_graph=True)
+    two, = torch.autograd.grad(loss, [x])
+    assert torch.equal(one, two)
+    del loss
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        inner = small_model(x, blobs, bias, ids, t, logits)
+        gi, = torch.autograd.grad(inner, [x])
+    graph.replay()
+    assert torch.equal(gi, one)
+
+
+def test_offsets_past_32_bits():
+    """A head of 2.15e9 elements (4.3 GB): more than 2^31 elements and 2^32 bytes."""
+    rows, cols = 600_064, 3584
+    w = torch.empty((rows, cols), dtype=BF, device=DEV).normal_(0.0, 0.02, generator=torch.Generator(device=DEV).manual_seed(0))
+    blob = z.compress_tensor(w, readback_to_cpu=False)
+    for tokens in (1, 5):
+        x = rnd(tokens, cols)
+        y = z.blob_linear(x, blob)
+        for a, b in ((0, 300), (rows // 2, rows // 2 + 300), (rows - 300, rows)):
+            want = x.double() @ w[a:b].double().t()
+            s = x.double().abs() @ w[a:b].double().abs().t()
+            assert_within(y[:, a:b], want, u_of(BF) * want.abs() + sum_bound(cols) * s + 2.0**-25)
+    t = torch.tensor([rows - 1, 0, rows // 2, -100, rows - 7], device=DEV)
+    h = rnd(5, cols).requires_grad_()
+    loss = z.blob_cross_entropy(h, blob, t, reduction="none")
+    dh, = grads(loss, [h], torch.ones(5, device=DEV))
+    lse = torch.full((5,), -math.inf, dtype=torch.double, device=DEV)
+    ref = torch.zeros(5, cols, dtype=torch.double, device=DEV)
+    hd = h.detach().double()
+    for a in range(0, rows, 50_000):
+        lse = torch.logaddexp(lse, torch.logsumexp(hd @ w[a : a + 50_000].double().t(), 1))
+    for a in range(0, rows, 50_000):
+        wd = w[a : a + 50_000].double()
+        ref += torch.exp(hd @ wd.t() - lse[:, None]) @ wd
+    keep = t >= 0
+    wt = w[t.clamp(min=0)].double()
+    want = torch.where(keep, lse - (hd * wt).sum(1), 0.0)
+    ref = torch.where(keep[:, None], ref - wt, 0.0)
+    smax = float((hd.abs() @ w[:1000].double().abs().t()).amax()) * 1.1
+    assert_within(loss, want, torch.full_like(want, 2 * sum_bound(cols) * smax + 2.0**-20 * (2 + 14 + smax)))
+    assert float((dh.double() - ref).norm()) <= 4 * u_of(BF) * float(ref.norm())
+
+
 @pytest.mark.parametrize("tokens", [1, 30])
 def test_malformed_blob_is_reported(tokens):
     """A blob whose payload or tables were damaged sets the status, is read inside its bounds only, and
