@@ -203,6 +203,19 @@ __device__ __forceinline__ void store_words(uint8_t* p, const uint32_t* w, int n
   }
 }
 
+// Loads of bytes that are used once: they take no L1 line from data that is read again.
+__device__ __forceinline__ uint4 load_once16(const uint8_t* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint2 load_once8(const uint8_t* p) {
+  uint2 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return v;
+}
+
 // NW words (a multiple of 8) in 32-byte stores, 32-byte aligned.
 template <int NW>
 __device__ __forceinline__ void store_sectors(uint8_t* p, const uint32_t* w) {

@@ -894,10 +894,10 @@ __device__ __forceinline__ void decode_chunk(const DecArgs& a, int64_t j, bool o
                 if (LAST ? b == K - 1 : coded[b]) continue;
                 const uint8_t* sp = src[b] + off[c] + kRound;
                 if (raw16) {
-                  const uint4 v = *reinterpret_cast<const uint4*>(sp);
+                  const uint4 v = load_once16(sp);
                   pn[c][b][0] = v.x; pn[c][b][1] = v.y; pn[c][b][2] = v.z; pn[c][b][3] = v.w;
                 } else {
-                  const uint2 v0 = reinterpret_cast<const uint2*>(sp)[0], v1 = reinterpret_cast<const uint2*>(sp)[1];
+                  const uint2 v0 = load_once8(sp), v1 = load_once8(sp + 8);
                   pn[c][b][0] = v0.x; pn[c][b][1] = v0.y; pn[c][b][2] = v1.x; pn[c][b][3] = v1.y;
                 }
               }
