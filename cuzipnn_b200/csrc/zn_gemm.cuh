@@ -39,11 +39,24 @@ constexpr uint32_t kPollNs = 256;
 struct GemmShape {
   int64_t M, N, K;
   int tiles_m, tiles_n;  // output tiles
-  int splits;            // the contraction is cut into this many parts, one tile each
-  int kblocks;           // 64-wide blocks of the whole contraction
   int group_m;           // row tiles that share a column tile before the next one is taken
+  int kblocks;           // 64-wide blocks of the contraction
+  int64_t full;          // the first `full` tiles are computed whole,
+  int rest, splits;      // the `rest` last ones in `splits` parts of the contraction each,
+  float* parts;          // whose sums go to parts[rest][splits][tile rows][tile columns]
   int32_t* status;
 };
+
+// Tile order: within a group of row tiles, the row tile runs fastest, then the column tile, so that
+// the CTAs of one wave share a few column blocks of B and a group's rows of A in L2.
+__host__ __device__ inline void tile_place(const GemmShape& g, int64_t t, int& tm, int& tn) {
+  const int64_t per = int64_t(g.group_m) * g.tiles_n;
+  const int grp = int(t / per);
+  const int64_t r = t - grp * per;
+  const int left = g.tiles_m - grp * g.group_m, gm = left < g.group_m ? left : g.group_m;
+  tm = grp * g.group_m + int(r % gm);
+  tn = int(r / gm);
+}
 
 // ---- PTX ------------------------------------------------------------------------------------
 
@@ -228,7 +241,51 @@ __device__ constexpr uint32_t instr_desc() {
          (uint32_t(GemmCfg<CG>::kBN / 8) << 17) | (uint32_t(kBM * CG / 16) << 24);
 }
 
-// Epilogue interface.  Epi::Row row(epi, m, n0, split, buf) at the start of a thread's half row (the
+// acc[m][n] (32 bits) = or += the tile: what a product over one piece of a contraction adds to the
+// pieces before, or a part of a tile's contraction.  A thread's 128 bytes per 32 columns go through
+// the staging buffer, so that the warp reads and writes 4 rows of whole 128-byte lines at a time.
+struct EpiAccum {
+  static constexpr bool kParts = true;
+  float* acc;
+  int64_t M, N, ld;  // ld: a multiple of 4
+  bool add;
+  struct Row {
+    int64_t m, n0;
+    uint8_t* buf;
+    __device__ __forceinline__ Row(const EpiAccum&, int64_t m_, int64_t n0_, uint8_t* b) : m(m_), n0(n0_), buf(b) {}
+    __device__ __forceinline__ float4* at(int row, int chunk) const {
+      return reinterpret_cast<float4*>(buf + row * 128 + ((chunk ^ (row & 7)) << 4));
+    }
+    __device__ __forceinline__ void cols(const EpiAccum& e, int c, const float* v) {
+      const int lane = threadIdx.x & 31;
+      if (n0 + c >= e.N) return;
+#pragma unroll
+      for (int g = 0; g < 8; ++g) *at(lane, g) = make_float4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
+      __syncwarp();
+      const int64_t n = n0 + c + 4 * (lane & 7), m0 = m - lane;
+      float4 s[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = 4 * i + (lane >> 3);
+        s[i] = *at(r, lane & 7);
+        if (e.add && m0 + r < e.M && n < e.N) {
+          const float4 o = *reinterpret_cast<const float4*>(e.acc + (m0 + r) * e.ld + n);
+          s[i] = make_float4(s[i].x + o.x, s[i].y + o.y, s[i].z + o.z, s[i].w + o.w);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = 4 * i + (lane >> 3);
+        if (m0 + r < e.M && n < e.N) *reinterpret_cast<float4*>(e.acc + (m0 + r) * e.ld + n) = s[i];
+      }
+      __syncwarp();
+    }
+    __device__ __forceinline__ void end(const EpiAccum&) {}
+  };
+};
+
+// Epilogue interface.  Epi::kParts: tiles may be computed in parts (else GemmShape::rest is 0), whose
+// sums another kernel hands to the epilogue.  Epi::Row row(epi, m, n0, buf) at the start of a thread's half row (the
 // warp holds rows m - lane .. m - lane + 31; m may be past the last row: nothing may be accessed
 // then), row.cols(epi, c, v) for each 32 columns n0 + c .. n0 + c + 31, by whole warps, row.end(epi)
 // after the last.  buf: kWarpBuf bytes of the warp's own shared memory.
@@ -272,33 +329,33 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
   const uint32_t tmem = s_tmem;
   volatile int* abort_flag = &s_abort;
 
-  const int64_t total = int64_t(g.tiles_m) * g.tiles_n * g.splits;
   const int64_t first = blockIdx.x / CG, step = gridDim.x / CG;
-  // Tile order: within a group of row tiles, the row tile runs fastest, then the column tile, so
-  // that the CTAs of one wave share a few column blocks of B and a group's rows of A in L2.
-  auto tile_of = [&](int64_t t, int& tm, int& tn, int& ks) {
-    ks = int(t % g.splits);
-    t /= g.splits;
-    const int64_t per = int64_t(g.group_m) * g.tiles_n;
-    const int grp = int(t / per);
-    const int64_t r = t - grp * per;
-    const int gm = min(g.group_m, g.tiles_m - grp * g.group_m);
-    tm = grp * g.group_m + int(r % gm);
-    tn = int(r / gm);
-  };
-  auto k_range = [&](int ks, int& kb0, int& kb1) {
+  // The n-th tile (or part of a tile, its place in `parts` in `part`) of this CTA or pair.  With parts,
+  // `full` is a multiple of the grid, and every CTA has at most one part, after its whole tiles.
+  auto item = [&](int64_t n, int& tm, int& tn, int& kb0, int& kb1, int& part) {
+    const int64_t t = first + n * step;
+    if (t < g.full) {
+      tile_place(g, t, tm, tn);
+      kb0 = 0;
+      kb1 = g.kblocks;
+      part = -1;
+      return true;
+    }
+    if (t - g.full >= int64_t(g.rest) * g.splits) return false;
+    part = int(t - g.full);
+    const int ks = part % g.splits;
+    tile_place(g, g.full + part / g.splits, tm, tn);
     kb0 = int(int64_t(g.kblocks) * ks / g.splits);
     kb1 = int(int64_t(g.kblocks) * (ks + 1) / g.splits);
+    return true;
   };
 
   if (warp == 0) {
     if (lane == 0) {
       int64_t it = 0;  // blocks loaded
       bool ok = true;
-      for (int64_t t = first; t < total && ok; t += step) {
-        int tm, tn, ks, kb0, kb1;
-        tile_of(t, tm, tn, ks);
-        k_range(ks, kb0, kb1);
+      int tm, tn, kb0, kb1, part;
+      for (int64_t n = 0; ok && item(n, tm, tn, kb0, kb1, part); ++n) {
         const int ya = (tm * CG + int(rank)) * kBM, yb = tn * BN + int(rank) * 128;
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const int s = int(it % kStages);
@@ -331,12 +388,10 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     __syncwarp();
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {
-      int64_t it = 0, n = 0;  // blocks consumed, tiles done
+      int64_t it = 0;  // blocks consumed
       bool ok = true;
-      for (int64_t t = first; t < total && ok; t += step, ++n) {
-        int tm, tn, ks, kb0, kb1;
-        tile_of(t, tm, tn, ks);
-        k_range(ks, kb0, kb1);
+      int tm, tn, kb0, kb1, part;
+      for (int64_t n = 0; ok && item(n, tm, tn, kb0, kb1, part); ++n) {
         const int acc = int(n & 1);
         if (n >= 2 && !mbar_wait(accempty0 + 8 * acc, uint32_t((n / 2 - 1) & 1), abort_flag)) {
           ok = false;
@@ -371,33 +426,43 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     constexpr int kHalf = BN / 2;
     const int quarter = warp & 3, half = (warp - 4) >> 2;
     uint8_t* buf = smem_dyn + (stage0 - smem_addr(smem_dyn)) + kStages * Cfg::kStageBytes + (warp - 4) * Cfg::kWarpBuf;
-    int64_t n = 0;
-    for (int64_t t = first; t < total; t += step, ++n) {
-      int tm, tn, ks;
-      tile_of(t, tm, tn, ks);
+    int tm, tn, kb0, kb1, part;
+    for (int64_t n = 0; item(n, tm, tn, kb0, kb1, part); ++n) {
       const int acc = int(n & 1);
       const bool ok = mbar_wait(accfull0 + 8 * acc, uint32_t((n / 2) & 1), abort_flag);
       if (!__all_sync(0xFFFFFFFFu, ok)) break;
       tc_fence_after();
       const uint32_t src = tmem + (uint32_t(quarter * 32) << 16) + acc * BN + half * kHalf;
-      typename Epi::Row row(epi, (int64_t(tm) * CG + rank) * kBM + quarter * 32 + lane,
-                             int64_t(tn) * BN + half * kHalf, ks, buf);
+      // The accumulator's columns through `row`; it is handed back before the last ones' work.
+      auto drain_tile = [&](auto& row, const auto& e) {
 #pragma unroll 1
-      for (int c = 0; c < kHalf; c += 32) {
-        float v[32];
-        tc_load32(src + c, v);
-        tc_wait_load();
-        if (c + 32 >= kHalf) {  // the accumulator is read: hand it back before the last columns' work
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) {
-            if constexpr (CG == 2) mbar_arrive_cluster(in_leader(accempty0 + 8 * acc));
-            else mbar_arrive(accempty0 + 8 * acc);
+        for (int c = 0; c < kHalf; c += 32) {
+          float v[32];
+          tc_load32(src + c, v);
+          tc_wait_load();
+          if (c + 32 >= kHalf) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+              if constexpr (CG == 2) mbar_arrive_cluster(in_leader(accempty0 + 8 * acc));
+              else mbar_arrive(accempty0 + 8 * acc);
+            }
           }
+          row.cols(e, c, v);
         }
-        row.cols(epi, c, v);
+        row.end(e);
+      };
+      const int64_t m = rank * kBM + quarter * 32 + lane, c0 = half * kHalf;  // in the tile
+      if constexpr (Epi::kParts) {
+        if (part >= 0) {
+          const EpiAccum e{g.parts + int64_t(part) * (CG * kBM * BN), CG * kBM, BN, BN, false};
+          EpiAccum::Row row(e, m, c0, buf);
+          drain_tile(row, e);
+          continue;
+        }
       }
-      row.end(epi);
+      typename Epi::Row row(epi, int64_t(tm) * CG * kBM + m, int64_t(tn) * BN + c0, buf);
+      drain_tile(row, epi);
     }
   }
   tc_fence_before();
@@ -415,16 +480,57 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
 int make_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t pitch, int box_rows, bool bf16);
 int sm_count(int* sms);
 
-inline GemmShape gemm_shape(int64_t M, int64_t N, int64_t K, int cg, int32_t* status) {
+// How a product [M, K] x [N, K] is cut: tiles of 256 x 256 by pairs of CTAs or of 128 x 128 by single
+// ones, and whether the tiles of the last, incomplete wave are computed in parts of the contraction.
+struct Cut {
+  int cg;
+  int64_t full;
+  int rest, splits;
+};
+// The cheaper of the possible cuts by these figures, measured on products of a thousand and more
+// blocks: 0.43 us per 64-wide block of a pair's tile (4096 x 18944 x 3584: 1400 TFLOP/s), 0.29 us of a
+// single CTA's (301 x 1280 x 51866), 6 us for the kernel that adds the parts.  Parts are at least 8
+// blocks long.
+inline Cut cut_of(int64_t M, int64_t N, int64_t K, int sms, bool parts) {
+  Cut best{1, 0, 0, 1};
+  double least = 0;
+  const int64_t kb = cdiv(K, kBK);
+  for (int cg = 1; cg <= 2; ++cg) {
+    const int64_t workers = sms / cg, tiles = cdiv(M, 128 * cg) * cdiv(N, 128 * cg);
+    const double block = cg == 1 ? 0.29 : 0.43;
+    auto take = [&](const Cut& c, double us) {
+      if (least == 0 || us < least) {
+        best = c;
+        least = us;
+      }
+    };
+    take({cg, tiles, 0, 1}, double(cdiv(tiles, workers)) * double(kb) * block);
+    const int64_t rest = tiles % workers;
+    const int64_t splits = rest ? (workers / rest < kb / 8 ? workers / rest : kb / 8) : 0;
+    if (parts && splits >= 2)
+      take({cg, tiles - rest, int(rest), int(splits)},
+           (double(tiles / workers) * double(kb) + double(cdiv(kb, splits))) * block + 6.0);
+  }
+  return best;
+}
+// Whole tiles only, of a given kind (every piece of a weight cut alike).
+inline Cut whole_cut(int cg, int64_t M, int64_t N) { return {cg, cdiv(M, 128 * cg) * cdiv(N, 128 * cg), 0, 1}; }
+// Bytes of GemmShape::parts that any cut needs: a tile per CTA or pair.
+inline size_t parts_bytes(int sms) { return size_t(sms) * (2 * kBM * kBM) * sizeof(float); }
+
+inline GemmShape gemm_shape(int64_t M, int64_t N, int64_t K, const Cut& cut, float* parts, int32_t* status) {
   GemmShape g{};
   g.M = M;
   g.N = N;
   g.K = K;
-  g.tiles_m = int(cdiv(M, kBM * cg));
-  g.tiles_n = int(cdiv(N, 128 * cg));
+  g.tiles_m = int(cdiv(M, kBM * cut.cg));
+  g.tiles_n = int(cdiv(N, 128 * cut.cg));
   g.kblocks = int(cdiv(K, kBK));
-  g.splits = 1;
-  g.group_m = 32 / cg;
+  g.group_m = 32 / cut.cg;
+  g.full = cut.full;
+  g.rest = cut.rest;
+  g.splits = cut.splits;
+  g.parts = parts;
   g.status = status;
   return g;
 }
@@ -435,7 +541,8 @@ int launch_gemm(const CUtensorMap& a, const CUtensorMap& b, const GemmShape& g, 
   if (int rc = set_max_smem(reinterpret_cast<const void*>(fn), GemmCfg<CG>::kSmem)) return rc;
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
-  const int64_t total = int64_t(g.tiles_m) * g.tiles_n * g.splits;
+  // With parts, the grid is all workers (`full` is a multiple of it, or 0).
+  const int64_t total = g.rest && g.full ? sms / CG : g.full + int64_t(g.rest) * g.splits;
   if (total <= 0) return ZN_OK;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(unsigned(CG * (total < sms / CG ? total : sms / CG)));

@@ -84,6 +84,7 @@ __device__ __forceinline__ void stage_rows(uint8_t* buf, const uint32_t* w, T* o
 // y = act(acc + bias) + residual, rounded once to 16 bits, and (where asked for) the slopes.
 template <typename T>
 struct EpiLinear {
+  static constexpr bool kParts = true;
   const T* bias;  // or null
   const T* res;   // or null
   T* y;
@@ -95,7 +96,7 @@ struct EpiLinear {
   struct Row {
     int64_t m, n0;
     uint8_t* buf;
-    __device__ __forceinline__ Row(const EpiLinear&, int64_t m_, int64_t n0_, int, uint8_t* b) : m(m_), n0(n0_), buf(b) {}
+    __device__ __forceinline__ Row(const EpiLinear&, int64_t m_, int64_t n0_, uint8_t* b) : m(m_), n0(n0_), buf(b) {}
 
     template <int ACT, bool SLOPE>
     __device__ __forceinline__ void run(const EpiLinear& e, int64_t n, float* v) {
@@ -176,13 +177,23 @@ struct DotValue {
   }
 };
 
-// y = act(z + bias) + residual from z = sum of the splits of acc, or from weight_dot; or
-// y = z * (a scale per row) for the gradient of a loss.
+// One element of the epilogue.
+template <typename T>
+__device__ __forceinline__ void finish_value(const EpiLinear<T>& e, int64_t m, int64_t n, float z) {
+  if (e.bias) z += Num<T>::to(e.bias[n]);
+  float sl;
+  z = e.slope ? activate<true>(e.act, z, sl) : activate<false>(e.act, z, sl);
+  if (e.res) z += Num<T>::to(e.res[m * e.ldr + n]);
+  e.y[m * e.ldy + n] = Num<T>::from(z);
+  if (e.slope) e.slope[m * e.ldy + n] = int16_t(slope_code(sl));
+}
+
+// y = act(z + bias) + residual from z = acc, or from weight_dot; or y = z * (a scale per row) for the
+// gradient of a loss.
 template <typename T>
 struct Finish {
-  const float* acc;  // [splits][M][ld], or null: dot
+  const float* acc;  // [M][ld], or null: dot
   int64_t M, N, ld;
-  int splits;
   DotValue dot;
   EpiLinear<T> lin;
   // gradient of a loss: row m is scaled by T * grad / (rows that count for a mean) / gain
@@ -196,23 +207,14 @@ struct Finish {
 template <typename T>
 __device__ __forceinline__ void finish_element(const Finish<T>& f, int64_t i) {
   const int64_t m = i / f.N, n = i - m * f.N;
-  float z = 0.0f;
-  if (f.acc)
-    for (int s = 0; s < f.splits; ++s) z += f.acc[(s * f.M + m) * f.ld + n];
-  else z = f.dot.get(m, n);
-  const EpiLinear<T>& e = f.lin;
-  if (f.grad) {
-    if (f.count[m] == 0) z = 0.0f;
-    else z *= f.factor * f.grad[m * f.grad_step] / (f.mean_rows ? *f.mean_rows : 1.0f);
-    e.y[m * e.ldy + n] = Num<T>::from(z);
+  float z = f.acc ? f.acc[m * f.ld + n] : f.dot.get(m, n);
+  if (!f.grad) {
+    finish_value(f.lin, m, n, z);
     return;
   }
-  if (e.bias) z += Num<T>::to(e.bias[n]);
-  float sl;
-  z = e.slope ? activate<true>(e.act, z, sl) : activate<false>(e.act, z, sl);
-  if (e.res) z += Num<T>::to(e.res[m * e.ldr + n]);
-  e.y[m * e.ldy + n] = Num<T>::from(z);
-  if (e.slope) e.slope[m * e.ldy + n] = int16_t(slope_code(sl));
+  if (f.count[m] == 0) z = 0.0f;
+  else z *= f.factor * f.grad[m * f.grad_step] / (f.mean_rows ? *f.mean_rows : 1.0f);
+  f.lin.y[m * f.lin.ldy + n] = Num<T>::from(z);
 }
 
 // weight_dot, then f (whose dot it fills in) on every element.

@@ -58,51 +58,6 @@ constexpr int kMaxTop = 256;
 
 // ---- epilogues ------------------------------------------------------------------------------
 
-// acc[split][m][n] (32 bits) = or += the tile: the parts of a contraction that is cut, across the
-// CTAs of one product or across the pieces of a weight.  finish_kernel adds the splits in order.
-// A thread's 128 bytes per 32 columns go through the staging buffer, so that the warp reads and
-// writes 4 rows of whole 128-byte lines at a time.
-struct EpiAccum {
-  float* acc;
-  int64_t M, N, ld;  // ld: a multiple of 4
-  bool add;
-  struct Row {
-    int64_t m, n0;
-    float* p;
-    uint8_t* buf;
-    __device__ __forceinline__ Row(const EpiAccum& e, int64_t m_, int64_t n0_, int split, uint8_t* b)
-        : m(m_), n0(n0_), p(e.acc + int64_t(split) * e.M * e.ld), buf(b) {}
-    __device__ __forceinline__ float4* at(int row, int chunk) const {
-      return reinterpret_cast<float4*>(buf + row * 128 + ((chunk ^ (row & 7)) << 4));
-    }
-    __device__ __forceinline__ void cols(const EpiAccum& e, int c, const float* v) {
-      const int lane = threadIdx.x & 31;
-      if (n0 + c >= e.N) return;
-#pragma unroll
-      for (int g = 0; g < 8; ++g) *at(lane, g) = make_float4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
-      __syncwarp();
-      const int64_t n = n0 + c + 4 * (lane & 7), m0 = m - lane;
-      float4 s[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int r = 4 * i + (lane >> 3);
-        s[i] = *at(r, lane & 7);
-        if (e.add && m0 + r < e.M && n < e.N) {
-          const float4 o = *reinterpret_cast<const float4*>(p + (m0 + r) * e.ld + n);
-          s[i] = make_float4(s[i].x + o.x, s[i].y + o.y, s[i].z + o.z, s[i].w + o.w);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int r = 4 * i + (lane >> 3);
-        if (m0 + r < e.M && n < e.N) *reinterpret_cast<float4*>(p + (m0 + r) * e.ld + n) = s[i];
-      }
-      __syncwarp();
-    }
-    __device__ __forceinline__ void end(const EpiAccum&) {}
-  };
-};
-
 // Per-row state of a loss (state buffer of a call, kept for the backward pass).
 struct LossRows {
   float* lse;      // log sum exp of s (NaN for a row with an id out of range)
@@ -139,6 +94,7 @@ __device__ __forceinline__ void stats_join(RowStats& a, float mx, float sum, flo
 }
 
 struct EpiStats {
+  static constexpr bool kParts = false;
   LossRows rows;
   float* part;    // [half tile][3][M]: max, sum, hit
   int64_t M, N;   // N: columns of this piece
@@ -153,7 +109,7 @@ struct EpiStats {
     const float* q;
     int at, count;
     int64_t next;  // column (of the piece) of the next id
-    __device__ __forceinline__ Row(const EpiStats& e, int64_t m_, int64_t n0_, int, uint8_t*) : m(m_), n0(n0_) {
+    __device__ __forceinline__ Row(const EpiStats& e, int64_t m_, int64_t n0_, uint8_t*) : m(m_), n0(n0_) {
       st = {-INFINITY, 0.0f, 0.0f};
       at = count = 0;
       next = INT64_MAX;
@@ -208,6 +164,7 @@ struct EpiStats {
 // has the range of 32 bits (gain 1).  Rows that do not count are zero whatever their logits are.
 template <typename T>
 struct EpiProb {
+  static constexpr bool kParts = false;
   LossRows rows;
   T* p;
   int64_t M, N, ld, v0;  // ld: a multiple of 8
@@ -220,7 +177,7 @@ struct EpiProb {
     int at, count;
     int64_t next;
     uint8_t* buf;
-    __device__ __forceinline__ Row(const EpiProb& e, int64_t m_, int64_t n0_, int, uint8_t* b)
+    __device__ __forceinline__ Row(const EpiProb& e, int64_t m_, int64_t n0_, uint8_t* b)
         : m(m_), n0(n0_), buf(b) {
       at = count = 0;
       next = INT64_MAX;
@@ -265,6 +222,42 @@ __global__ void __launch_bounds__(256) pitch_kernel(const __grid_constant__ Pitc
   pdl_wait();
   pdl_trigger();
   pitch_rows(p, int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5), int64_t(gridDim.x) * 8);
+}
+
+__device__ __forceinline__ void parts_end(const EpiAccum& e, int64_t m, int64_t n, const float* v) {
+  for (int i = 0; i < 4; ++i)
+    if (n + i < e.N) {
+      float* p = e.acc + m * e.ld + n + i;
+      *p = (e.add ? *p : 0.0f) + v[i];
+    }
+}
+template <typename T>
+__device__ __forceinline__ void parts_end(const EpiLinear<T>& e, int64_t m, int64_t n, const float* v) {
+  for (int i = 0; i < 4; ++i)
+    if (n + i < e.N) finish_value(e, m, n + i, v[i]);
+}
+
+// The tiles that a product computed in parts: four columns per thread, the parts added in order.
+template <class Epi>
+__global__ void __launch_bounds__(256) parts_kernel(const __grid_constant__ GemmShape g,
+                                                    const __grid_constant__ Epi epi, int tile) {
+  pdl_wait();
+  pdl_trigger();
+  const int quads = tile / 4, blocks = tile * quads / 256, which = blockIdx.x / blocks;
+  const int i = (blockIdx.x - which * blocks) * 256 + threadIdx.x, r = i / quads, c = 4 * (i - r * quads);
+  int tm, tn;
+  tile_place(g, g.full + which, tm, tn);
+  const int64_t m = int64_t(tm) * tile + r, n = int64_t(tn) * tile + c;
+  if (m >= g.M || n >= g.N) return;
+  const float4* p = reinterpret_cast<const float4*>(g.parts + int64_t(which) * g.splits * tile * tile + r * tile + c);
+  float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+  for (int k = 0; k < g.splits; ++k) {
+    const float4 v = p[int64_t(k) * tile * tile / 4];
+    s = make_float4(s.x + v.x, s.y + v.y, s.z + v.z, s.w + v.w);
+  }
+  const float v[4] = {s.x, s.y, s.z, s.w};
+  parts_end(epi, m, n, v);
 }
 
 template <typename T>
@@ -653,31 +646,32 @@ Matrix load_matrix(const void* p, int64_t rows, int64_t cols, int64_t pitch, voi
   return {copy, rows, cols, round8(cols)};
 }
 
-// How a product [M, K] x [N, K] is cut.  Pairs of CTAs with tiles of 256 x 256 when there are more
-// than 128 rows and the tiles fill the GPU; else single CTAs with tiles of 128 x 128, and the
-// contraction is split until there is about one tile per SM, with at least 8 blocks of 64 per part (a
-// part of 8 blocks takes about 2 us, the pass that adds the parts 4).
-struct Cut {
-  int cg, splits;
-};
-Cut cut_of(int64_t M, int64_t N, int64_t K, int sms, bool split) {
-  if (M > 128 && cdiv(M, 256) * cdiv(N, 256) >= sms / 2) return {2, 1};
-  const int64_t tiles = cdiv(M, 128) * cdiv(N, 128), kb = cdiv(K, kBK);
-  if (!split) return {1, 1};
-  return {1, int(std::max<int64_t>(1, std::min(sms / std::max<int64_t>(1, tiles), kb / 8)))};
-}
-
 template <typename T, bool BMN, class Epi>
-int product(const Matrix& a, const Matrix& b, const Cut& cut, const Epi& epi, int32_t* status, cudaStream_t s) {
+int product(const Matrix& a, const Matrix& b, const Cut& cut, float* parts, const Epi& epi, int32_t* status,
+            cudaStream_t s) {
   const int64_t M = a.rows, K = a.cols, N = BMN ? b.cols : b.rows;
   constexpr bool bf16 = Num<T>::kCode == 1;
   CUtensorMap ma, mb;
   if (int rc = make_map(&ma, a.p, a.rows, a.cols, a.pitch, kBM, bf16)) return rc;
   if (int rc = make_map(&mb, b.p, b.rows, b.cols, b.pitch, BMN ? kBK : 128, bf16)) return rc;
-  GemmShape g = gemm_shape(M, N, K, cut.cg, status);
-  g.splits = cut.splits;
-  if (cut.cg == 2) return launch_gemm<T, 2, BMN>(ma, mb, g, epi, s);
-  return launch_gemm<T, 1, BMN>(ma, mb, g, epi, s);
+  const GemmShape g = gemm_shape(M, N, K, cut, parts, status);
+  if (int rc = cut.cg == 2 ? launch_gemm<T, 2, BMN>(ma, mb, g, epi, s) : launch_gemm<T, 1, BMN>(ma, mb, g, epi, s))
+    return rc;
+  if constexpr (Epi::kParts) {
+    if (g.rest) {
+      const int tile = kBM * cut.cg;
+      TimedLaunch tl("finish", s);
+      return launch_after(parts_kernel<Epi>, dim3(unsigned(int64_t(g.rest) * (tile * tile / 4 / 256))), 256, 0, s,
+                          "parts_kernel", g, epi, tile);
+    }
+  }
+  return ZN_OK;
+}
+// Products whose epilogue takes parts: cut by their own sizes.
+template <typename T, bool BMN, class Epi>
+int product(const Matrix& a, const Matrix& b, int sms, float* parts, const Epi& epi, int32_t* status, cudaStream_t s) {
+  const Cut cut = cut_of(a.rows, BMN ? b.cols : b.rows, a.cols, sms, true);
+  return product<T, BMN>(a, b, cut, parts, epi, status, s);
 }
 
 template <typename T>
@@ -705,11 +699,9 @@ bool sizes_ok(int64_t tokens, int64_t pitch, int64_t cols) {
 struct LinearPlan {
   Weight w;
   bool dot;
-  Cut cut;
   void* x_copy;
-  float* acc;   // split parts of a piece, or z of the dot path
+  float* acc;   // parts of a product's last tiles, or z of the dot path
   float* part;  // dot path
-  int64_t ld;
   int sms;
 };
 
@@ -729,9 +721,7 @@ int plan_linear(const zn_weight* w, const void* x, int64_t ldx, int64_t tokens, 
     return ZN_OK;
   }
   if (int rc = plan_weight(w, 0, status, ar, &p->w)) return rc;
-  p->cut = cut_of(tokens, p->w.piece_rows, w->cols, p->sms, true);
-  p->ld = (p->w.piece_rows + 3) & ~int64_t(3);
-  if (p->cut.splits > 1) p->acc = ar.take<float>(size_t(p->cut.splits) * tokens * p->ld * 4);
+  p->acc = ar.take<float>(parts_bytes(p->sms));
   return ZN_OK;
 }
 
@@ -775,28 +765,18 @@ int run_linear(const LinearPlan& p, const void* x, int64_t ldx, int64_t tokens, 
     Matrix wm;
     if (int rc = load_piece(p.w, r0, r1, x_job, &wm, s)) return rc;
     const EpiLinear<T> e = linear_epilogue<T>(bias, res, ldr, y, slope, rows, tokens, r0, r1, act);
-    if (p.cut.splits == 1) {
-      if (int rc = product<T, false>(xm, wm, p.cut, e, p.w.status, s)) return rc;
-      continue;
-    }
-    const EpiAccum a{p.acc, tokens, r1 - r0, p.ld, false};
-    if (int rc = product<T, false>(xm, wm, p.cut, a, p.w.status, s)) return rc;
-    f.acc = p.acc;
-    f.N = r1 - r0;
-    f.ld = p.ld;
-    f.splits = p.cut.splits;
-    f.lin = e;
-    if (int rc = run_finish(f, s)) return rc;
+    if (int rc = product<T, false>(xm, wm, p.sms, p.acc, e, p.w.status, s)) return rc;
   }
   return ZN_OK;
 }
 
 struct LinearGradPlan {
   Weight w;
-  Cut cut;
+  int sms;
   void* dz;  // dy * slope, or an aligned copy of dy
   int64_t ldz;
-  float* acc;
+  float* acc;  // dx in 32 bits over the pieces, when there are several
+  float* parts;
   float* part;
   int64_t ld, sum_rows, sum_blocks;
 };
@@ -804,8 +784,7 @@ struct LinearGradPlan {
 int plan_linear_grad(const zn_weight* w, const void* dy, int64_t ldy, int64_t tokens, bool slope, bool dx, bool dbias,
                      int32_t* status, Arena& ar, LinearGradPlan* p) {
   *p = {};
-  int sms = 0;
-  if (int rc = sm_count(&sms)) return rc;
+  if (int rc = sm_count(&p->sms)) return rc;
   p->sum_rows = tokens <= kSumAll ? kSumAll : kSumRows;
   p->sum_blocks = cdiv(tokens, p->sum_rows);
   if (dbias && p->sum_blocks > 1) p->part = ar.take<float>(size_t(p->sum_blocks) * w->rows * 4);
@@ -814,9 +793,9 @@ int plan_linear_grad(const zn_weight* w, const void* dy, int64_t ldy, int64_t to
   p->ldz = round8(w->rows);
   if (slope || !tma_ready(dy, ldy)) p->dz = ar.take(size_t(tokens) * p->ldz * 2);
   if (int rc = plan_weight(w, 0, status, ar, &p->w)) return rc;
-  p->cut = cut_of(tokens, w->cols, p->w.piece_rows, sms, true);
   p->ld = (w->cols + 3) & ~int64_t(3);
-  if (p->cut.splits > 1 || p->w.pieces > 1) p->acc = ar.take<float>(size_t(p->cut.splits) * tokens * p->ld * 4);
+  p->parts = ar.take<float>(parts_bytes(p->sms));
+  if (p->w.pieces > 1) p->acc = ar.take<float>(size_t(tokens) * p->ld * 4);
   return ZN_OK;
 }
 
@@ -855,12 +834,10 @@ int run_linear_grad(const LinearGradPlan& p, const zn_weight* w, const void* dy,
     if (int rc = load_piece(p.w, r0, r1, dy_job, &wm, s)) return rc;
     // Columns [r0, r1) of dz (r0 is a multiple of 256: the rows stay 16-byte aligned).
     const Matrix a{static_cast<const T*>(dzm.p) + r0, tokens, r1 - r0, dzm.pitch};
-    if (!p.acc) {
-      if (int rc = product<T, true>(a, wm, p.cut, e, p.w.status, s)) return rc;
-      continue;
-    }
     const EpiAccum acc{p.acc, tokens, cols, p.ld, r0 > 0};
-    if (int rc = product<T, true>(a, wm, p.cut, acc, p.w.status, s)) return rc;
+    if (int rc = p.acc ? product<T, true>(a, wm, p.sms, p.parts, acc, p.w.status, s)
+                       : product<T, true>(a, wm, p.sms, p.parts, e, p.w.status, s))
+      return rc;
   }
   if (!p.acc) return ZN_OK;
   Finish<T> f{};
@@ -868,7 +845,6 @@ int run_linear_grad(const LinearGradPlan& p, const zn_weight* w, const void* dy,
   f.M = tokens;
   f.N = cols;
   f.ld = p.ld;
-  f.splits = p.cut.splits;
   f.lin = e;
   return run_finish(f, s);
 }
@@ -950,7 +926,8 @@ int run_loss(const LossPlan& p, const void* x, int64_t ldx, int64_t tokens, cons
       Matrix wm;
       if (int rc = load_piece(p.w, r0, r1, x_job, &wm, s)) return rc;
       const EpiStats e{rows, p.part, tokens, r1 - r0, r0, r0 / (64 * p.cut.cg), 64 * p.cut.cg, kLog2e * inv_t};
-      if (int rc = product<T, false>(xm, wm, p.cut, e, p.w.status, s)) return rc;
+      const Cut cut = whole_cut(p.cut.cg, tokens, r1 - r0);
+      if (int rc = product<T, false>(xm, wm, cut, nullptr, e, p.w.status, s)) return rc;
     }
   }
   float* row_loss = reduction == kRows ? loss : p.row_loss;
@@ -967,26 +944,27 @@ constexpr int64_t kProbBytes = int64_t(1) << 29;
 
 struct LossGradPlan {
   Weight w;
-  Cut cut, cut_dh;
+  Cut cut;
+  int sms;
   void* x_copy;
   void* prob;
   int64_t ldp, ld;
   float* acc;
+  float* parts;
 };
 
 int plan_loss_grad(const zn_weight* w, const void* x, int64_t ldx, int64_t tokens, int32_t* status, Arena& ar,
                    LossGradPlan* p) {
   *p = {};
-  int sms = 0;
-  if (int rc = sm_count(&sms)) return rc;
+  if (int rc = sm_count(&p->sms)) return rc;
   p->x_copy = plan_matrix(x, tokens, w->cols, ldx, ar);
   if (int rc = plan_weight(w, std::max<int64_t>(256, kProbBytes / 2 / tokens), status, ar, &p->w)) return rc;
-  p->cut = cut_of(tokens, p->w.piece_rows, w->cols, sms, false);
-  p->cut_dh = cut_of(tokens, w->cols, p->w.piece_rows, sms, true);
+  p->cut = cut_of(tokens, p->w.piece_rows, w->cols, p->sms, false);
   p->ldp = round8(p->w.piece_rows);
   p->prob = ar.take(size_t(tokens) * p->ldp * 2);
   p->ld = (w->cols + 3) & ~int64_t(3);
-  p->acc = ar.take<float>(size_t(p->cut_dh.splits) * tokens * p->ld * 4);
+  p->acc = ar.take<float>(size_t(tokens) * p->ld * 4);
+  p->parts = ar.take<float>(parts_bytes(p->sms));
   return ZN_OK;
 }
 
@@ -1003,17 +981,17 @@ int run_loss_grad(const LossGradPlan& p, const void* x, int64_t ldx, int64_t tok
     Matrix wm;
     if (int rc = load_piece(p.w, r0, r1, x_job, &wm, s)) return rc;
     const EpiProb<T> e{rows, static_cast<T*>(p.prob), tokens, r1 - r0, p.ldp, r0, kLog2e / temperature, gain};
-    if (int rc = product<T, false>(xm, wm, p.cut, e, p.w.status, s)) return rc;
+    const Cut cut = whole_cut(p.cut.cg, tokens, r1 - r0);
+    if (int rc = product<T, false>(xm, wm, cut, nullptr, e, p.w.status, s)) return rc;
     const Matrix pm{p.prob, tokens, r1 - r0, p.ldp};
     const EpiAccum a{p.acc, tokens, cols, p.ld, r0 > 0};
-    if (int rc = product<T, true>(pm, wm, p.cut_dh, a, p.w.status, s)) return rc;
+    if (int rc = product<T, true>(pm, wm, p.sms, p.parts, a, p.w.status, s)) return rc;
   }
   Finish<T> f{};
   f.acc = p.acc;
   f.M = tokens;
   f.N = cols;
   f.ld = p.ld;
-  f.splits = p.cut_dh.splits;
   f.lin.y = static_cast<T*>(dx);
   f.lin.ldy = cols;
   f.grad = grad;
