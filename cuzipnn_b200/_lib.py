@@ -68,10 +68,9 @@ SIGNATURES |= {
     "zn_linear_grad_temp_bytes": (_sz, [_w, _p, _i64, _i64, _i32, _i32, _i32]),
     "zn_linear_grad": (_i32, [_w, _p, _i64, _i64, _p, _p, _p, _p, _p, _sz, _p]),
     "zn_loss_state_bytes": (_sz, [_i64, _i32]),
-    "zn_loss_temp_bytes": (_sz, [_w, _p, _i64, _i64]),
-    "zn_loss": (_i32, [_w, _p, _i64, _i64, _p, _p, _i32, _i64, _f, _i32, _p, _p, _p, _p, _sz, _p]),
-    "zn_loss_grad_temp_bytes": (_sz, [_w, _p, _i64, _i64]),
-    "zn_loss_grad": (_i32, [_w, _p, _i64, _i64, _i32, _f, _i32, _p, _p, _p, _p, _p, _sz, _p]),
+    "zn_loss_temp_bytes": (_sz, [_w, _p, _i64, _i64, _i32, _i32]),
+    "zn_loss": (_i32, [_w, _p, _i64, _i64, _p, _p, _i32, _i64, _f, _i32, _p, _p, _p, _p, _p, _sz, _p]),
+    "zn_loss_grad": (_i32, [_i32, _i64, _i64, _i32, _i32, _p, _p, _p, _p, _p]),
 }
 
 

@@ -30,7 +30,7 @@ _MAX_TOP = 256
 _MAX_DIM = 1 << 31
 _MIN_TEMPERATURE, _MAX_TEMPERATURE = 2.0**-20, 2.0**20  # its square and inverse stay far inside float32
 _ENTRIES = {name: (getattr(_lib.lib, name + "_temp_bytes"), getattr(_lib.lib, name))
-            for name in ("zn_linear", "zn_linear_grad", "zn_loss", "zn_loss_grad")}
+            for name in ("zn_linear", "zn_linear_grad", "zn_loss")}
 
 
 def upload_blob(blob: torch.Tensor, *, compute_device: torch.device | str | None = None) -> torch.Tensor:
@@ -232,59 +232,59 @@ def blob_linear(
         return y
 
 
-def _loss_forward(w: _Weight, hidden, ids, logits, top, ignore_index, temperature, reduction, status):
-    """(loss, state, hidden as rows, their pitch)"""
+def _loss_forward(w: _Weight, hidden, ids, logits, top, ignore_index, temperature, reduction, want_grad, status):
+    """(loss, the rows' own gradients in 32 bits or None, state)"""
     h, ldh = _rows(hidden, w.cols)
     tokens = h.shape[0]
-    loss = torch.empty(ids.shape[0] if reduction == 2 else (), dtype=torch.float32, device=w.device)
-    state = torch.empty(max(1, int(_lib.lib.zn_loss_state_bytes(tokens, top))), dtype=torch.uint8, device=w.device)
+    loss = torch.empty(tokens if reduction == 2 else (), dtype=torch.float32, device=w.device)
+    unit = torch.empty((tokens, w.cols), dtype=torch.float32, device=w.device) if want_grad else None
+    state = torch.empty(_lib.lib.zn_loss_state_bytes(tokens, top) or 1, dtype=torch.uint8, device=w.device)
     if tokens:
-        w.call("zn_loss", (h.data_ptr(), ldh, tokens),
+        w.call("zn_loss", (h.data_ptr(), ldh, tokens, top, int(want_grad)),
                (h.data_ptr(), ldh, tokens, ids.data_ptr(), _ptr(logits), top, ignore_index, temperature, reduction,
-                loss.data_ptr(), state.data_ptr()), status)
+                loss.data_ptr(), _ptr(unit), state.data_ptr()), status)
     else:
         loss.zero_()
         status.zero_()
-    return loss, state
+    return loss, unit, state
 
 
 class _Loss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, hidden, blob, w, ids, logits, top, ignore_index, temperature, reduction):
+    def forward(ctx, hidden, w, ids, logits, top, ignore_index, temperature, reduction):
         status = torch.empty(1, dtype=torch.int32, device=w.device)
-        loss, state = _loss_forward(w, hidden, ids, logits, top, ignore_index, temperature, reduction, status)
+        loss, unit, state = _loss_forward(w, hidden, ids, logits, top, ignore_index, temperature, reduction, True,
+                                          status)
         _set_status(w.device, status)
-        ctx.w, ctx.status, ctx.args = w, status, (top, temperature, reduction)
-        ctx.save_for_backward(hidden, blob, state)
+        ctx.args = (_CODES[w.dtype], w.dtype, hidden.shape, top, reduction)
+        ctx.save_for_backward(unit, state)
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        w = ctx.w
-        hidden, _, state = ctx.saved_tensors
-        top, temperature, reduction = ctx.args
-        dh = torch.empty(hidden.shape, dtype=w.dtype, device=w.device)
+        unit, state = ctx.saved_tensors
+        code, dtype, shape, top, reduction = ctx.args
+        dh = torch.empty(shape, dtype=dtype, device=unit.device)
         if dh.numel():
-            with _on(w.device):
-                h, ldh = _rows(hidden, w.cols)
+            with _on(unit.device):
                 g = grad.float().contiguous()
-                w.call("zn_loss_grad", (h.data_ptr(), ldh, h.shape[0]),
-                       (h.data_ptr(), ldh, h.shape[0], top, temperature, reduction, state.data_ptr(), g.data_ptr(),
-                        dh.data_ptr()), ctx.status)
-        return dh, *(None,) * 8
+                _lib.check(_lib.lib.zn_loss_grad(code, unit.shape[0], unit.shape[1], top, reduction, state.data_ptr(),
+                                                 unit.data_ptr(), g.data_ptr(), dh.data_ptr(), _stream(unit.device)),
+                           "zn_loss_grad")
+        return dh, *(None,) * 7
 
 
-def _loss(hidden, blob, w, ids, logits, top, ignore_index, temperature, reduction, shape):
+def _loss(hidden, w, ids, logits, top, ignore_index, temperature, reduction, shape):
     w.place("hidden")
     red = _REDUCTIONS[reduction]
     args = (ids, logits, top, ignore_index, temperature, red)
     with _on(w.device):
         if torch.is_grad_enabled() and hidden.requires_grad:
-            loss = _Loss.apply(hidden, blob, w, *args)
+            loss = _Loss.apply(hidden, w, *args)
         else:
             status = torch.empty(1, dtype=torch.int32, device=w.device)
-            loss, _ = _loss_forward(w, hidden, *args, status)
+            loss, _, _ = _loss_forward(w, hidden, *args, False, status)
             _set_status(w.device, status)
         return loss.reshape(shape) if red == 2 else loss
 
@@ -319,16 +319,17 @@ def blob_cross_entropy(
     "sum", or with "none" one loss per row (0 where ignored).  Any other target outside the
     vocabulary makes the row's loss and gradient NaN.
 
-    Differentiable in hidden; the backward pass decodes the head and computes the logits again, a
-    piece of the vocabulary at a time.  A piece of softmax - onehot is rounded to the dtype before
-    the product with the piece (sums are in 32 bits); ignored rows get zero gradients whatever they
+    Differentiable in hidden: where hidden requires a gradient, the forward pass computes it with the
+    loss, in the same pass over the vocabulary, a piece at a time, and keeps it in 32 bits (tokens x
+    cols).  The softmax's weights are rounded to the dtype before the product with a piece, except
+    at the row's own target (sums are in 32 bits); ignored rows get zero gradients whatever they
     hold."""
     _check_reduction(reduction)
     w = _Weight(blob, hidden, "hidden")
     shape = tuple(hidden.shape[:-1])
     _check_ids("targets", targets, shape, w)
     ids = targets.detach().reshape(-1).contiguous()
-    return _loss(hidden, blob, w, ids, None, 1, int(ignore_index), 1.0, reduction, shape)
+    return _loss(hidden, w, ids, None, 1, int(ignore_index), 1.0, reduction, shape)
 
 
 def blob_distillation(
@@ -370,4 +371,4 @@ def blob_distillation(
         raise ValueError(f"teacher_logits is on {teacher_logits.device}, hidden on {w.device}")
     ids = teacher_ids.detach().reshape(-1, top).contiguous()
     logits = teacher_logits.detach().reshape(-1, top).float().contiguous()
-    return _loss(hidden, blob, w, ids, logits, top, 0, temperature, reduction, shape)
+    return _loss(hidden, w, ids, logits, top, 0, temperature, reduction, shape)

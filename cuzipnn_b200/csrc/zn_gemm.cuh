@@ -45,6 +45,7 @@ struct GemmShape {
   int rest, splits;      // the `rest` last ones in `splits` parts of the contraction each,
   float* parts;          // whose sums go to parts[rest][splits][tile rows][tile columns]
   int32_t* status;
+  const int32_t* go;     // or null: the kernel does nothing where *go is 0
 };
 
 // Tile order: within a group of row tiles, the row tile runs fastest, then the column tile, so that
@@ -241,14 +242,15 @@ __device__ constexpr uint32_t instr_desc() {
          (uint32_t(GemmCfg<CG>::kBN / 8) << 17) | (uint32_t(kBM * CG / 16) << 24);
 }
 
-// acc[m][n] (32 bits) = or += the tile: what a product over one piece of a contraction adds to the
-// pieces before, or a part of a tile's contraction.  A thread's 128 bytes per 32 columns go through
+// acc[m][n] (32 bits) = the tile, or acc[m][n] * scale[m] + the tile: what a product over one piece of a
+// contraction adds to the pieces before, or a part of a tile's contraction.  A thread's 128 bytes per 32 columns go through
 // the staging buffer, so that the warp reads and writes 4 rows of whole 128-byte lines at a time.
 struct EpiAccum {
   static constexpr bool kParts = true;
   float* acc;
   int64_t M, N, ld;  // ld: a multiple of 4
   bool add;
+  const float* scale;  // with add, or null: 1
   struct Row {
     int64_t m, n0;
     uint8_t* buf;
@@ -270,7 +272,8 @@ struct EpiAccum {
         s[i] = *at(r, lane & 7);
         if (e.add && m0 + r < e.M && n < e.N) {
           const float4 o = *reinterpret_cast<const float4*>(e.acc + (m0 + r) * e.ld + n);
-          s[i] = make_float4(s[i].x + o.x, s[i].y + o.y, s[i].z + o.z, s[i].w + o.w);
+          const float f = e.scale ? e.scale[m0 + r] : 1.0f;
+          s[i] = make_float4(fmaf(o.x, f, s[i].x), fmaf(o.y, f, s[i].y), fmaf(o.z, f, s[i].z), fmaf(o.w, f, s[i].w));
         }
       }
 #pragma unroll
@@ -305,6 +308,10 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
   const uint32_t accfull0 = empty0 + 8 * kStages, accempty0 = accfull0 + 16, drain = accempty0 + 16;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = CG == 2 ? cta_rank() : 0;
+  if (g.go) {  // the same value for every CTA: the kernel before wrote it
+    pdl_wait();
+    if (*reinterpret_cast<const volatile int32_t*>(g.go) == 0) return;
+  }
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
@@ -455,7 +462,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
       const int64_t m = rank * kBM + quarter * 32 + lane, c0 = half * kHalf;  // in the tile
       if constexpr (Epi::kParts) {
         if (part >= 0) {
-          const EpiAccum e{g.parts + int64_t(part) * (CG * kBM * BN), CG * kBM, BN, BN, false};
+          const EpiAccum e{g.parts + int64_t(part) * (CG * kBM * BN), CG * kBM, BN, BN, false, nullptr};
           EpiAccum::Row row(e, m, c0, buf);
           drain_tile(row, e);
           continue;
@@ -518,7 +525,8 @@ inline Cut whole_cut(int cg, int64_t M, int64_t N) { return {cg, cdiv(M, 128 * c
 // Bytes of GemmShape::parts that any cut needs: a tile per CTA or pair.
 inline size_t parts_bytes(int sms) { return size_t(sms) * (2 * kBM * kBM) * sizeof(float); }
 
-inline GemmShape gemm_shape(int64_t M, int64_t N, int64_t K, const Cut& cut, float* parts, int32_t* status) {
+inline GemmShape gemm_shape(int64_t M, int64_t N, int64_t K, const Cut& cut, float* parts, int32_t* status,
+                            const int32_t* go = nullptr) {
   GemmShape g{};
   g.M = M;
   g.N = N;
@@ -532,6 +540,7 @@ inline GemmShape gemm_shape(int64_t M, int64_t N, int64_t K, const Cut& cut, flo
   g.splits = cut.splits;
   g.parts = parts;
   g.status = status;
+  g.go = go;
   return g;
 }
 

@@ -188,33 +188,19 @@ __device__ __forceinline__ void finish_value(const EpiLinear<T>& e, int64_t m, i
   if (e.slope) e.slope[m * e.ldy + n] = int16_t(slope_code(sl));
 }
 
-// y = act(z + bias) + residual from z = acc, or from weight_dot; or y = z * (a scale per row) for the
-// gradient of a loss.
+// y = act(z + bias) + residual from z = acc, or from weight_dot.
 template <typename T>
 struct Finish {
   const float* acc;  // [M][ld], or null: dot
   int64_t M, N, ld;
   DotValue dot;
   EpiLinear<T> lin;
-  // gradient of a loss: row m is scaled by T * grad / (rows that count for a mean) / gain
-  const float* grad;  // or null
-  int64_t grad_step;
-  const int32_t* count;
-  const float* mean_rows;  // or null
-  float factor;
 };
 
 template <typename T>
 __device__ __forceinline__ void finish_element(const Finish<T>& f, int64_t i) {
   const int64_t m = i / f.N, n = i - m * f.N;
-  float z = f.acc ? f.acc[m * f.ld + n] : f.dot.get(m, n);
-  if (!f.grad) {
-    finish_value(f.lin, m, n, z);
-    return;
-  }
-  if (f.count[m] == 0) z = 0.0f;
-  else z *= f.factor * f.grad[m * f.grad_step] / (f.mean_rows ? *f.mean_rows : 1.0f);
-  f.lin.y[m * f.lin.ldy + n] = Num<T>::from(z);
+  finish_value(f.lin, m, n, f.acc ? f.acc[m * f.ld + n] : f.dot.get(m, n));
 }
 
 // weight_dot, then f (whose dot it fills in) on every element.

@@ -4,16 +4,27 @@
 // scratch (about one wave of the decoder, so that a weight of any size needs a bounded buffer) and
 // multiplies each piece on the tensor cores (zn_gemm.cuh), with the rest of the operator in the
 // product's epilogue:
-//   linear          y = act(x W^T + b) + r                       EpiLinear
-//   loss, forward   running max and sum of exp over the columns  EpiStats (per row and column tile)
-//   loss, backward  P = softmax(s) - q, one piece wide           EpiProb, then dh += P W by EpiAccum
+//   linear              y = act(x W^T + b) + r                   EpiLinear
+//   loss                running maximum and sum of exp           EpiStats (per row and half tile)
+//   loss and gradient   P = exp(s - r), one piece wide           EpiSoft, then acc += P W by EpiAccum
 // A product with at most kDotRows rows is bound by decoding; it runs inside the decoder instead
 // (weight_dot) and W is never written at all.
 //
 // Losses.  With s = h W^T / T, lse = log sum_v exp s_v and a sparse distribution q over the ids of
 // a row (sum q = 1):  L = T^2 (sum_k q_k (log q_k - s_{id_k}) + lse),  dL/dh = T (softmax(s) - q) W.
-// A cross entropy is the case of one id with q = 1 and T = 1.  The logits are never kept: the
-// backward pass computes a piece of them again.
+// A cross entropy is the case of one id with q = 1 and T = 1.  The logits are never kept.
+//
+// The gradient comes with the loss, in one pass over the vocabulary, like attention with W as keys
+// and values:  softmax(s) W = (sum_v exp(s_v - r) W_v) / (sum_v exp(s_v - r)) for any reference r of
+// the row.  Each piece is decoded once and multiplied twice (4 tokens rows cols operations in all,
+// against 6 and two decodings for computing the logits again in a backward pass).  r is the maximum
+// over the first kSample rows of W; the 16-bit P then holds exp(s - r) up to a bound (2^100 for
+// bf16, 2^15 for fp16).  Where a group of 32 logits passes the bound, its P is zero, the row's r is
+// raised to its maximum, what was summed is scaled down, and the piece is multiplied again with
+// the groups that were left out alone (kernels that end at once when there are none).
+// P is rounded to 16 bits.  At the row's own ids that would be wrong where it matters most (a
+// confident softmax less q is a small difference), so P is zero there and the ids' terms
+// (exp(s_k - r) and q_k times their rows of W) are added in 32 bits by gather_kernel.
 #include <algorithm>
 
 #include "zn_linear.cuh"
@@ -60,7 +71,6 @@ constexpr int kMaxTop = 256;
 
 // Per-row state of a loss (state buffer of a call, kept for the backward pass).
 struct LossRows {
-  float* lse;      // log sum exp of s (NaN for a row with an id out of range)
   float* q0;       // sum_k q_k log q_k
   int32_t* count;  // ids of the row (0: the row does not count; -1: an id is out of range)
   int32_t* ids;    // [tokens][top], ascending
@@ -80,6 +90,13 @@ __device__ __forceinline__ int first_id(const int32_t* ids, int count, int64_t n
   return lo;
 }
 
+// 2^x, as the unit computes it (2 units of the last place; subnormal results are 0).
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // One pass over the logits of a row: running maximum and sum of 2^(s' - max) with s' = s log2(e),
 // and sum_k q_k s'_{id_k} over the row's ids among the columns seen.
 struct RowStats {
@@ -88,7 +105,7 @@ struct RowStats {
 __device__ __forceinline__ void stats_join(RowStats& a, float mx, float sum, float hit) {
   const float m = fmaxf(a.mx, mx);
   const float base = m == -INFINITY ? 0.0f : m;
-  a.sum = a.sum * exp2f(a.mx - base) + sum * exp2f(mx - base);
+  a.sum = a.sum * ex2(a.mx - base) + sum * ex2(mx - base);
   a.mx = m;
   a.hit += hit;
 }
@@ -136,8 +153,8 @@ struct EpiStats {
       const float m2 = fmaxf(st.mx, mx), base = m2 == -INFINITY ? 0.0f : m2;
       float sum = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) sum += exp2f(s[i] - base);
-      st.sum = st.sum * exp2f(st.mx - base) + sum;
+      for (int i = 0; i < 32; ++i) sum += ex2(s[i] - base);
+      st.sum = st.sum * ex2(st.mx - base) + sum;
       st.mx = m2;
       if (next < n0 + c + 32) {
 #pragma unroll
@@ -159,60 +176,98 @@ struct EpiStats {
   };
 };
 
-// P = (softmax(s) - q) * gain of one piece, in 16 bits, as the operand of the product with the
-// piece.  gain keeps small probabilities out of fp16's subnormals (2^15: |softmax - q| <= 1); bf16
-// has the range of 32 bits (gain 1).  Rows that do not count are zero whatever their logits are.
-template <typename T>
-struct EpiProb {
+// State of a loss with its gradient, per row, in units of log2(e) (s' = s log2(e)).
+struct SoftRows {
+  float* ref;      // r
+  float* before;   // r before this piece
+  float* scale;    // 2^(before - r)
+  float* sum;      // sum of 2^(s' - r) over the columns so far
+  float* hit;      // [tokens][top] s' at the row's ids
+  int32_t* again;  // of this piece: a group was left out
+};
+
+// P = 2^(s' - r) of one piece, in 16 bits, as the operand of the product with the piece; zero at the
+// row's ids, and in rows that do not count whatever their logits are.  AGAIN: the groups that the
+// first pass left out, with the r that was raised for them.
+template <typename T, bool AGAIN>
+struct EpiSoft {
   static constexpr bool kParts = false;
+  static constexpr float kBound = Num<T>::kCode == 1 ? 100.0f : 15.0f;
   LossRows rows;
+  SoftRows soft;
   T* p;
-  int64_t M, N, ld, v0;  // ld: a multiple of 8
-  float scale, gain;
+  float* part;       // [half tile][2][M]: sum, and the maximum s' of the groups left out
+  int64_t M, N, ld;  // N: columns of this piece; ld: a multiple of 8
+  int64_t v0;        // first vocabulary row of this piece
+  int tile_cols;     // columns of a half tile
+  float scale;       // log2(e) / T
   struct Row {
     int64_t m, n0;
-    const int32_t* ids;
-    const float* q;
-    float off;
-    int at, count;
-    int64_t next;
     uint8_t* buf;
-    __device__ __forceinline__ Row(const EpiProb& e, int64_t m_, int64_t n0_, uint8_t* b)
-        : m(m_), n0(n0_), buf(b) {
+    const int32_t* ids;
+    float ref, before, sum, out;
+    int at, count;
+    int64_t next;  // column (of the piece) of the next id
+    __device__ __forceinline__ Row(const EpiSoft& e, int64_t m_, int64_t n0_, uint8_t* b) : m(m_), n0(n0_), buf(b) {
       at = count = 0;
       next = INT64_MAX;
-      off = 0.0f;
+      ref = before = sum = 0.0f;
+      out = -INFINITY;
       ids = nullptr;
-      q = nullptr;
       if (m < e.M) {
-        count = e.rows.count[m];
-        off = e.rows.lse[m] * kLog2e;
+        count = max(0, e.rows.count[m]);
+        ref = e.soft.ref[m];
+        before = AGAIN ? e.soft.before[m] : ref;
         ids = e.rows.ids + m * e.rows.top;
-        q = e.rows.q + m * e.rows.top;
         at = first_id(ids, count, e.v0 + n0);
         if (at < count) next = ids[at] - e.v0;
       }
     }
-    __device__ __forceinline__ void cols(const EpiProb& e, int c, float* v) {
+    __device__ __forceinline__ void cols(const EpiSoft& e, int c, float* v) {
       if (n0 + c >= e.N) return;
+      const int left = int(min(int64_t(32), e.N - n0 - c));
+      float mx = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = count == 0 ? 0.0f : exp2f(v[i] * e.scale - off);
-      if (next < n0 + c + 32) {
+      for (int i = 0; i < 32; ++i)
+        if (i < left) mx = fmaxf(mx, v[i]);
+      const bool over = before == -INFINITY ? mx > -INFINITY : fmaf(mx, e.scale, -before) > kBound;
+      const bool take = count > 0 && over == AGAIN;
+      if (!AGAIN && over) out = fmaxf(out, mx * e.scale);
+      if (next < n0 + c + 32) {  // the ids' logits, and their columns out of P
+        const float base = ref == -INFINITY ? 0.0f : ref;
 #pragma unroll
         for (int i = 0; i < 32; ++i)
-          while (next == n0 + c + i) {
-            v[i] -= q[at];
-            ++at;
-            next = at < count ? ids[at] - e.v0 : INT64_MAX;
+          if (next == n0 + c + i) {
+            if (take) sum += ex2(fmaf(v[i], e.scale, -base));
+            while (next == n0 + c + i) {
+              if (!AGAIN) e.soft.hit[m * e.rows.top + at] = v[i] * e.scale;
+              ++at;
+              next = at < count ? ids[at] - e.v0 : INT64_MAX;
+            }
+            v[i] = -INFINITY;
           }
       }
+      const float base = ref == -INFINITY ? 0.0f : ref;
+      float add = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const float t = ex2(fmaf(v[i], e.scale, -base));
+        v[i] = take && i < left ? t : 0.0f;
+        add += v[i];
+      }
+      sum += add;
       uint32_t w[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) w[i] = Num<T>::pack(v[2 * i] * e.gain, v[2 * i + 1] * e.gain);
+      for (int i = 0; i < 16; ++i) w[i] = Num<T>::pack(v[2 * i], v[2 * i + 1]);
       // The pitch covers the last group of 8 columns.
       stage_rows(buf, w, e.p, e.ld, m - (threadIdx.x & 31), e.M, n0 + c, e.ld, true);
     }
-    __device__ __forceinline__ void end(const EpiProb&) {}
+    __device__ __forceinline__ void end(const EpiSoft& e) {
+      if (m >= e.M || n0 >= e.N) return;
+      float* p = e.part + (n0 / e.tile_cols) * 2 * e.M + m;
+      p[0] = sum;
+      p[e.M] = count > 0 ? out : -INFINITY;
+    }
   };
 };
 
@@ -228,7 +283,7 @@ __device__ __forceinline__ void parts_end(const EpiAccum& e, int64_t m, int64_t 
   for (int i = 0; i < 4; ++i)
     if (n + i < e.N) {
       float* p = e.acc + m * e.ld + n + i;
-      *p = (e.add ? *p : 0.0f) + v[i];
+      *p = e.add ? fmaf(*p, e.scale ? e.scale[m] : 1.0f, v[i]) : v[i];
     }
 }
 template <typename T>
@@ -462,7 +517,7 @@ __global__ void __launch_bounds__(256) dot_stats_kernel(DotValue v, LossRows row
   float sum = 0.0f, hit = 0.0f;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    sum += exp2f(s[i] - base);
+    sum += ex2(s[i] - base);
     const int64_t n = n0 + threadIdx.x + 256 * i;
     if (n < n1)
       for (int k = first_id(ids, count, n); k < count && ids[k] == n; ++k) hit += q[k] * s[i];
@@ -505,8 +560,170 @@ __global__ void __launch_bounds__(1024) loss_rows_kernel(const float* part, int6
   for (int i = 1; i < 32; ++i) stats_join(st, sm[i][threadIdx.x].mx, sm[i][threadIdx.x].sum, sm[i][threadIdx.x].hit);
   const int count = rows.count[m];
   const float lse = count < 0 ? NAN : (st.mx + log2f(st.sum)) * kLn2;
-  rows.lse[m] = lse;
   loss[m] = count == 0 ? 0.0f : temperature * temperature * (rows.q0[m] + (lse - st.hit * kLn2));
+}
+
+// The first reference of each row: its maximum over the columns of the sample.
+__global__ void __launch_bounds__(1024) sample_kernel(const float* part, int64_t tiles, int64_t tokens, SoftRows soft) {
+  pdl_wait();
+  pdl_trigger();
+  const int64_t m = int64_t(blockIdx.x) * 32 + (threadIdx.x & 31);
+  const int sub = threadIdx.x >> 5;
+  float mx = -INFINITY;
+  if (m < tokens)
+    for (int64_t t = sub; t < tiles; t += 32) mx = fmaxf(mx, part[t * 3 * tokens + m]);
+  __shared__ float sm[32][33];
+  sm[sub][threadIdx.x & 31] = mx;
+  __syncthreads();
+  if (sub != 0 || m >= tokens) return;
+  for (int i = 1; i < 32; ++i) mx = fmaxf(mx, sm[i][threadIdx.x]);
+  soft.ref[m] = mx;
+  soft.sum[m] = 0.0f;
+}
+
+// After a piece: its sums to the rows', and a new reference for the rows with groups left out.
+__global__ void __launch_bounds__(1024) soft_rows_kernel(const float* part, int64_t tiles, int64_t tokens,
+                                                         SoftRows soft) {
+  pdl_wait();
+  pdl_trigger();
+  const int64_t m = int64_t(blockIdx.x) * 32 + (threadIdx.x & 31);
+  const int sub = threadIdx.x >> 5;
+  float sum = 0.0f, out = -INFINITY;
+  if (m < tokens)
+    for (int64_t t = sub; t < tiles; t += 32) {
+      sum += part[t * 2 * tokens + m];
+      out = fmaxf(out, part[t * 2 * tokens + tokens + m]);
+    }
+  __shared__ float2 sm[32][33];
+  sm[sub][threadIdx.x & 31] = make_float2(sum, out);
+  __syncthreads();
+  if (sub != 0 || m >= tokens) return;
+  for (int i = 1; i < 32; ++i) {
+    sum += sm[i][threadIdx.x].x;
+    out = fmaxf(out, sm[i][threadIdx.x].y);
+  }
+  const float ref = soft.ref[m];
+  sum += soft.sum[m];
+  soft.before[m] = ref;
+  float scale = 1.0f;
+  if (out > -INFINITY) {
+    const float raised = fmaxf(ref, out);
+    scale = ref == -INFINITY ? 0.0f : ex2(ref - raised);
+    soft.ref[m] = raised;
+    *soft.again = 1;
+  }
+  soft.scale[m] = scale;
+  soft.sum[m] = sum * scale;
+}
+
+// The terms of a row's ids in this piece: acc += 2^(s'_k - r) W[id_k], acc_q += q_k W[id_k], in 32 bits;
+// and the sums of the groups that were multiplied again.  One CTA per row.
+template <typename T>
+__global__ void __launch_bounds__(128) gather_kernel(LossRows rows, SoftRows soft, const T* w, int64_t pitch,
+                                                     int64_t v0, int64_t v1, int64_t cols, float* acc, float* acc_q,
+                                                     int64_t ld, const float* part, int64_t tiles, int64_t tokens) {
+  pdl_wait();
+  pdl_trigger();
+  __shared__ float s_p[kMaxTop], s_q[kMaxTop], s_sum[128];
+  const int64_t m = blockIdx.x;
+  const int count = max(0, rows.count[m]), tid = threadIdx.x;
+  const int32_t* ids = rows.ids + m * rows.top;
+  const int a = first_id(ids, count, v0), b = first_id(ids, count, v1);
+  if (*soft.again) {
+    float v = 0.0f;
+    for (int64_t t = tid; t < tiles; t += 128) v += part[t * 2 * tokens + m];
+    s_sum[tid] = v;
+    __syncthreads();
+    for (int o = 64; o; o >>= 1) {
+      if (tid < o) s_sum[tid] += s_sum[tid + o];
+      __syncthreads();
+    }
+    if (tid == 0) soft.sum[m] += s_sum[0];
+  }
+  if (a == b) return;
+  const float ref = soft.ref[m], base = ref == -INFINITY ? 0.0f : ref;
+  for (int k = a + tid; k < b; k += 128) {
+    // An id given twice is one column of the softmax: only its first entry carries it.
+    s_p[k - a] = k > a && ids[k] == ids[k - 1] ? 0.0f : ex2(soft.hit[m * rows.top + k] - base);
+    s_q[k - a] = rows.q[m * rows.top + k];
+  }
+  __syncthreads();
+  for (int64_t c = 8 * tid; c < cols; c += 8 * 128) {
+    float x[8] = {}, y[8] = {};
+    for (int k = a; k < b; ++k) {
+      const uint4 q = *reinterpret_cast<const uint4*>(w + (ids[k] - v0) * pitch + c);
+      const uint32_t ww[4] = {q.x, q.y, q.z, q.w};
+      const float fp = s_p[k - a], fq = s_q[k - a];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float lo = Num<T>::lo(ww[i]), hi = Num<T>::hi(ww[i]);
+        if (fp != 0.0f) {
+          x[2 * i] = fmaf(fp, lo, x[2 * i]);
+          x[2 * i + 1] = fmaf(fp, hi, x[2 * i + 1]);
+        }
+        y[2 * i] = fmaf(fq, lo, y[2 * i]);
+        y[2 * i + 1] = fmaf(fq, hi, y[2 * i + 1]);
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < 8; h += 4)
+      if (c + h < cols) {  // the pitch covers the last group of 4
+        float4* pa = reinterpret_cast<float4*>(acc + m * ld + c + h);
+        float4* pq = reinterpret_cast<float4*>(acc_q + m * ld + c + h);
+        const float4 va = *pa, vq = *pq;
+        *pa = make_float4(va.x + x[h], va.y + x[h + 1], va.z + x[h + 2], va.w + x[h + 3]);
+        *pq = make_float4(vq.x + y[h], vq.y + y[h + 1], vq.z + y[h + 2], vq.w + y[h + 3]);
+      }
+  }
+}
+
+// A row's loss, and its gradient T (acc / sum - acc_q).  One CTA per row.
+__global__ void __launch_bounds__(128) soft_end_kernel(LossRows rows, SoftRows soft, const float* acc,
+                                                       const float* acc_q, int64_t ld, int64_t cols, float temperature,
+                                                       float* loss, float* unit) {
+  pdl_wait();
+  pdl_trigger();
+  __shared__ float s_sum[128];
+  const int64_t m = blockIdx.x;
+  const int count = rows.count[m], tid = threadIdx.x;
+  float hit = 0.0f;
+  for (int k = tid; k < count; k += 128) hit += rows.q[m * rows.top + k] * soft.hit[m * rows.top + k];
+  s_sum[tid] = hit;
+  __syncthreads();
+  for (int o = 64; o; o >>= 1) {
+    if (tid < o) s_sum[tid] += s_sum[tid + o];
+    __syncthreads();
+  }
+  const float sum = soft.sum[m];
+  if (tid == 0) {
+    const float lse = count < 0 ? NAN : (soft.ref[m] + log2f(sum)) * kLn2;
+    loss[m] = count == 0 ? 0.0f : temperature * temperature * (rows.q0[m] + (lse - s_sum[0] * kLn2));
+  }
+  const float f = temperature / sum;
+  for (int64_t c = tid; c < cols; c += 128) {
+    float v = 0.0f;
+    if (count < 0) v = NAN;
+    else if (count > 0) v = fmaf(acc[m * ld + c], f, -temperature * acc_q[m * ld + c]);
+    unit[m * cols + c] = v;
+  }
+}
+
+// dh = unit * (gradient of the row's loss) in 16 bits.
+template <typename T>
+__global__ void __launch_bounds__(256) unit_kernel(const float* unit, int64_t tokens, int64_t cols, LossRows rows,
+                                                   const float* grad, int64_t grad_step, bool mean, T* dh) {
+  pdl_wait();
+  pdl_trigger();
+  const int64_t per_row = cdiv(cols, 256), total = tokens * per_row;
+  const int lane = threadIdx.x & 31;
+  for (int64_t i = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5); i < total; i += int64_t(gridDim.x) * 8) {
+    const int64_t m = i / per_row, c0 = (i - m * per_row) * 256 + lane;
+    const bool counts = rows.count[m] != 0;
+    const float f = counts ? grad[m * grad_step] / (mean ? *rows.rows : 1.0f) : 0.0f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (c0 + 32 * k < cols) dh[m * cols + c0 + 32 * k] = Num<T>::from(counts ? unit[m * cols + c0 + 32 * k] * f : 0.0f);
+  }
 }
 
 // Sum or mean over the rows that count, added in 64 bits by one block in a fixed order.
@@ -648,13 +865,13 @@ Matrix load_matrix(const void* p, int64_t rows, int64_t cols, int64_t pitch, voi
 
 template <typename T, bool BMN, class Epi>
 int product(const Matrix& a, const Matrix& b, const Cut& cut, float* parts, const Epi& epi, int32_t* status,
-            cudaStream_t s) {
+            cudaStream_t s, const int32_t* go = nullptr) {
   const int64_t M = a.rows, K = a.cols, N = BMN ? b.cols : b.rows;
   constexpr bool bf16 = Num<T>::kCode == 1;
   CUtensorMap ma, mb;
   if (int rc = make_map(&ma, a.p, a.rows, a.cols, a.pitch, kBM, bf16)) return rc;
   if (int rc = make_map(&mb, b.p, b.rows, b.cols, b.pitch, BMN ? kBK : 128, bf16)) return rc;
-  const GemmShape g = gemm_shape(M, N, K, cut, parts, status);
+  const GemmShape g = gemm_shape(M, N, K, cut, parts, status, go);
   if (int rc = cut.cg == 2 ? launch_gemm<T, 2, BMN>(ma, mb, g, epi, s) : launch_gemm<T, 1, BMN>(ma, mb, g, epi, s))
     return rc;
   if constexpr (Epi::kParts) {
@@ -834,7 +1051,7 @@ int run_linear_grad(const LinearGradPlan& p, const zn_weight* w, const void* dy,
     if (int rc = load_piece(p.w, r0, r1, dy_job, &wm, s)) return rc;
     // Columns [r0, r1) of dz (r0 is a multiple of 256: the rows stay 16-byte aligned).
     const Matrix a{static_cast<const T*>(dzm.p) + r0, tokens, r1 - r0, dzm.pitch};
-    const EpiAccum acc{p.acc, tokens, cols, p.ld, r0 > 0};
+    const EpiAccum acc{p.acc, tokens, cols, p.ld, r0 > 0, nullptr};
     if (int rc = p.acc ? product<T, true>(a, wm, p.sms, p.parts, acc, p.w.status, s)
                        : product<T, true>(a, wm, p.sms, p.parts, e, p.w.status, s))
       return rc;
@@ -854,7 +1071,6 @@ int run_linear_grad(const LinearGradPlan& p, const zn_weight* w, const void* dy,
 LossRows loss_state(void* state, int64_t tokens, int top, size_t* bytes) {
   Arena ar{static_cast<uint8_t*>(state)};
   LossRows r{};
-  r.lse = ar.take<float>(size_t(tokens) * 4);
   r.q0 = ar.take<float>(size_t(tokens) * 4);
   r.count = ar.take<int32_t>(size_t(tokens) * 4);
   r.ids = ar.take<int32_t>(size_t(tokens) * top * 4);
@@ -939,8 +1155,9 @@ int run_loss(const LossPlan& p, const void* x, int64_t ldx, int64_t tokens, cons
                       rows, tokens, reduction == kMean, loss);
 }
 
-// The backward pass's pieces are bounded so that P [tokens, piece] stays within 512 MB too.
+// With the gradient, pieces are bounded so that P [tokens, piece] stays within 512 MB too.
 constexpr int64_t kProbBytes = int64_t(1) << 29;
+constexpr int64_t kSample = 512;
 
 struct LossGradPlan {
   Weight w;
@@ -949,11 +1166,16 @@ struct LossGradPlan {
   void* x_copy;
   void* prob;
   int64_t ldp, ld;
+  float* part;
+  float* row_loss;
   float* acc;
+  float* acc_q;  // followed by the pieces' `again` flags: zeroed together
+  size_t zeroed;
   float* parts;
+  SoftRows soft;
 };
 
-int plan_loss_grad(const zn_weight* w, const void* x, int64_t ldx, int64_t tokens, int32_t* status, Arena& ar,
+int plan_loss_grad(const zn_weight* w, const void* x, int64_t ldx, int64_t tokens, int top, int32_t* status, Arena& ar,
                    LossGradPlan* p) {
   *p = {};
   if (int rc = sm_count(&p->sms)) return rc;
@@ -963,43 +1185,85 @@ int plan_loss_grad(const zn_weight* w, const void* x, int64_t ldx, int64_t token
   p->ldp = round8(p->w.piece_rows);
   p->prob = ar.take(size_t(tokens) * p->ldp * 2);
   p->ld = (w->cols + 3) & ~int64_t(3);
+  const int64_t tiles = cdiv(std::max(p->w.piece_rows, std::min(kSample, w->rows)), 64);
+  p->part = ar.take<float>(size_t(tiles) * 3 * tokens * 4);
+  p->row_loss = ar.take<float>(size_t(tokens) * 4);
   p->acc = ar.take<float>(size_t(tokens) * p->ld * 4);
+  const size_t acc_bytes = size_t(tokens) * p->ld * 4;
+  p->zeroed = acc_bytes + size_t(p->w.pieces) * 4;
+  p->acc_q = ar.take<float>(p->zeroed);
+  p->soft.again = p->acc_q ? reinterpret_cast<int32_t*>(reinterpret_cast<uint8_t*>(p->acc_q) + acc_bytes) : nullptr;
   p->parts = ar.take<float>(parts_bytes(p->sms));
+  for (float** f : {&p->soft.ref, &p->soft.before, &p->soft.scale, &p->soft.sum}) *f = ar.take<float>(size_t(tokens) * 4);
+  p->soft.hit = ar.take<float>(size_t(tokens) * top * 4);
   return ZN_OK;
 }
 
+// One decoded piece: P and its sums, acc += P W, again for the groups left out, and the ids' terms.
 template <typename T>
-int run_loss_grad(const LossGradPlan& p, const void* x, int64_t ldx, int64_t tokens, float temperature, int reduction,
-                  const LossRows& rows, const float* grad, void* dx, cudaStream_t s) {
+int soft_piece(const LossGradPlan& p, const Matrix& xm, const Matrix& wm, int64_t r0, const LossRows& rows,
+               const SoftRows& soft, float scale, cudaStream_t s) {
+  const int64_t tokens = xm.rows, cols = xm.cols, n = wm.rows;
+  const int half = 64 * p.cut.cg;
+  const int64_t tiles = cdiv(n, half);
+  const unsigned row_blocks = unsigned(cdiv(tokens, 32));
+  const Matrix pm{p.prob, tokens, n, p.ldp};
+  const Cut cut = whole_cut(p.cut.cg, tokens, n);
+  if (r0 == 0) {
+    const Matrix first{wm.p, std::min(kSample, n), cols, wm.pitch};
+    const Cut c = cut_of(tokens, first.rows, cols, p.sms, false);
+    const EpiStats e{rows, p.part, tokens, first.rows, 0, 0, 64 * c.cg, scale};
+    if (int rc = product<T, false>(xm, first, c, nullptr, e, p.w.status, s)) return rc;
+    if (int rc = launch_after(sample_kernel, dim3(row_blocks), 1024, 0, s, "sample_kernel",
+                              static_cast<const float*>(p.part), cdiv(first.rows, 64 * c.cg), tokens, soft))
+      return rc;
+  }
+  const EpiSoft<T, false> e{rows, soft, static_cast<T*>(p.prob), p.part, tokens, n, p.ldp, r0, half, scale};
+  if (int rc = product<T, false>(xm, wm, cut, nullptr, e, p.w.status, s)) return rc;
+  const EpiAccum a{p.acc, tokens, cols, p.ld, r0 > 0, nullptr};
+  if (int rc = product<T, true>(pm, wm, p.sms, p.parts, a, p.w.status, s)) return rc;
+  if (int rc = launch_after(soft_rows_kernel, dim3(row_blocks), 1024, 0, s, "soft_rows_kernel",
+                            static_cast<const float*>(p.part), tiles, tokens, soft))
+    return rc;
+  const EpiSoft<T, true> e2{rows, soft, static_cast<T*>(p.prob), p.part, tokens, n, p.ldp, r0, half, scale};
+  if (int rc = product<T, false>(xm, wm, cut, nullptr, e2, p.w.status, s, soft.again)) return rc;
+  const EpiAccum a2{p.acc, tokens, cols, p.ld, true, soft.scale};
+  const Cut whole = cut_of(tokens, cols, n, p.sms, false);
+  if (int rc = product<T, true>(pm, wm, whole, nullptr, a2, p.w.status, s, soft.again)) return rc;
+  return launch_after(gather_kernel<T>, dim3(unsigned(tokens)), 128, 0, s, "gather_kernel", rows, soft,
+                      static_cast<const T*>(wm.p), wm.pitch, r0, r0 + n, cols, p.acc, p.acc_q, p.ld,
+                      static_cast<const float*>(p.part), tiles, tokens);
+}
+
+template <typename T>
+int run_loss_grad(const LossGradPlan& p, const void* x, int64_t ldx, int64_t tokens, const int64_t* ids,
+                  const float* logits, int64_t ignore, float temperature, int reduction, float* loss, float* unit,
+                  const LossRows& rows, cudaStream_t s) {
   const int64_t vocab = p.w.b.rows, cols = p.w.b.cols;
-  const float gain = Num<T>::kCode == 1 ? 1.0f : 32768.0f;
+  const float inv_t = 1.0f / temperature;
+  const cudaError_t err = cudaMemsetAsync(p.acc_q, 0, p.zeroed, s);
+  if (err != cudaSuccess) return set_error(ZN_ERR_CUDA, "zn_loss: %s", cudaGetErrorString(err));
+  if (int rc = launch_after(loss_prep_kernel, dim3(unsigned(cdiv(tokens, 4))), 128, 0, s, "loss_prep_kernel", ids,
+                            logits, tokens, vocab, ignore, inv_t, rows))
+    return rc;
   if (int rc = start_weight(p.w, s)) return rc;
   PitchCopy x_job;
   const Matrix xm = load_matrix(x, tokens, cols, ldx, p.x_copy, &x_job);
-  for (int64_t r0 = 0; r0 < vocab; r0 += p.w.piece_rows) {
+  SoftRows soft = p.soft;
+  for (int64_t r0 = 0; r0 < vocab; r0 += p.w.piece_rows, ++soft.again) {
     const int64_t r1 = std::min(vocab, r0 + p.w.piece_rows);
     Matrix wm;
     if (int rc = load_piece(p.w, r0, r1, x_job, &wm, s)) return rc;
-    const EpiProb<T> e{rows, static_cast<T*>(p.prob), tokens, r1 - r0, p.ldp, r0, kLog2e / temperature, gain};
-    const Cut cut = whole_cut(p.cut.cg, tokens, r1 - r0);
-    if (int rc = product<T, false>(xm, wm, cut, nullptr, e, p.w.status, s)) return rc;
-    const Matrix pm{p.prob, tokens, r1 - r0, p.ldp};
-    const EpiAccum a{p.acc, tokens, cols, p.ld, r0 > 0};
-    if (int rc = product<T, true>(pm, wm, p.sms, p.parts, a, p.w.status, s)) return rc;
+    if (int rc = soft_piece<T>(p, xm, wm, r0, rows, soft, kLog2e * inv_t, s)) return rc;
   }
-  Finish<T> f{};
-  f.acc = p.acc;
-  f.M = tokens;
-  f.N = cols;
-  f.ld = p.ld;
-  f.lin.y = static_cast<T*>(dx);
-  f.lin.ldy = cols;
-  f.grad = grad;
-  f.grad_step = reduction == kRows;
-  f.count = rows.count;
-  f.mean_rows = reduction == kMean ? rows.rows : nullptr;
-  f.factor = temperature / gain;
-  return run_finish(f, s);
+  float* row_loss = reduction == kRows ? loss : p.row_loss;
+  if (int rc = launch_after(soft_end_kernel, dim3(unsigned(tokens)), 128, 0, s, "soft_end_kernel", rows, soft,
+                            static_cast<const float*>(p.acc), static_cast<const float*>(p.acc_q), p.ld, cols,
+                            temperature, row_loss, unit))
+    return rc;
+  if (reduction == kRows) return ZN_OK;
+  return launch_after(loss_reduce_kernel, dim3(1), 1024, 0, s, "loss_reduce_kernel", static_cast<const float*>(row_loss),
+                      rows, tokens, reduction == kMean, loss);
 }
 
 bool loss_ok(const zn_weight* w, int64_t tokens, int64_t ldx, int top, float temperature, int reduction) {
@@ -1069,56 +1333,61 @@ size_t zn_loss_state_bytes(int64_t tokens, int top) {
   return bytes;
 }
 
-size_t zn_loss_temp_bytes(const zn_weight* w, const void* hidden, int64_t ldh, int64_t tokens) {
-  if (!loss_ok(w, tokens, ldh, 1, 1.0f, 0)) return 0;
+size_t zn_loss_temp_bytes(const zn_weight* w, const void* hidden, int64_t ldh, int64_t tokens, int top, int with_grad) {
+  if (!loss_ok(w, tokens, ldh, top, 1.0f, 0)) return 0;
   Arena ar{nullptr};
   LossPlan p;
-  return plan_loss(w, hidden, ldh, tokens, nullptr, ar, &p) ? 0 : ar.used;
+  LossGradPlan g;
+  const int rc = with_grad ? plan_loss_grad(w, hidden, ldh, tokens, top, nullptr, ar, &g)
+                           : plan_loss(w, hidden, ldh, tokens, nullptr, ar, &p);
+  return rc ? 0 : ar.used;
 }
 
 int zn_loss(const zn_weight* w, const void* hidden, int64_t ldh, int64_t tokens, const int64_t* ids,
             const float* logits, int top, int64_t ignore_index, float temperature, int reduction, float* loss,
-            void* state, int32_t* status, void* temp, size_t temp_bytes, void* stream) {
+            float* unit_grad, void* state, int32_t* status, void* temp, size_t temp_bytes, void* stream) {
   if (!loss_ok(w, tokens, ldh, top, temperature, reduction) || (!logits && top != 1) || !w->blob ||
       (reinterpret_cast<uintptr_t>(w->blob) & 7) || !hidden || !ids || !loss || !state || !status)
     return bad("zn_loss");
   NvtxScope range("zn_loss");
   Arena ar{static_cast<uint8_t*>(temp)};
+  const LossRows rows = loss_state(state, tokens, top, nullptr);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool bf16 = w->dtype == 8;
+  if (unit_grad) {
+    LossGradPlan p;
+    if (int rc = plan_loss_grad(w, hidden, ldh, tokens, top, status, ar, &p)) return rc;
+    if (!temp || temp_bytes < ar.used) return set_error(ZN_ERR_SPACE, "zn_loss: temp buffer too small");
+    return bf16 ? run_loss_grad<__nv_bfloat16>(p, hidden, ldh, tokens, ids, logits, ignore_index, temperature,
+                                               reduction, loss, unit_grad, rows, s)
+                : run_loss_grad<__half>(p, hidden, ldh, tokens, ids, logits, ignore_index, temperature, reduction,
+                                        loss, unit_grad, rows, s);
+  }
   LossPlan p;
   if (int rc = plan_loss(w, hidden, ldh, tokens, status, ar, &p)) return rc;
   if (!temp || temp_bytes < ar.used) return set_error(ZN_ERR_SPACE, "zn_loss: temp buffer too small");
-  const LossRows rows = loss_state(state, tokens, top, nullptr);
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return w->dtype == 8 ? run_loss<__nv_bfloat16>(p, hidden, ldh, tokens, ids, logits, ignore_index, temperature,
-                                                 reduction, loss, rows, s)
-                       : run_loss<__half>(p, hidden, ldh, tokens, ids, logits, ignore_index, temperature, reduction,
-                                          loss, rows, s);
+  return bf16 ? run_loss<__nv_bfloat16>(p, hidden, ldh, tokens, ids, logits, ignore_index, temperature, reduction,
+                                        loss, rows, s)
+              : run_loss<__half>(p, hidden, ldh, tokens, ids, logits, ignore_index, temperature, reduction, loss,
+                                 rows, s);
 }
 
-size_t zn_loss_grad_temp_bytes(const zn_weight* w, const void* hidden, int64_t ldh, int64_t tokens) {
-  if (!loss_ok(w, tokens, ldh, 1, 1.0f, 0)) return 0;
-  Arena ar{nullptr};
-  LossGradPlan p;
-  return plan_loss_grad(w, hidden, ldh, tokens, nullptr, ar, &p) ? 0 : ar.used;
-}
-
-int zn_loss_grad(const zn_weight* w, const void* hidden, int64_t ldh, int64_t tokens, int top, float temperature,
-                 int reduction, const void* state, const float* grad_loss, void* dhidden, int32_t* status, void* temp,
-                 size_t temp_bytes, void* stream) {
-  if (!loss_ok(w, tokens, ldh, top, temperature, reduction) || !w->blob ||
-      (reinterpret_cast<uintptr_t>(w->blob) & 7) || !hidden || !state || !grad_loss || !dhidden || !status)
+int zn_loss_grad(int dtype, int64_t tokens, int64_t cols, int top, int reduction, const void* state,
+                 const float* unit_grad, const float* grad_loss, void* dhidden, void* stream) {
+  if ((dtype != 7 && dtype != 8) || tokens <= 0 || tokens >= (int64_t(1) << 31) || cols <= 0 ||
+      cols >= (int64_t(1) << 31) || top < 1 || top > kMaxTop || reduction < kMean || reduction > kRows || !state ||
+      !unit_grad || !grad_loss || !dhidden)
     return bad("zn_loss_grad");
   NvtxScope range("zn_loss_grad");
-  Arena ar{static_cast<uint8_t*>(temp)};
-  LossGradPlan p;
-  if (int rc = plan_loss_grad(w, hidden, ldh, tokens, status, ar, &p)) return rc;
-  if (!temp || temp_bytes < ar.used) return set_error(ZN_ERR_SPACE, "zn_loss_grad: temp buffer too small");
   const LossRows rows = loss_state(const_cast<void*>(state), tokens, top, nullptr);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return w->dtype == 8 ? run_loss_grad<__nv_bfloat16>(p, hidden, ldh, tokens, temperature, reduction, rows, grad_loss,
-                                                      dhidden, s)
-                       : run_loss_grad<__half>(p, hidden, ldh, tokens, temperature, reduction, rows, grad_loss,
-                                               dhidden, s);
+  const dim3 grid(grid_1d(tokens * cdiv(cols, 256), 8, 148 * 16));
+  const int64_t step = reduction == kRows;
+  const bool mean = reduction == kMean;
+  return dtype == 8 ? launch_after(unit_kernel<__nv_bfloat16>, grid, 256, 0, s, "unit_kernel", unit_grad, tokens, cols,
+                                   rows, grad_loss, step, mean, static_cast<__nv_bfloat16*>(dhidden))
+                    : launch_after(unit_kernel<__half>, grid, 256, 0, s, "unit_kernel", unit_grad, tokens, cols, rows,
+                                   grad_loss, step, mean, static_cast<__half*>(dhidden));
 }
 
 }  // extern "C"

@@ -193,18 +193,17 @@ int zn_linear_grad(const zn_weight *w, const void *dy, int64_t ldy, int64_t toke
  * temperature^2 * KL(q || softmax(s)).  A row without entries, or whose logits are all -inf, does not
  * count; a row with an id >= rows (or a negative target other than ignore_index) has loss and
  * gradient NaN.  reduction: 0 the mean of the rows that count (0 if none does), 1 their sum, 2 one
- * loss per row (0 where it does not count).  `state` (zn_loss_state_bytes) is filled for
- * zn_loss_grad, which computes the logits again: dhidden [tokens, cols], with grad_loss one float
- * (one per row for reduction 2). */
+ * loss per row (0 where it does not count).  unit_grad [tokens, cols] (or NULL) gets the gradient of
+ * each row's own loss, in 32 bits, in the same pass over the weight; `state` (zn_loss_state_bytes)
+ * is filled for zn_loss_grad, which makes dhidden [tokens, cols] of it: grad_loss is one float (one
+ * per row for reduction 2), dtype 7 or 8 as in zn_weight. */
 size_t zn_loss_state_bytes(int64_t tokens, int top);
-size_t zn_loss_temp_bytes(const zn_weight *w, const void *hidden, int64_t ldh, int64_t tokens);
+size_t zn_loss_temp_bytes(const zn_weight *w, const void *hidden, int64_t ldh, int64_t tokens, int top, int with_grad);
 int zn_loss(const zn_weight *w, const void *hidden, int64_t ldh, int64_t tokens, const int64_t *ids,
             const float *logits, int top, int64_t ignore_index, float temperature, int reduction, float *loss,
-            void *state, int32_t *status, void *temp, size_t temp_bytes, void *stream);
-size_t zn_loss_grad_temp_bytes(const zn_weight *w, const void *hidden, int64_t ldh, int64_t tokens);
-int zn_loss_grad(const zn_weight *w, const void *hidden, int64_t ldh, int64_t tokens, int top, float temperature,
-                 int reduction, const void *state, const float *grad_loss, void *dhidden, int32_t *status, void *temp,
-                 size_t temp_bytes, void *stream);
+            float *unit_grad, void *state, int32_t *status, void *temp, size_t temp_bytes, void *stream);
+int zn_loss_grad(int dtype, int64_t tokens, int64_t cols, int top, int reduction, const void *state,
+                 const float *unit_grad, const float *grad_loss, void *dhidden, void *stream);
 
 #ifdef __cplusplus
 }

@@ -106,10 +106,10 @@ def test_abi_refusals_without_a_gpu():
     assert _lib.lib.zn_linear(r, None, 8, 1, None, 0, None, 0, None, None, None, None, 0, None) == _lib.ZN_ERR_INVALID
     assert _lib.lib.zn_linear_temp_bytes(r, None, 7, 1) == 0  # pitch below the row
     assert _lib.lib.zn_linear_grad(r, None, 4, 1, None, None, None, None, None, 0, None) == _lib.ZN_ERR_INVALID
-    assert _lib.lib.zn_loss(r, None, 8, 1, None, None, 1, 0, 1.0, 0, None, None, None, None, 0, None) == _lib.ZN_ERR_INVALID
-    assert _lib.lib.zn_loss_grad(r, None, 8, 1, 1, 1.0, 3, None, None, None, None, None, 0, None) == _lib.ZN_ERR_INVALID
+    assert _lib.lib.zn_loss(r, None, 8, 1, None, None, 1, 0, 1.0, 0, None, None, None, None, None, 0, None) == _lib.ZN_ERR_INVALID
+    assert _lib.lib.zn_loss_grad(8, 1, 8, 1, 3, None, None, None, None, None) == _lib.ZN_ERR_INVALID
     assert _lib.lib.zn_loss_state_bytes(5, 257) == 0 and _lib.lib.zn_loss_state_bytes(5, 256) > 0
     for field, value in (("rows", 0), ("cols", -1), ("dtype", 9), ("chunk_bytes", 12), ("blob_bytes", 10)):
         bad = _lib.Weight(None, 1000, 4, 8, 0, 8)
         setattr(bad, field, value)
-        assert _lib.lib.zn_loss_temp_bytes(ctypes.byref(bad), None, 8, 1) == 0
+        assert _lib.lib.zn_loss_temp_bytes(ctypes.byref(bad), None, 8, 1, 1, 1) == 0

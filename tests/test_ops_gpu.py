@@ -336,6 +336,28 @@ def test_distillation(tokens, vocab, cols, chunk, top, temperature, dtype):
                    ids, q, counts, temperature, reduction, dtype)
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("tokens,vocab,cols,chunk", [(20, 900, 64, 4096), (40, 12000, 256, 1024), (300, 6000, 128, 4096)])
+@pytest.mark.parametrize("std", [3.0, 30.0, 300.0])
+def test_loss_gradient_with_steep_logits(tokens, vocab, cols, chunk, dtype, std):
+    """Logits whose maximum is far above the first columns': the references are raised in some pieces,
+    in others not, and in some rows only."""
+    w, blob = weight(vocab, cols, dtype, chunk=chunk)
+    h = rnd(tokens, cols, dtype=dtype, scale=std / (0.05 * math.sqrt(cols)))
+    h[::3] *= 0.1
+    t = torch.randint(vocab, (tokens,), device=DEV, generator=torch.Generator(device=DEV).manual_seed(3))
+    t[::2] = (h.double() @ w.double().t()).argmax(1)[::2]  # confident rows: a small difference of p and 1
+    t[1] = -100
+    counts = t >= 0
+    check_loss(lambda x: z.blob_cross_entropy(x, blob, t, reduction="none"), h, w, t[:, None], counts[:, None].double(),
+               counts, 1.0, "none", dtype)
+    ids, logits = teacher(tokens, vocab, 9)
+    ids[::2, 0] = t[::2].clamp(min=0)
+    q, counts = distribution(ids, logits, 1.0)
+    check_loss(lambda x: z.blob_distillation(x, blob, logits, ids, reduction="none"), h, w, ids, q, counts, 1.0, "none",
+               dtype)
+
+
 def test_loss_no_row_counts():
     w, blob = weight(500, 64, BF)
     for tokens in (2, 20):
@@ -362,9 +384,10 @@ def test_loss_bad_rows_stay_alone(tokens):
     w, blob = weight(700, 128, BF)
     h = rnd(tokens, 128)
     t = torch.randint(700, (tokens,), device=DEV)
-    clean = z.blob_cross_entropy(h, blob, t, reduction="none")
     hc = h.clone().requires_grad_()
-    dh_clean, = grads(z.blob_cross_entropy(hc, blob, t, reduction="none"), [hc], torch.ones(tokens, device=DEV))
+    clean = z.blob_cross_entropy(hc, blob, t, reduction="none")
+    dh_clean, = grads(clean, [hc], torch.ones(tokens, device=DEV))
+    clean = clean.detach()
     t2, h2 = t.clone(), h.clone()
     t2[0], t2[1], t2[2] = 700, -1, 1 << 40
     h2[3], h2[4] = math.nan, math.inf
@@ -378,7 +401,7 @@ def test_loss_bad_rows_stay_alone(tokens):
     loss = z.blob_distillation(h, blob, torch.zeros(tokens, 3, device=DEV), ids, reduction="none")
     assert bool(loss[0].isnan()) and bool(loss[1:].isfinite().all())
     # ignore_index may be any value, an id of the vocabulary among them.
-    some = z.blob_cross_entropy(h, blob, t, ignore_index=int(t[0]), reduction="none")
+    some = z.blob_cross_entropy(h.requires_grad_(), blob, t, ignore_index=int(t[0]), reduction="none").detach()
     assert some[0] == 0 and torch.equal(some[t != t[0]], clean[t != t[0]])
 
 
