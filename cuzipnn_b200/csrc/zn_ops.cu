@@ -846,9 +846,16 @@ int load_piece(const Weight& w, int64_t r0, int64_t r1, const PitchCopy& other, 
     first = {reinterpret_cast<const uint16_t*>(src), reinterpret_cast<uint16_t*>(w.padded), cols, w.pitch, r1 - r0, cols};
     *out = {w.padded, r1 - r0, cols, w.pitch};
   }
-  if (!w.stored) return weight_decode(w.b, w.temp, c0, cdiv(r1 * cols, w.b.chunk), w.flat, first, second, w.status, s);
-  if (int rc = copy_pitch(first, s)) return rc;
-  return copy_pitch(second, s);
+  const bool tail0 = first.rows * first.cols <= kTailCopy, tail1 = second.rows * second.cols <= kTailCopy;
+  if (!w.stored)
+    if (int rc = weight_decode(w.b, w.temp, c0, cdiv(r1 * cols, w.b.chunk), w.flat, tail0 ? first : PitchCopy{},
+                               tail1 ? second : PitchCopy{}, w.status, s))
+      return rc;
+  if (w.stored || !tail0)
+    if (int rc = copy_pitch(first, s)) return rc;
+  if (w.stored || !tail1)
+    if (int rc = copy_pitch(second, s)) return rc;
+  return ZN_OK;
 }
 
 // A caller's matrix, copied to an aligned pitch when TMA cannot read it as it lies; the copy is left

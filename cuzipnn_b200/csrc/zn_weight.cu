@@ -161,7 +161,7 @@ int weight_decode(const WeightBlob& w, void* temp, int64_t c0, int64_t c1, void*
   DecArgs a = weight_args(w, temp, status, w.direct ? kDirect : kScanned);
   a.out = static_cast<uint8_t*>(out) - c0 * w.chunk * 2;
   const PitchFin fin{{copy0, copy1}};
-  const int64_t work = copy0.rows * copy0.cols + copy1.rows * copy1.cols;
+  const int64_t work = (copy0.rows * copy0.cols + copy1.rows * copy1.cols) / 8;
   return w.bf16 ? launch_weight<true>(a, c0, c1, StoreSink(), fin, work, s)
                 : launch_weight<false>(a, c0, c1, StoreSink(), fin, work, s);
 }

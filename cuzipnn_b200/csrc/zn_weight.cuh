@@ -34,33 +34,51 @@ size_t weight_temp_bytes(const WeightBlob& w);
 inline bool weight_direct(const WeightBlob& w, int64_t pieces) { return pieces == 1 && weight_chunks(w) <= 2048; }
 // First step of a call unless w.direct: the offsets of the blob's units; sets the status word.
 int weight_scan(const WeightBlob& w, void* temp, int32_t* status, cudaStream_t s);
-// A copy of `rows` rows of `cols` 16-bit elements to another pitch (rows = 0: none).
+// A copy of `rows` rows of `cols` 16-bit elements to another pitch, a multiple of 8 (rows = 0: none).
 struct PitchCopy {
   const uint16_t* src;
   uint16_t* dst;
   int64_t lds, ldd, rows, cols;
 };
 #ifdef __CUDACC__
-// Its share of warp `w` of `n`: 256 columns of a row at a time.
+// Its share of warp `w` of `n`: 256 columns of a row at a time, 8 per lane.  A row of the source may
+// start at any element, and does so alike for all its groups of 8: a lane loads the one or two
+// 16-byte blocks that hold its elements (never one without any of them) and shifts them into place;
+// the shift is the warp's.
 __device__ __forceinline__ void pitch_rows(const PitchCopy& p, int64_t w, int64_t n) {
   const int64_t per_row = cdiv(p.cols, 256), total = p.rows * per_row;
   const int lane = threadIdx.x & 31;
   for (int64_t i = w; i < total; i += n) {
-    const int64_t r = i / per_row, c0 = (i - r * per_row) * 256 + lane;
-    uint16_t v[8];
+    const int64_t r = i / per_row, c = (i - r * per_row) * 256 + 8 * lane;
+    if (c >= p.cols) continue;
+    const int held = int(min(int64_t(8), p.cols - c));
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p.src + r * p.lds + c);
+    const int shift = int(at & 15) / 2;  // elements before the first in its block
+    const uint4* block = reinterpret_cast<const uint4*>(at & ~uintptr_t(15));
+    const uint4 v0 = block[0], v1 = held > 8 - shift ? block[1] : make_uint4(0, 0, 0, 0);
+    const uint32_t q[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+    uint32_t o[5];
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (c0 + 32 * k < p.cols) v[k] = p.src[r * p.lds + c0 + 32 * k];
+    for (int k = 0; k < 5; ++k) {
+      const int word = shift >> 1;
+      o[k] = word == 0 ? q[k] : word == 1 ? q[(k + 1) & 7] : word == 2 ? q[(k + 2) & 7] : q[(k + 3) & 7];
+    }
+    if (shift & 1) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (c0 + 32 * k < p.cols) p.dst[r * p.ldd + c0 + 32 * k] = v[k];
+      for (int k = 0; k < 4; ++k) o[k] = __byte_perm(o[k], o[k + 1], 0x5432);
+    }
+    // The pitch covers the last group of 8 (its padding gets whatever the block held).
+    *reinterpret_cast<uint4*>(p.dst + r * p.ldd + c) = make_uint4(o[0], o[1], o[2], o[3]);
   }
 }
 #endif
 
+// Copies up to this size are made by the kernel that checks the chunks, so that odd sizes cost no
+// launches; that kernel has a few CTAs per SM only and moves a larger one at a third of the rate.
+constexpr int64_t kTailCopy = 1 << 20;  // elements
 // Decode chunks [c0, c1) to `out` (the address of chunk c0's first element, 16-byte aligned), then make
-// the two copies (of the decoded rows, and of another operand: in the same kernel as the check of the
-// chunks, so that odd sizes cost no launches).  Sets the status word (w.direct) or adds to it.
+// the two copies (of the decoded rows, and of another operand; each at most kTailCopy elements or
+// empty).  Sets the status word (w.direct) or adds to it.
 int weight_decode(const WeightBlob& w, void* temp, int64_t c0, int64_t c1, void* out, const PitchCopy& copy0,
                   const PitchCopy& copy1, int32_t* status, cudaStream_t s);
 // Chunks that the decoder works on at once on this device (its resident blocks).
