@@ -81,6 +81,34 @@ __device__ __forceinline__ void stage_rows(uint8_t* buf, const uint32_t* w, T* o
   __syncwarp();
 }
 
+// The reverse: the thread's own row of columns n0 .. n0 + 31 (those below N) of rows m0 .. m0 + 31
+// (those below M) as 16 words, loaded by the warp as whole sectors.
+template <typename T>
+__device__ __forceinline__ void unstage_rows(uint8_t* buf, const T* in, int64_t ld, int64_t m0, int64_t M, int64_t n0,
+                                             int64_t N, bool vec, uint32_t* w) {
+  const int lane = threadIdx.x & 31;
+  if (vec) {
+    const int64_t n = n0 + 8 * (lane & 3);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = 8 * i + (lane >> 2);
+      if (m0 + r < M && n < N) *stage_at(buf, r, lane & 3) = *reinterpret_cast<const uint4*>(in + (m0 + r) * ld + n);
+    }
+  } else if (n0 + lane < N) {
+    const int rows = int(min(int64_t(32), M - m0));
+#pragma unroll 8
+    for (int r = 0; r < rows; ++r)
+      reinterpret_cast<T*>(stage_at(buf, r, lane >> 3))[lane & 7] = in[(m0 + r) * ld + n0 + lane];
+  }
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint4 q = *stage_at(buf, lane, i);
+    w[4 * i] = q.x; w[4 * i + 1] = q.y; w[4 * i + 2] = q.z; w[4 * i + 3] = q.w;
+  }
+  __syncwarp();
+}
+
 // y = act(acc + bias) + residual, rounded once to 16 bits, and (where asked for) the slopes.
 template <typename T>
 struct EpiLinear {
@@ -114,7 +142,7 @@ struct EpiLinear {
     __device__ __forceinline__ void cols(const EpiLinear& e, int c, float* v) {
       const int64_t n = n0 + c;
       if (n >= e.N) return;
-      if (e.bias) add(e.bias, n, e, v);
+      if (e.bias) add_bias(e.bias, n, e, v);
       if (e.slope) {
         switch (e.act) {
           case kRelu: run<kRelu, true>(e, n, v); break;
@@ -132,16 +160,23 @@ struct EpiLinear {
           default: break;
         }
       }
-      if (e.res && m < e.M) add(e.res + m * e.ldr, n, e, v);
       uint32_t w[16];
+      if (e.res) {
+        unstage_rows(buf, e.res, e.ldr, m - (threadIdx.x & 31), e.M, n, e.N, e.vec, w);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          v[2 * i] += Num<T>::lo(w[i]);
+          v[2 * i + 1] += Num<T>::hi(w[i]);
+        }
+      }
 #pragma unroll
       for (int i = 0; i < 16; ++i) w[i] = Num<T>::pack(v[2 * i], v[2 * i + 1]);
       stage_rows(buf, w, e.y, e.ldy, m - (threadIdx.x & 31), e.M, n, e.N, e.vec);
     }
     __device__ __forceinline__ void end(const EpiLinear&) {}
 
-    // v += row[n .. n + 31], as far as the columns go.
-    static __device__ __forceinline__ void add(const T* row, int64_t n, const EpiLinear& e, float* v) {
+    // v += row[n .. n + 31], as far as the columns go: the same for all rows, one broadcast load each.
+    static __device__ __forceinline__ void add_bias(const T* row, int64_t n, const EpiLinear& e, float* v) {
       if (e.vec) {
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
