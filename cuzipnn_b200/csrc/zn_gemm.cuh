@@ -254,7 +254,7 @@ struct EpiAccum {
   struct Row {
     int64_t m, n0;
     uint8_t* buf;
-    __device__ __forceinline__ Row(const EpiAccum&, int64_t m_, int64_t n0_, uint8_t* b) : m(m_), n0(n0_), buf(b) {}
+    __device__ __forceinline__ Row(const EpiAccum&, int64_t m_, int64_t n0_, int, uint8_t* b) : m(m_), n0(n0_), buf(b) {}
     __device__ __forceinline__ float4* at(int row, int chunk) const {
       return reinterpret_cast<float4*>(buf + row * 128 + ((chunk ^ (row & 7)) << 4));
     }
@@ -288,7 +288,7 @@ struct EpiAccum {
 };
 
 // Epilogue interface.  Epi::kParts: tiles may be computed in parts (else GemmShape::rest is 0), whose
-// sums another kernel hands to the epilogue.  Epi::Row row(epi, m, n0, buf) at the start of a thread's half row (the
+// sums another kernel hands to the epilogue.  Epi::Row row(epi, m, n0, width, buf) at the start of a thread's half row (the
 // warp holds rows m - lane .. m - lane + 31; m may be past the last row: nothing may be accessed
 // then), row.cols(epi, c, v) for each 32 columns n0 + c .. n0 + c + 31, by whole warps, row.end(epi)
 // after the last.  buf: kWarpBuf bytes of the warp's own shared memory.
@@ -463,12 +463,12 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
       if constexpr (Epi::kParts) {
         if (part >= 0) {
           const EpiAccum e{g.parts + int64_t(part) * (CG * kBM * BN), CG * kBM, BN, BN, false, nullptr};
-          EpiAccum::Row row(e, m, c0, buf);
+          EpiAccum::Row row(e, m, c0, kHalf, buf);
           drain_tile(row, e);
           continue;
         }
       }
-      typename Epi::Row row(epi, int64_t(tm) * CG * kBM + m, int64_t(tn) * BN + c0, buf);
+      typename Epi::Row row(epi, int64_t(tm) * CG * kBM + m, int64_t(tn) * BN + c0, kHalf, buf);
       drain_tile(row, epi);
     }
   }

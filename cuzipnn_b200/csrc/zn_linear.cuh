@@ -81,30 +81,35 @@ __device__ __forceinline__ void stage_rows(uint8_t* buf, const uint32_t* w, T* o
   __syncwarp();
 }
 
-// The reverse: the thread's own row of columns n0 .. n0 + 31 (those below N) of rows m0 .. m0 + 31
-// (those below M) as 16 words, loaded by the warp as whole sectors.
+// The reverse, for the residual: a warp's rows m0 .. m0 + 31 (those below M) of columns n0 .. n0 + 31
+// (those below N), loaded as whole sectors into registers and handed to the threads that own the
+// rows.  The aligned form is split, so that the next columns' loads run during this columns' work.
 template <typename T>
-__device__ __forceinline__ void unstage_rows(uint8_t* buf, const T* in, int64_t ld, int64_t m0, int64_t M, int64_t n0,
-                                             int64_t N, bool vec, uint32_t* w) {
+__device__ __forceinline__ void fetch_rows(const T* in, int64_t ld, int64_t m0, int64_t M, int64_t n0, int64_t N,
+                                           uint4* q) {
   const int lane = threadIdx.x & 31;
-  if (vec) {
-    const int64_t n = n0 + 8 * (lane & 3);
+  const int64_t n = n0 + 8 * (lane & 3);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = 8 * i + (lane >> 2);
-      if (m0 + r < M && n < N) *stage_at(buf, r, lane & 3) = *reinterpret_cast<const uint4*>(in + (m0 + r) * ld + n);
-    }
-  } else if (n0 + lane < N) {
-    const int rows = int(min(int64_t(32), M - m0));
+  for (int i = 0; i < 4; ++i) {
+    const int r = 8 * i + (lane >> 2);
+    if (m0 + r < M && n < N) q[i] = *reinterpret_cast<const uint4*>(in + (m0 + r) * ld + n);
+  }
+}
+__device__ __forceinline__ void hand_rows(uint8_t* buf, const uint4* q) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) *stage_at(buf, 8 * i + (lane >> 2), lane & 3) = q[i];
+  __syncwarp();
+}
+template <typename T>
+__device__ __forceinline__ void fetch_rows_plain(uint8_t* buf, const T* in, int64_t ld, int64_t m0, int64_t M,
+                                                 int64_t n0, int64_t N) {
+  const int lane = threadIdx.x & 31;
+  const int rows = int(min(int64_t(32), M - m0));
+  if (n0 + lane < N) {
 #pragma unroll 8
     for (int r = 0; r < rows; ++r)
       reinterpret_cast<T*>(stage_at(buf, r, lane >> 3))[lane & 7] = in[(m0 + r) * ld + n0 + lane];
-  }
-  __syncwarp();
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint4 q = *stage_at(buf, lane, i);
-    w[4 * i] = q.x; w[4 * i + 1] = q.y; w[4 * i + 2] = q.z; w[4 * i + 3] = q.w;
   }
   __syncwarp();
 }
@@ -123,8 +128,13 @@ struct EpiLinear {
 
   struct Row {
     int64_t m, n0;
+    int width;
     uint8_t* buf;
-    __device__ __forceinline__ Row(const EpiLinear&, int64_t m_, int64_t n0_, uint8_t* b) : m(m_), n0(n0_), buf(b) {}
+    uint4 ahead[4];  // the residual of the next 32 columns
+    __device__ __forceinline__ Row(const EpiLinear& e, int64_t m_, int64_t n0_, int width_, uint8_t* b)
+        : m(m_), n0(n0_), width(width_), buf(b) {
+      if (e.res && e.vec) fetch_rows(e.res, e.ldr, m - (threadIdx.x & 31), e.M, n0, e.N, ahead);
+    }
 
     template <int ACT, bool SLOPE>
     __device__ __forceinline__ void run(const EpiLinear& e, int64_t n, float* v) {
@@ -162,7 +172,19 @@ struct EpiLinear {
       }
       uint32_t w[16];
       if (e.res) {
-        unstage_rows(buf, e.res, e.ldr, m - (threadIdx.x & 31), e.M, n, e.N, e.vec, w);
+        const int64_t m0 = m - (threadIdx.x & 31);
+        if (e.vec) {
+          hand_rows(buf, ahead);
+          if (c + 32 < width) fetch_rows(e.res, e.ldr, m0, e.M, n + 32, e.N, ahead);
+        } else {
+          fetch_rows_plain(buf, e.res, e.ldr, m0, e.M, n, e.N);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint4 q = *stage_at(buf, threadIdx.x & 31, i);
+          w[4 * i] = q.x; w[4 * i + 1] = q.y; w[4 * i + 2] = q.z; w[4 * i + 3] = q.w;
+        }
+        __syncwarp();
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           v[2 * i] += Num<T>::lo(w[i]);

@@ -126,7 +126,7 @@ struct EpiStats {
     const float* q;
     int at, count;
     int64_t next;  // column (of the piece) of the next id
-    __device__ __forceinline__ Row(const EpiStats& e, int64_t m_, int64_t n0_, uint8_t*) : m(m_), n0(n0_) {
+    __device__ __forceinline__ Row(const EpiStats& e, int64_t m_, int64_t n0_, int, uint8_t*) : m(m_), n0(n0_) {
       st = {-INFINITY, 0.0f, 0.0f};
       at = count = 0;
       next = INT64_MAX;
@@ -208,7 +208,7 @@ struct EpiSoft {
     float ref, before, sum, out;
     int at, count;
     int64_t next;  // column (of the piece) of the next id
-    __device__ __forceinline__ Row(const EpiSoft& e, int64_t m_, int64_t n0_, uint8_t* b) : m(m_), n0(n0_), buf(b) {
+    __device__ __forceinline__ Row(const EpiSoft& e, int64_t m_, int64_t n0_, int, uint8_t* b) : m(m_), n0(n0_), buf(b) {
       at = count = 0;
       next = INT64_MAX;
       ref = before = sum = 0.0f;
