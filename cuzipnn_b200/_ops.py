@@ -103,7 +103,7 @@ class _Weight:
             raise ValueError(f"{name} has too many rows")
         self.device, self.dtype = x.device, dtype
         self.chunk_bytes = 0 if stored else chunk_bytes
-        self.blob = blob.detach()
+        self.blob = blob
 
     def place(self, name: str) -> None:
         if self.device.type != "cuda":
@@ -144,8 +144,7 @@ def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
-def _linear_forward(w: _Weight, x, bias, act: int, residual, want_slope: bool, status):
-    shape = (*x.shape[:-1], w.rows)
+def _linear_forward(w: _Weight, x, shape, bias, act: int, residual, want_slope: bool, status):
     y = torch.empty(shape, dtype=w.dtype, device=w.device)
     slope = torch.empty(shape, dtype=torch.int16, device=w.device) if want_slope else None
     x2, ldx = _rows(x, w.cols)
@@ -162,10 +161,10 @@ def _linear_forward(w: _Weight, x, bias, act: int, residual, want_slope: bool, s
 
 class _Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, blob, bias, residual, w, act):
+    def forward(ctx, x, blob, bias, residual, w, shape, act):
         status = torch.empty(1, dtype=torch.int32, device=w.device)
         want = act != 0 and (ctx.needs_input_grad[0] or ctx.needs_input_grad[2])
-        y, slope = _linear_forward(w, x, bias, act, residual, want, status)
+        y, slope = _linear_forward(w, x, shape, bias, act, residual, want, status)
         _set_status(w.device, status)
         ctx.w, ctx.status, ctx.x_shape = w, status, x.shape
         ctx.save_for_backward(blob, slope)  # the blob: an in-place change before backward raises
@@ -180,14 +179,14 @@ class _Linear(torch.autograd.Function):
         dx = torch.empty(ctx.x_shape, dtype=w.dtype, device=w.device) if need_x else None
         db = torch.empty(w.rows, dtype=w.dtype, device=w.device) if need_b else None
         if not dy.numel():
-            return dx, None, db.zero_() if need_b else None, dy if need_r else None, None, None
+            return dx, None, db.zero_() if need_b else None, dy if need_r else None, None, None, None
         if need_x or need_b:
             with _on(w.device):
                 g, ldy = _rows(dy, w.rows)
                 w.call("zn_linear_grad",
                        (g.data_ptr(), ldy, g.shape[0], int(slope is not None), int(need_x), int(need_b)),
                        (g.data_ptr(), ldy, g.shape[0], _ptr(slope), _ptr(dx), _ptr(db)), ctx.status)
-        return dx, None, db, dy if need_r else None, None, None
+        return dx, None, db, dy if need_r else None, None, None, None
 
 
 def blob_linear(
@@ -211,13 +210,14 @@ def blob_linear(
     if activation not in _ACTIVATIONS:
         raise ValueError(f"activation must be one of {sorted(map(str, _ACTIVATIONS))}, not {activation!r}")
     w = _Weight(blob, x, "x")
-    for name, t, shape in (("bias", bias, (w.rows,)), ("residual", residual, (*x.shape[:-1], w.rows))):
+    shape = (*x.shape[:-1], w.rows)
+    for name, t, expected in (("bias", bias, (w.rows,)), ("residual", residual, shape)):
         if t is None:
             continue
         if t.dtype != w.dtype:
             raise TypeError(f"{name} has dtype {t.dtype}, the blob holds {w.dtype}")
-        if tuple(t.shape) != shape:
-            raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {shape}")
+        if t.shape != expected:
+            raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {expected}")
         if t.device != w.device:
             raise ValueError(f"{name} is on {t.device}, x on {w.device}")
     w.place("x")
@@ -225,9 +225,9 @@ def blob_linear(
     with _on(w.device):
         if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)
                                         or (residual is not None and residual.requires_grad)):
-            return _Linear.apply(x, blob, bias, residual, w, act)
+            return _Linear.apply(x, blob, bias, residual, w, shape, act)
         status = torch.empty(1, dtype=torch.int32, device=w.device)
-        y, _ = _linear_forward(w, x, bias, act, residual, False, status)
+        y, _ = _linear_forward(w, x, shape, bias, act, residual, False, status)
         _set_status(w.device, status)
         return y
 
