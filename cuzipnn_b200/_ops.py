@@ -2,7 +2,7 @@
 
 A model whose weights are kept compressed in GPU memory is used through these calls instead of
 decompress_tensor followed by a product: the weight is decoded a piece of rows at a time into a
-bounded scratch buffer (or, for a few tokens, only in the decoder's registers) and is frozen, so
+bounded scratch buffer (or, for a single token, only in the decoder's registers) and is frozen, so
 gradients go to the other operands.  The reference has no counterpart.
 
 Blobs must be on the GPU of the other operands.  A blob that compress_tensor(..., readback_to_cpu=

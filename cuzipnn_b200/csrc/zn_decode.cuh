@@ -397,7 +397,7 @@ struct StoreSink {
 };
 
 // DotSink: the elements are rows of a weight W[rows, cols] and are multiplied with the matching
-// elements of up to MT vectors x as they leave the decoder; W itself is never written.
+// elements of up to kDotRows vectors x as they leave the decoder; W itself is never written.
 //
 // A lane's 16 elements of a round lie in one row (cols and the chunk size are multiples of 16), and
 // a row is at least one round (128 elements) long, so a segment (8 lanes, one sub-chunk) crosses at
@@ -415,11 +415,10 @@ struct StoreSink {
 // which the CTA adds in order at the end; rows that span chunks leave their parts in `part` with the
 // same rule per chunk.  No atomics: the result does not depend on the order in which chunks are
 // decoded.
-template <typename T, int MT>
+template <typename T>
 struct DotSink {
   static constexpr bool kDot = true;
-  static constexpr int kRows = MT;
-  static constexpr bool kAhead = MT == 1;  // x is loaded before the round is decoded (8 registers)
+  static constexpr int kRows = kDotRows;
   using Elem = T;
   const T* x;
   int64_t ldx, rows;
@@ -435,7 +434,7 @@ struct DotState {
   int row;         // the segment's current row
   bool first;      // no row end met in this sub-chunk yet
   bool mid;        // the sub-chunk starts inside a row
-  uint4 x[2];      // kAhead: the round's elements of x
+  uint4 x[MT][2];  // the round's elements of x, loaded before it is decoded
 };
 
 // Column of the next round's elements (lanes without elements get a valid one too).
@@ -444,11 +443,16 @@ __device__ __forceinline__ int dot_col(const Sink& k, const DotState<Sink::kRows
   const int col = st.col + kRound + l * kSteps;
   return col >= k.cols ? col - k.cols : col;
 }
+// Loads the next round's elements of x (those of row 0 for rows past the last).
 template <class Sink>
-__device__ __forceinline__ void dot_load(const Sink& k, int m, int col, uint4* x) {
-  const uint4* xp = reinterpret_cast<const uint4*>(k.x + m * k.ldx + col);
-  x[0] = __ldg(xp);
-  x[1] = __ldg(xp + 1);
+__device__ __forceinline__ void dot_load(const Sink& k, DotState<Sink::kRows>& st, int l) {
+  const int col = dot_col(k, st, l);
+#pragma unroll
+  for (int m = 0; m < Sink::kRows; ++m) {
+    const uint4* xp = reinterpret_cast<const uint4*>(k.x + (m < k.tokens ? m * k.ldx : 0) + col);
+    st.x[m][0] = __ldg(xp);
+    st.x[m][1] = __ldg(xp + 1);
+  }
 }
 
 // One step of the products: rows 0-7 of A from a0, a2, rows 8-15 zero.
@@ -466,21 +470,14 @@ __device__ __forceinline__ void dot_mma(float* c, uint32_t a0, uint32_t a2, uint
 }
 // Lanes with `use` add their products, the others nothing (both factors are zeroed: 0 * inf is NaN).
 template <class Sink, bool MASKED>
-__device__ __forceinline__ void dot_products(const Sink& k, DotState<Sink::kRows>& st, const uint32_t* e, int col,
-                                             bool use) {
+__device__ __forceinline__ void dot_products(DotState<Sink::kRows>& st, const uint32_t* e, bool use) {
   uint32_t w[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) w[i] = !MASKED || use ? e[i] : 0u;
 #pragma unroll
   for (int m = 0; m < Sink::kRows; ++m) {
-    uint4 q[2];
-    if constexpr (Sink::kAhead) {
-      q[0] = st.x[0];
-      q[1] = st.x[1];
-    } else {
-      dot_load(k, m < k.tokens ? m : 0, col, q);
-    }
-    uint32_t x[8] = {q[0].x, q[0].y, q[0].z, q[0].w, q[1].x, q[1].y, q[1].z, q[1].w};
+    const uint4 a = st.x[m][0], b = st.x[m][1];
+    uint32_t x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       if (MASKED && !use) x[i] = 0u;
@@ -508,15 +505,14 @@ template <class Sink, bool ALL>
 __device__ __forceinline__ void dot_round(const Sink& k, DotState<Sink::kRows>& st, const uint32_t* e, bool active,
                                           int l, int seg, float* slot0) {
   constexpr int MT = Sink::kRows;
-  const int col = dot_col(k, st, l);
   st.col += kRound;
   const bool wrapped = active && st.col + l * kSteps >= k.cols;  // the lane's elements lie in the next row
   const uint32_t over = __ballot_sync(0xFFFFFFFFu, wrapped);
   if (!over) {
-    dot_products<Sink, !ALL>(k, st, e, col, active);
+    dot_products<Sink, !ALL>(st, e, active);
     return;
   }
-  dot_products<Sink, true>(k, st, e, col, active && !wrapped);
+  dot_products<Sink, true>(st, e, active && !wrapped);
   float v[MT];
   segment_sum<MT>(st, v);
   if ((over >> (8 * seg)) & 0xFF) {
@@ -534,7 +530,7 @@ __device__ __forceinline__ void dot_round(const Sink& k, DotState<Sink::kRows>& 
     ++st.row;
     st.col -= k.cols;  // below 0 when the row ended inside the round
   }
-  dot_products<Sink, true>(k, st, e, col, wrapped);
+  dot_products<Sink, true>(st, e, wrapped);
 }
 
 // The rows of chunk j (elements [g0, g1)) that no single sub-chunk completed: the sums of their
@@ -877,8 +873,7 @@ __device__ __forceinline__ void decode_chunk(const DecArgs& a, int64_t j, bool o
               if (cb.nload) cb.r0 = block(cb.fill / 8);
             }
           }
-          if constexpr (Sink::kDot)
-            if constexpr (Sink::kAhead) dot_load(sink, 0, dot_col(sink, dot, l), dot.x);
+          if constexpr (Sink::kDot) dot_load(sink, dot, l);
           uint32_t p[kChains][K][4];
 #pragma unroll
           for (int c = 0; c < kChains; ++c)
@@ -979,8 +974,7 @@ __device__ __forceinline__ void decode_chunk(const DecArgs& a, int64_t j, bool o
 #pragma unroll
           for (int i = 0; i < 4; ++i) p[c][b][i] = pn[c][b][i];
       if (r + 1 < rounds) load_raw_round<K, kChains>(src, coded, base, len, r + 1, l, pn);
-      if constexpr (Sink::kDot)
-        if constexpr (Sink::kAhead) dot_load(sink, 0, dot_col(sink, dot, l), dot.x);
+      if constexpr (Sink::kDot) dot_load(sink, dot, l);
       const bool full = nact[0] == kSteps && nact[kChains - 1] == kSteps;
 #pragma unroll
       for (int q = 0; q < KC; ++q) {

@@ -8,16 +8,13 @@ namespace {
 
 // ---- a weight's chunks (zn_weight.cuh) -------------------------------------------------------
 
-// CTAs per SM that the registers have to allow.
-template <class Sink>
-constexpr int weight_blocks() {
-  if constexpr (Sink::kDot) return Sink::kRows <= 1 ? 5 : 4;
-  else return 5;
-}
+// CTAs per SM that the registers have to allow.  With 6 (80 registers, and less shared memory for L1's
+// share of the streams) a single wave of chunks took 5 to 40 % longer.
+constexpr int kWeightBlocks = 5;
 
 // Chunks [c0, c0 + gridDim.x) of one weight.
 template <bool REORDER, class Sink>
-__global__ void __launch_bounds__(kDecThreads, weight_blocks<Sink>()) weight_kernel(const __grid_constant__ DecArgs a, int64_t c0,
+__global__ void __launch_bounds__(kDecThreads, kWeightBlocks) weight_kernel(const __grid_constant__ DecArgs a, int64_t c0,
                                                              const __grid_constant__ Sink sink, uint32_t* counter) {
   pdl_wait();
   pdl_trigger();
@@ -140,14 +137,8 @@ int launch_weight(const DecArgs& a, int64_t c0, int64_t c1, const Sink& sink, co
 template <typename T, bool REORDER, class Fin>
 int launch_dot(const DecArgs& a, const WeightBlob& w, const void* x, int64_t ldx, int tokens, float* z, float* part,
                const Fin& fin, int64_t work, cudaStream_t s) {
-  auto go = [&](auto mt) {
-    constexpr int MT = decltype(mt)::value;
-    DotSink<T, MT> k{static_cast<const T*>(x), ldx, w.rows, int(w.cols), tokens, z, part};
-    return launch_weight<REORDER>(a, 0, a.nch, k, fin, work, s);
-  };
-  if (tokens == 1) return go(std::integral_constant<int, 1>());
-  if (tokens == 2) return go(std::integral_constant<int, 2>());
-  return go(std::integral_constant<int, kDotRows>());
+  const DotSink<T> k{static_cast<const T*>(x), ldx, w.rows, int(w.cols), tokens, z, part};
+  return launch_weight<REORDER>(a, 0, a.nch, k, fin, work, s);
 }
 
 }  // namespace
@@ -170,7 +161,7 @@ int weight_wave(const WeightBlob& w, int64_t* chunks) {
   // The register bound of weight_kernel; a query of the occupancy costs a microsecond of every call.
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
-  *chunks = int64_t(sms) * weight_blocks<StoreSink>();
+  *chunks = int64_t(sms) * kWeightBlocks;
   return ZN_OK;
 }
 

@@ -16,10 +16,11 @@ struct WeightBlob {
   bool direct;    // every chunk finds its units itself, without weight_scan (weight_direct)
 };
 
-// Rows of one product inside the decoder, and the shape rule of that path (see DotSink).  Each row of x
-// adds its loads to a decoder that is bound by the same pipe: over 152064 x 3584 (128 Ki chunks) 682,
-// 822 and 974 us for 1, 2 and 4 rows, against 1080 us for decoding and a product of any number up to 128.
-constexpr int kDotRows = 4;
+// Rows of one product inside the decoder, and the shape rule of that path (see DotSink).  Measured over
+// 152064 x 3584 (128 Ki chunks), in the decoder with 1, 2 and 4 rows 689, 1016 and 1141 us (a second
+// row's registers cost a fifth of the decoder's occupancy), against 1000 us for decoding and a product
+// of any number up to 128; over 3584 x 3584 (16 Ki) 51, 52 and 57 us against 54.
+constexpr int kDotRows = 1;
 inline bool dot_shape(int64_t tokens, int64_t cols, int64_t chunk) {
   return tokens >= 1 && tokens <= kDotRows && cols % 16 == 0 && cols >= kRound && cols < (int64_t(1) << 30) &&
          chunk % 16 == 0;
