@@ -93,6 +93,7 @@ SIZES = [
     (129, 257, 63, 1024), (300, 700, 1016, 32768), (513, 1111, 333, 32768), (17, 5, 30000, 131072), (1000, 3, 8, 1024),
     (2100, 2503, 136, 32768),  # pairs of CTAs, ragged on both sides
     (2100, 2503, 4104, 65536),  # and the last tiles in parts of the contraction
+    (20, 16000, 256, 1024),  # in pieces
 ]
 
 
@@ -149,7 +150,8 @@ def grads(y, leaves, g):
 
 @pytest.mark.parametrize("act", list(ACTS))
 @pytest.mark.parametrize("tokens,rows,cols,chunk", [(1, 64, 128, 1024), (5, 333, 75, 4096), (200, 130, 264, 8192),
-                                                    (777, 1000, 520, 32768), (64, 5000, 256, 1024), (2100, 72, 2504, 32768), (2100, 4104, 2104, 65536)])
+                                                    (777, 1000, 520, 32768), (64, 5000, 256, 1024), (2100, 72, 2504, 32768), (2100, 4104, 2104, 65536),
+                                                    (64, 16000, 256, 1024)])
 @pytest.mark.parametrize("dtype", [BF, HF])
 def test_linear_gradients(act, tokens, rows, cols, chunk, dtype):
     w, blob = weight(rows, cols, dtype, chunk=chunk)
@@ -279,7 +281,8 @@ LOSS_SIZES = [  # tokens, vocabulary, cols, chunk
     (1, 1, 16, 1024), (1, 300, 128, 1024), (3, 5000, 144, 4096), (8, 2049, 256, 1024), (9, 513, 64, 4096),
     (100, 1001, 75, 4096), (130, 4000, 96, 8192), (257, 777, 512, 32768), (40, 12000, 256, 1024), (333, 7000, 40, 1024),
     (2100, 2503, 2104, 65536),  # every product by pairs of CTAs
-    (2100, 8000, 2104, 8192),  # in pieces, with tiles in parts
+    (2100, 8000, 2104, 2048),  # in pieces, with tiles in parts
+    (50, 40000, 256, 1024),
 ]
 
 
@@ -337,7 +340,7 @@ def test_distillation(tokens, vocab, cols, chunk, top, temperature, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, HF])
-@pytest.mark.parametrize("tokens,vocab,cols,chunk", [(20, 900, 64, 4096), (40, 12000, 256, 1024), (300, 6000, 128, 4096)])
+@pytest.mark.parametrize("tokens,vocab,cols,chunk", [(20, 900, 64, 4096), (40, 40000, 256, 1024), (300, 6000, 128, 4096)])
 @pytest.mark.parametrize("std", [3.0, 30.0, 300.0])
 def test_loss_gradient_with_steep_logits(tokens, vocab, cols, chunk, dtype, std):
     """Logits whose maximum is far above the first columns': the references are raised in some pieces,
