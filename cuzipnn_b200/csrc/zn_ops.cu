@@ -18,7 +18,7 @@
 // and values:  softmax(s) W = (sum_v exp(s_v - r) W_v) / (sum_v exp(s_v - r)) for any reference r of
 // the row.  Each piece is decoded once and multiplied twice (4 tokens rows cols operations in all,
 // against 6 and two decodings for computing the logits again in a backward pass).  r is the maximum
-// over the first kSample rows of W; the 16-bit P then holds exp(s - r) up to a bound (2^100 for
+// over the first kSample rows of W; the 16-bit P then holds exp(s - r) up to a bound (2^60 for
 // bf16, 2^15 for fp16).  Where a group of 32 logits passes the bound, its P is zero, the row's r is
 // raised to its maximum, what was summed is scaled down, and the piece is multiplied again with
 // the groups that were left out alone (kernels that end at once when there are none).
@@ -167,7 +167,7 @@ struct EpiStats {
       }
     }
     __device__ __forceinline__ void end(const EpiStats& e) {
-      if (m >= e.M) return;
+      if (m >= e.M || n0 >= e.N) return;  // (the last tile's second half may hold no column)
       float* p = e.part + (e.tile0 + n0 / e.tile_cols) * 3 * e.M + m;
       p[0] = st.mx;
       p[e.M] = st.sum;
@@ -192,7 +192,7 @@ struct SoftRows {
 template <typename T, bool AGAIN>
 struct EpiSoft {
   static constexpr bool kParts = false;
-  static constexpr float kBound = Num<T>::kCode == 1 ? 100.0f : 15.0f;
+  static constexpr float kBound = Num<T>::kCode == 1 ? 60.0f : 15.0f;
   LossRows rows;
   SoftRows soft;
   T* p;

@@ -666,6 +666,61 @@ def test_offsets_past_32_bits():
     assert float((dh.double() - ref).norm()) <= 4 * u_of(BF) * float(ref.norm())
 
 
+@pytest.mark.parametrize("rows", [1, 60, 64, 65, 100, 130, 321])
+@pytest.mark.parametrize("tokens,cols", [(1, 128), (2, 64), (20, 75), (130, 144), (600, 200)])
+def test_calls_stay_inside_their_buffers(tokens, rows, cols):
+    """Every entry point with exactly the scratch, state and output sizes it asks for, each followed by a
+    pattern that must stay."""
+    import ctypes
+
+    from cuzipnn_b200 import _lib, _ops
+
+    lib, guard, fill = _lib.lib, 1 << 16, 0xA5
+    w, blob = weight(rows, cols, BF, chunk=1024)
+    x, g = rnd(tokens, cols), rnd(tokens, rows)
+    weight_desc = _ops._Weight(blob, x, "x")
+    weight_desc.place("x")
+    d = ctypes.byref(weight_desc.desc)
+    stream = torch.cuda.current_stream().cuda_stream
+    buffers = []
+
+    def buf(nbytes):
+        b = torch.full((nbytes + guard,), fill, dtype=torch.uint8, device=DEV)
+        buffers.append((b, nbytes))
+        return b.data_ptr()
+
+    status = buf(4)
+    ptr, ldx = x.data_ptr(), cols if tokens > 1 else (cols + 7) // 8 * 8
+    ldg = rows if tokens > 1 else (rows + 7) // 8 * 8
+    n = lib.zn_linear_temp_bytes(d, ptr, ldx, tokens)
+    y, slope = buf(tokens * rows * 2), buf(tokens * rows * 2)
+    assert lib.zn_linear(d, ptr, ldx, tokens, None, 4, None, 0, y, slope, status, buf(n), n, stream) == 0
+    n = lib.zn_linear_grad_temp_bytes(d, g.data_ptr(), ldg, tokens, 1, 1, 1)
+    assert lib.zn_linear_grad(d, g.data_ptr(), ldg, tokens, slope, buf(tokens * cols * 2), buf(rows * 2), status,
+                              buf(n), n, stream) == 0
+    for top in (1, 3):
+        ids = torch.randint(rows, (tokens, top), device=DEV)
+        logits = None if top == 1 else torch.zeros(tokens, top, device=DEV)
+        grad = torch.ones(tokens, device=DEV)
+        for with_grad in (0, 1):
+            state = buf(lib.zn_loss_state_bytes(tokens, top))
+            n = lib.zn_loss_temp_bytes(d, ptr, ldx, tokens, top, with_grad)
+            unit = buf(tokens * cols * 4) if with_grad else None
+            for reduction in (0, 2):
+                loss = buf(4 * (tokens if reduction == 2 else 1))
+                assert lib.zn_loss(d, ptr, ldx, tokens, ids.data_ptr(), None if logits is None else logits.data_ptr(), top,
+                                   -100, 1.0, reduction, loss, unit, state, status, buf(n), n, stream) == 0
+            if with_grad:
+                assert lib.zn_loss_grad(8, tokens, cols, top, 2, state, unit, grad.data_ptr(), buf(tokens * cols * 2),
+                                        stream) == 0
+            too_small = lib.zn_loss(d, ptr, ldx, tokens, ids.data_ptr(), None if logits is None else logits.data_ptr(), top,
+                                    -100, 1.0, 0, loss, unit, state, status, buf(n), n - 1, stream)
+            assert too_small == _lib.ZN_ERR_SPACE
+    torch.cuda.synchronize()
+    for b, nbytes in buffers:
+        assert bool((b[nbytes:] == fill).all()), nbytes
+
+
 @pytest.mark.parametrize("tokens", [1, 30])
 def test_malformed_blob_is_reported(tokens):
     """A blob whose payload or tables were damaged sets the status, is read inside its bounds only, and
