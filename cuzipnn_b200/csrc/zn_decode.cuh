@@ -1050,6 +1050,10 @@ __device__ __forceinline__ void decode_chunk(const DecArgs& a, int64_t j, bool o
   const bool any_err = __syncthreads_or(err);
   if constexpr (Sink::kDot) dot_finish_chunk(sink, j, j * a.C, j * a.C + m, g.sc, slots, any_err);
   if constexpr (WEIGHT) {
+    // A broken stream shows at its end only: what was stored is replaced by zeros.
+    if constexpr (!Sink::kDot)
+      if (any_err)
+        for (int64_t i = tid; i < m * K; i += kDecThreads) outc[i] = 0;
     if (tid == 0) a.overflow[j] = uint8_t((overflow_pass ? kChunkOver : 0) | flags | (any_err ? kErrStream : 0));
     return;
   }

@@ -1,6 +1,6 @@
 // A compressed weight as the operand of a product: a rows x cols matrix of 16-bit floats held as a
 // blob (the non-stored layout), decoded a range of chunks at a time into a caller's buffer, or
-// multiplied with a few vectors inside the decoder.  Implemented in zn_decode.cu.
+// multiplied with a few vectors inside the decoder.  Implemented in zn_weight.cu (weight_scan in zn_decode.cu).
 #pragma once
 
 #include "zn_common.cuh"

@@ -748,3 +748,27 @@ def test_malformed_blob_is_reported(tokens):
             y = z.blob_linear(x, cut)
             assert z.last_decode_status() != 0 and bool(y.isfinite().all())
     assert z.blob_linear(x, blob).equal(good) and z.last_decode_status() == 0
+
+
+@pytest.mark.parametrize("tokens", [1, 30])
+@pytest.mark.parametrize("chunk", [1024, 4096])
+def test_broken_stream_counts_as_zeros(tokens, chunk):
+    """A stream that does not end where it should sets the status; its chunk's elements count as zeros,
+    both in the decoder's own product and in a decoded piece."""
+    w, blob = weight(64, 256, BF, chunk=chunk)
+    nch, rows = 64 * 256 // chunk, chunk // 256
+    x = rnd(tokens, 256)
+    good = z.blob_linear(x, blob)
+    sizes = blob[40 : 40 + 4 * 2 * nch].cpu().view(torch.int32).tolist()
+    n_comp = int(blob[12:16].cpu().view(torch.int32))
+    data = (40 + 4 * (2 * nch + n_comp) + 7) // 8 * 8
+    assert sizes[nch + 1] < chunk  # coded
+    end = data + sum((s + 7) // 8 * 8 for s in sizes[: nch + 1]) + sizes[nch + 1]
+    bad = blob.clone()
+    bad[end - 40 : end] ^= 0x5A
+    bad = z.upload_blob(bad)
+    y = z.blob_linear(x, bad)
+    assert z.last_decode_status() != 0
+    keep = torch.ones(64, dtype=torch.bool, device=DEV)
+    keep[rows : 2 * rows] = False
+    assert torch.equal(y[:, keep], good[:, keep]) and bool((y[:, ~keep] == 0).all())
