@@ -139,8 +139,10 @@ def _remember(blob: torch.Tensor, dtype: torch.dtype, shape: tuple[int, ...], fl
     """Keep the header fields of a GPU blob made here on the returned tensor object, with the
     blob's version counter, address and size: decompressing the unchanged blob then needs no host
     read of its header (a synchronization that would drain the stream).  Any in-place write to
-    the blob or to a view of its storage bumps the shared version counter and voids the record."""
-    blob._zn_header = (blob._version, blob.data_ptr(), blob.numel(), dtype, shape, flags, chunk_bytes, n)
+    the blob or to a view of its storage bumps the shared version counter and voids the record.
+    A tensor made in inference mode has no such counter and gets no record."""
+    if not blob.is_inference():
+        blob._zn_header = (blob._version, blob.data_ptr(), blob.numel(), dtype, shape, flags, chunk_bytes, n)
     return blob
 
 
@@ -157,6 +159,8 @@ def _trim_and_remember(out: torch.Tensor, views, sizes: list[int], offs: list[in
     asked for them."""
     for v, size in zip(views, sizes):
         v.resize_(size)
+    if out.is_inference():
+        return
     ver, base = out._version, out.data_ptr()
     for v, o, size, f in zip(views, offs, sizes, fields):
         v._zn_header = (ver, base + o, size) + f

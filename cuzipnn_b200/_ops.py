@@ -43,7 +43,8 @@ def upload_blob(blob: torch.Tensor, *, compute_device: torch.device | str | None
     if blob.device == device and _known_header(blob) is not None:
         return blob
     dtype, shape, flags, chunk_bytes, _, n = _read_header(blob)
-    with _on(device):
+    # A tensor of inference mode has no version counter, which the record needs.
+    with _on(device), torch.inference_mode(False):
         if blob.is_cuda:
             out = blob.detach().to(device, non_blocking=True).clone(memory_format=torch.contiguous_format)
         else:

@@ -772,3 +772,38 @@ def test_broken_stream_counts_as_zeros(tokens, chunk):
     keep = torch.ones(64, dtype=torch.bool, device=DEV)
     keep[rows : 2 * rows] = False
     assert torch.equal(y[:, keep], good[:, keep]) and bool((y[:, ~keep] == 0).all())
+
+
+def test_inference_mode():
+    """Blobs are made, uploaded and used in inference mode; what upload_blob returns carries its header
+    (it can be captured) and stays usable outside, in training too."""
+    w, blob = weight(512, 256, BF)
+    x, x1 = rnd(30, 256), rnd(1, 256)
+    y, y1 = z.blob_linear(x, blob), z.blob_linear(x1, blob)
+    t = torch.arange(30, device=DEV)
+    loss = z.blob_cross_entropy(x, blob, t)
+    with torch.inference_mode():
+        host = z.compress_tensor(w)
+        made = z.compress_tensor(w, readback_to_cpu=False)
+        many = z.compress_tensors([w, w], readback_to_cpu=False)
+        for b in (made, *many, z.upload_blob(host, compute_device=DEV), z.upload_blob(made), blob):
+            assert torch.equal(z.decompress_tensor(b), w)
+            assert torch.equal(z.blob_linear(x, b), y) and torch.equal(z.blob_linear(x1, b), y1)
+            assert torch.equal(z.blob_cross_entropy(x, b, t), loss)
+        for b in z.decompress_tensors(list(many)):
+            assert torch.equal(b, w)
+        up = z.upload_blob(host, compute_device=DEV)
+        assert z.upload_blob(up) is up
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            yg = z.blob_linear(x, up)
+        g.replay()
+        assert torch.equal(yg, y)
+    xg = x.clone().requires_grad_()
+    xe = x.clone().requires_grad_()
+    z.blob_linear(xg, up).sum().backward()
+    z.blob_linear(xe, blob).sum().backward()
+    assert torch.equal(xg.grad, xe.grad)
+    z.blob_cross_entropy(xg, made, t).backward()  # the head is not kept for the backward pass
+    with pytest.raises(RuntimeError, match="[Ii]nference"):
+        z.blob_linear(xg, made)
