@@ -226,10 +226,13 @@ struct DotValue {
   const float* part;
   int64_t rows, cols, chunk;
   __device__ __forceinline__ float get(int64_t t, int64_t r) const {
-    const int64_t c0 = r * cols / chunk, c1 = ((r + 1) * cols - 1) / chunk;
-    if (c0 == c1) return z[t * rows + r];
+    // The chunk of the row's first element, and how many more the row reaches into (32 bits: a chunk has
+    // 2^24 elements at most, dot_shape's rows fewer than 2^30).
+    const int64_t c0 = r * cols / chunk;
+    const uint32_t more = (uint32_t(r * cols - c0 * chunk) + uint32_t(cols) - 1) / uint32_t(chunk);
+    if (more == 0) return z[t * rows + r];
     float v = part[(2 * c0 + 1) * kDotRows + t];
-    for (int64_t c = c0 + 1; c <= c1; ++c) v += part[2 * c * kDotRows + t];
+    for (int64_t c = c0 + 1; c <= c0 + more; ++c) v += part[2 * c * kDotRows + t];
     return v;
   }
 };

@@ -495,7 +495,7 @@ __global__ void __launch_bounds__(128) loss_prep_kernel(const int64_t* ids, cons
 }
 
 // Statistics of the logits of weight_dot: a block per (column tile of kStatCols, token).
-constexpr int kStatCols = 2048;
+constexpr int kStatCols = 512;
 __global__ void __launch_bounds__(256) dot_stats_kernel(DotValue v, LossRows rows, float* part, int64_t tokens,
                                                         float scale) {
   pdl_wait();
