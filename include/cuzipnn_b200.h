@@ -45,7 +45,7 @@ const char *zn_last_error(void);
 uint64_t zn_launch_count(void);
 /* Kernel timing for measurement (no reference counterpart): while enabled, every launch of the
  * named kernel kind ("hist", "encode", "scan", "pack", "dscan", "decode", "decode_overflow",
- * "crc", or "*" for all) is bracketed by CUDA events on its launching stream.  zn_timing_read
+ * "crc", "gemm", "finish", or "*" for all) is bracketed by CUDA events on its launching stream.  zn_timing_read
  * waits for the recorded events of one kind (NULL: all) and returns the launches' count and the
  * time during which at least one of them ran (the union of their intervals: their summed duration
  * when they do not overlap), then forgets them. */
