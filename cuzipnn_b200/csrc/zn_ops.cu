@@ -840,6 +840,8 @@ struct Weight {
   int32_t* status;
 };
 
+constexpr int64_t kStoredPiece = 4 * 5 * 148 * (int64_t(1) << 17);  // as four waves of default chunks: 0.78 GB
+
 // rows_cap bounds the rows of a piece (0: no bound).
 int plan_weight(const zn_weight* w, int64_t rows_cap, int32_t* status, Arena& ar, Weight* out) {
   *out = {};
@@ -859,8 +861,9 @@ int plan_weight(const zn_weight* w, int64_t rows_cap, int32_t* status, Arena& ar
     const int64_t wave_rows = std::max<int64_t>(1, wave * w->chunk_bytes / w->cols);
     rows = 4 * wave_rows;
     if (rows_cap > 0 && rows > rows_cap) rows = rows_cap >= wave_rows ? rows_cap / wave_rows * wave_rows : rows_cap;
-  } else if (rows_cap > 0) {
-    rows = std::min(rows, rows_cap);
+  } else {  // copied to an address that TMA can read, as many elements at a time
+    rows = std::min(rows, std::max<int64_t>(1, kStoredPiece / w->cols));
+    if (rows_cap > 0) rows = std::min(rows, rows_cap);
   }
   if (rows < w->rows) rows = std::max<int64_t>(256, rows / 256 * 256);
   out->piece_rows = std::min(rows, w->rows);

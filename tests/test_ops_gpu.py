@@ -807,3 +807,45 @@ def test_inference_mode():
     z.blob_cross_entropy(xg, made, t).backward()  # the head is not kept for the backward pass
     with pytest.raises(RuntimeError, match="[Ii]nference"):
         z.blob_linear(xg, made)
+
+
+def test_large_stored_weight():
+    """A weight stored uncompressed is copied a bounded piece at a time (here two), never whole."""
+    vocab, cols, tokens = 130000, 3592, 30
+    w = torch.empty(vocab, cols, dtype=BF, device=DEV).normal_(0, 0.02)
+    blob = z.compress_tensor(w, readback_to_cpu=False, min_compress_bytes=1 << 40)
+    assert blob.numel() == 40 + w.numel() * 2
+    x = rnd(tokens, cols).requires_grad_()
+    dy = rnd(tokens, vocab)
+    torch.cuda.synchronize()
+    held = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    y = z.blob_linear(x, blob)
+    (dx,) = torch.autograd.grad(y, x, dy)
+    t = torch.randint(vocab, (tokens,), device=DEV)
+    loss = z.blob_cross_entropy(x, blob, t)
+    (dh,) = torch.autograd.grad(loss, x)
+    plain = z.blob_cross_entropy(x.detach(), blob, t)
+    torch.cuda.synchronize()
+    assert torch.cuda.max_memory_allocated() - held < 0.9e9
+    xe = x.detach().double().requires_grad_()
+    z64 = torch.cat([xe.detach() @ p.double().T for p in w.split(13000)], 1)
+    # The result: one rounding (2^-8) and the 32-bit sum (cols 2^-24 of the sum of magnitudes).
+    mag = torch.cat([xe.detach().abs() @ p.double().abs().T for p in w.split(13000)], 1)
+    assert bool(((y.double() - z64).abs() <= 2.0**-8 * z64.abs() + cols * 2.0**-24 * mag).all())
+    exact = sum(d.double() @ p.double() for d, p in zip(dy.split(13000, 1), w.split(13000)))
+    mag = sum(d.double().abs() @ p.double().abs() for d, p in zip(dy.split(13000, 1), w.split(13000)))
+    assert bool(((dx.double() - exact).abs() <= 2.0**-8 * exact.abs() + vocab * 2.0**-24 * mag).all())
+    zl = z64.requires_grad_()
+    le = torch.nn.functional.cross_entropy(zl, t)
+    (ds,) = torch.autograd.grad(le, zl)
+    # 32-bit logits are off by cols 2^-24 mag at most, the loss by no more than twice that; 1e-5 leaves 80
+    # roundings of 2^-24 for the exponentials, their sum and its logarithm on top.
+    loss, le = loss.detach(), le.detach()
+    assert abs(float(loss.double() - le)) <= 2 * cols * 2.0**-24 * float(
+        (xe.detach().abs() * w[:1].double().abs().max()).sum(1).max()) + 1e-5 * float(le)
+    assert abs(float(plain.double() - loss.double())) <= 1e-5 * float(le)
+    exact = sum(d @ p.double() for d, p in zip(ds.split(13000, 1), w.split(13000)))
+    mag = sum(d.abs() @ p.double().abs() for d, p in zip(ds.split(13000, 1), w.split(13000)))
+    # dh: one rounding of the result and one of P, relative to what is summed, and the sums' own error.
+    assert bool(((dh.double() - exact).abs() <= 2.0**-8 * exact.abs() + (2.0**-8 + 2.0**-10) * mag).all())
