@@ -18,7 +18,7 @@ CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libcuzipnn_b200.so")
 SOURCES = ["zn_api.cu", "zn_planes.cu", "zn_crc32.cu", "zn_encode.cu", "zn_decode.cu", "zn_weight.cu",
            "zn_ops.cu"]
-HEADERS = ["zn_common.cuh", "zn_decode.cuh", "zn_gemm.cuh", "zn_linear.cuh", "zn_weight.cuh"]
+HEADERS = ["zn_common.cuh", "zn_decode.cuh", "zn_dot_cols.h", "zn_gemm.cuh", "zn_linear.cuh", "zn_weight.cuh"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-O2", "-shared", "--expt-relaxed-constexpr"]
 

@@ -9,6 +9,7 @@
 #include <cuda_fp16.h>
 
 #include "zn_common.cuh"
+#include "zn_dot_cols.h"
 #include "zn_weight.cuh"
 
 namespace zn {
@@ -16,6 +17,7 @@ namespace {
 
 constexpr int kDecThreads = 128;  // 4 warps per chunk
 constexpr int kChains = 1;        // rANS states per lane (sub-chunks per lane)
+static_assert(kDotSteps == kSteps && kDotRound == kRound, "a round of the decoder");
 constexpr int64_t kCodedBit = int64_t(1) << 62;
 constexpr int64_t kOffMask = kCodedBit - 1;
 
@@ -430,23 +432,19 @@ struct DotSink {
 template <int MT>
 struct DotState {
   float c[MT][2];  // row lane / 4, columns 2 (lane % 4) and + 1 of each accumulator
-  int col;         // of the segment's first element in its current row (of the round before)
+  DotCols cols;    // the segment's place in its current row
   int row;         // the segment's current row
   bool first;      // no row end met in this sub-chunk yet
   bool mid;        // the sub-chunk starts inside a row
   uint4 x[MT][2];  // the round's elements of x, loaded before it is decoded
 };
 
-// Column of the next round's elements (lanes without elements get a valid one too).
+// Loads the next round's elements of x (those of row 0 for rows past the last).  Lanes without elements
+// load nothing: dot_products masks what they hold.
 template <class Sink>
-__device__ __forceinline__ int dot_col(const Sink& k, const DotState<Sink::kRows>& st, int l) {
-  const int col = st.col + kRound + l * kSteps;
-  return col >= k.cols ? col - k.cols : col;
-}
-// Loads the next round's elements of x (those of row 0 for rows past the last).
-template <class Sink>
-__device__ __forceinline__ void dot_load(const Sink& k, DotState<Sink::kRows>& st, int l) {
-  const int col = dot_col(k, st, l);
+__device__ __forceinline__ void dot_load(const Sink& k, DotState<Sink::kRows>& st, int l, bool active) {
+  const int col = st.cols.next(l, active, k.cols);
+  if (col < 0) return;
 #pragma unroll
   for (int m = 0; m < Sink::kRows; ++m) {
     const uint4* xp = reinterpret_cast<const uint4*>(k.x + (m < k.tokens ? m * k.ldx : 0) + col);
@@ -505,8 +503,8 @@ template <class Sink, bool ALL>
 __device__ __forceinline__ void dot_round(const Sink& k, DotState<Sink::kRows>& st, const uint32_t* e, bool active,
                                           int l, int seg, float* slot0) {
   constexpr int MT = Sink::kRows;
-  st.col += kRound;
-  const bool wrapped = active && st.col + l * kSteps >= k.cols;  // the lane's elements lie in the next row
+  st.cols.advance();
+  const bool wrapped = st.cols.wrapped(l, active, k.cols);  // the lane's elements lie in the next row
   const uint32_t over = __ballot_sync(0xFFFFFFFFu, wrapped);
   if (!over) {
     dot_products<Sink, !ALL>(st, e, active);
@@ -528,7 +526,7 @@ __device__ __forceinline__ void dot_round(const Sink& k, DotState<Sink::kRows>& 
     for (int m = 0; m < MT; ++m) st.c[m][0] = st.c[m][1] = 0.0f;
     st.first = false;
     ++st.row;
-    st.col -= k.cols;  // below 0 when the row ended inside the round
+    st.cols.wrap(k.cols);
   }
   dot_products<Sink, true>(st, e, wrapped);
 }
@@ -818,7 +816,7 @@ __device__ __forceinline__ void decode_chunk(const DecArgs& a, int64_t j, bool o
         const int64_t e0 = j * a.C + base[0];
         st.row = int(e0 / sink.cols);
         const int c0 = int(e0 - int64_t(st.row) * sink.cols);
-        st.col = c0 - kRound;  // dot_round advances it by a round first
+        st.cols.start(c0);
         st.first = true;
         st.mid = c0 != 0;
         return st;
@@ -873,7 +871,7 @@ __device__ __forceinline__ void decode_chunk(const DecArgs& a, int64_t j, bool o
               if (cb.nload) cb.r0 = block(cb.fill / 8);
             }
           }
-          if constexpr (Sink::kDot) dot_load(sink, dot, l);
+          if constexpr (Sink::kDot) dot_load(sink, dot, l, true);
           uint32_t p[kChains][K][4];
 #pragma unroll
           for (int c = 0; c < kChains; ++c)
@@ -974,7 +972,7 @@ __device__ __forceinline__ void decode_chunk(const DecArgs& a, int64_t j, bool o
 #pragma unroll
           for (int i = 0; i < 4; ++i) p[c][b][i] = pn[c][b][i];
       if (r + 1 < rounds) load_raw_round<K, kChains>(src, coded, base, len, r + 1, l, pn);
-      if constexpr (Sink::kDot) dot_load(sink, dot, l);
+      if constexpr (Sink::kDot) dot_load(sink, dot, l, nact[0] == kSteps);
       const bool full = nact[0] == kSteps && nact[kChains - 1] == kSteps;
 #pragma unroll
       for (int q = 0; q < KC; ++q) {
