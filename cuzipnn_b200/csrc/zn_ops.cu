@@ -17,14 +17,20 @@
 // The gradient comes with the loss, in one pass over the vocabulary, like attention with W as keys
 // and values:  softmax(s) W = (sum_v exp(s_v - r) W_v) / (sum_v exp(s_v - r)) for any reference r of
 // the row.  Each piece is decoded once and multiplied twice (4 tokens rows cols operations in all,
-// against 6 and two decodings for computing the logits again in a backward pass).  r is the maximum
-// over the first kSample rows of W; the 16-bit P then holds exp(s - r) up to a bound (2^60 for
-// bf16, 2^15 for fp16).  Where a group of 32 logits passes the bound, its P is zero, the row's r is
-// raised to its maximum, what was summed is scaled down, and the piece is multiplied again with
-// the groups that were left out alone (kernels that end at once when there are none).
-// P is rounded to 16 bits.  At the row's own ids that would be wrong where it matters most (a
-// confident softmax less q is a small difference), so P is zero there and the ids' terms
-// (exp(s_k - r) and q_k times their rows of W) are added in 32 bits by gather_kernel.
+// against 6 and two decodings for computing the logits again in a backward pass).
+//
+// P = exp(s - r) is rounded to 16 bits.  At the row's own ids that would be wrong where it matters most
+// (a confident softmax less q is a small difference), so the ids' columns take no part in P nor in r:
+// P is zero there, and the ids' terms are added in 32 bits (gather_kernel, soft_end_kernel).  With a
+// single id p - q is -S / (S + e), from the sum S over the other columns and the id's own e: no
+// difference is taken at all, and a confident row's gradient is as exact as any other's.
+// r is the maximum of the other columns of the first kSample rows of W, less kBelow powers of two in
+// fp16, whose P would else lose the tail of the softmax: it spans 2^kBelow at the largest column down to
+// 2^-25, so that of V columns those below lose V 2^(-25 - kBelow) of the sum at most (2^-15.8 for
+// 152064, under fp16's rounding of 2^-11).  Up to a bound (2^60 for bf16, 2^15 for fp16) P may exceed
+// that.  Where a group of 32 logits passes the bound, its P is zero, the row's r is raised for its
+// maximum, what was summed is scaled down, and the piece is multiplied again with the groups that were
+// left out alone (kernels that end at once when there are none).
 #include <algorithm>
 
 #include "zn_linear.cuh"
@@ -176,15 +182,77 @@ struct EpiStats {
   };
 };
 
+// The ids of a row among the columns that a thread reads from n0 on, in their order.
+struct IdWalk {
+  const int32_t* ids = nullptr;
+  int at = 0, count = 0;
+  int64_t next = INT64_MAX;  // column (of the piece) of the next id
+  int64_t v0 = 0;
+  __device__ __forceinline__ IdWalk() {}
+  __device__ __forceinline__ IdWalk(const LossRows& rows, int64_t m, int64_t v0_, int64_t n0) : v0(v0_) {
+    count = max(0, rows.count[m]);
+    ids = rows.ids + m * rows.top;
+    at = first_id(ids, count, v0 + n0);
+    if (at < count) next = ids[at] - v0;
+  }
+  __device__ __forceinline__ void step() {
+    ++at;
+    next = at < count ? ids[at] - v0 : INT64_MAX;
+  }
+};
+
+// The maximum of a row's logits but for its ids' (for the first reference).
+struct EpiMax {
+  static constexpr bool kParts = false;
+  LossRows rows;
+  float* part;    // [half tile][M]
+  int64_t M, N;   // columns 0 .. N - 1 of the vocabulary
+  int tile_cols;  // columns of a half tile
+  float scale;    // log2(e) / T
+  struct Row {
+    int64_t m, n0;
+    float mx;
+    IdWalk walk;
+    __device__ __forceinline__ Row(const EpiMax& e, int64_t m_, int64_t n0_, int, uint8_t*)
+        : m(m_), n0(n0_), mx(-INFINITY) {
+      if (m < e.M) walk = IdWalk(e.rows, m, 0, n0);
+    }
+    __device__ __forceinline__ void cols(const EpiMax& e, int c, float* v) {
+      if (m >= e.M) return;
+      const int left = int(min(int64_t(32), e.N - n0 - c));
+      if (walk.next < n0 + c + 32) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          while (walk.next == n0 + c + i) {
+            v[i] = -INFINITY;
+            walk.step();
+          }
+      }
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (i < left) mx = fmaxf(mx, v[i] * e.scale);
+    }
+    __device__ __forceinline__ void end(const EpiMax& e) {
+      if (m < e.M && n0 < e.N) e.part[n0 / e.tile_cols * e.M + m] = mx;
+    }
+  };
+};
+
 // State of a loss with its gradient, per row, in units of log2(e) (s' = s log2(e)).
 struct SoftRows {
   float* ref;      // r
   float* before;   // r before this piece
   float* scale;    // 2^(before - r)
-  float* sum;      // sum of 2^(s' - r) over the columns so far
+  float* sum;      // sum of 2^(s' - r) over the columns so far, without the ids'
   float* hit;      // [tokens][top] s' at the row's ids
-  int32_t* again;  // of this piece: a group was left out
+  int32_t* again;  // of this piece: a group was left out, or an id lies far above r
 };
+
+// How far below the largest column r lies, in powers of two (see the head of this file).
+template <typename T>
+constexpr float kBelow = Num<T>::kCode == 1 ? 0.0f : 8.0f;
+// Rows of several ids add 2^(s'_k - r) W to the others' sum: r is raised so that this stays in a float.
+constexpr float kIdBound = 100.0f, kIdAbove = 64.0f;
 
 // P = 2^(s' - r) of one piece, in 16 bits, as the operand of the product with the piece; zero at the
 // row's ids, and in rows that do not count whatever their logits are.  AGAIN: the groups that the
@@ -196,7 +264,7 @@ struct EpiSoft {
   LossRows rows;
   SoftRows soft;
   T* p;
-  float* part;       // [half tile][2][M]: sum, and the maximum s' of the groups left out
+  float* part;       // [half tile][2][M]: sum, and the reference that the groups left out ask for
   int64_t M, N, ld;  // N: columns of this piece; ld: a multiple of 8
   int64_t v0;        // first vocabulary row of this piece
   int tile_cols;     // columns of a half tile
@@ -204,49 +272,40 @@ struct EpiSoft {
   struct Row {
     int64_t m, n0;
     uint8_t* buf;
-    const int32_t* ids;
     float ref, before, sum, out;
-    int at, count;
-    int64_t next;  // column (of the piece) of the next id
+    IdWalk walk;
     __device__ __forceinline__ Row(const EpiSoft& e, int64_t m_, int64_t n0_, int, uint8_t* b) : m(m_), n0(n0_), buf(b) {
-      at = count = 0;
-      next = INT64_MAX;
       ref = before = sum = 0.0f;
       out = -INFINITY;
-      ids = nullptr;
       if (m < e.M) {
-        count = max(0, e.rows.count[m]);
         ref = e.soft.ref[m];
         before = AGAIN ? e.soft.before[m] : ref;
-        ids = e.rows.ids + m * e.rows.top;
-        at = first_id(ids, count, e.v0 + n0);
-        if (at < count) next = ids[at] - e.v0;
+        walk = IdWalk(e.rows, m, e.v0, n0);
       }
     }
     __device__ __forceinline__ void cols(const EpiSoft& e, int c, float* v) {
       if (n0 + c >= e.N) return;
       const int left = int(min(int64_t(32), e.N - n0 - c));
+      if (walk.next < n0 + c + 32) {  // the ids' logits, and their columns out of P
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (walk.next == n0 + c + i) {
+            const float s = v[i] * e.scale;
+            if (!AGAIN && e.rows.top > 1 && (before == -INFINITY || s - before > kIdBound)) out = fmaxf(out, s - kIdAbove);
+            while (walk.next == n0 + c + i) {
+              if (!AGAIN) e.soft.hit[m * e.rows.top + walk.at] = s;
+              walk.step();
+            }
+            v[i] = -INFINITY;
+          }
+      }
       float mx = -INFINITY;
 #pragma unroll
       for (int i = 0; i < 32; ++i)
         if (i < left) mx = fmaxf(mx, v[i]);
       const bool over = before == -INFINITY ? mx > -INFINITY : fmaf(mx, e.scale, -before) > kBound;
-      const bool take = count > 0 && over == AGAIN;
-      if (!AGAIN && over) out = fmaxf(out, mx * e.scale);
-      if (next < n0 + c + 32) {  // the ids' logits, and their columns out of P
-        const float base = ref == -INFINITY ? 0.0f : ref;
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (next == n0 + c + i) {
-            if (take) sum += ex2(fmaf(v[i], e.scale, -base));
-            while (next == n0 + c + i) {
-              if (!AGAIN) e.soft.hit[m * e.rows.top + at] = v[i] * e.scale;
-              ++at;
-              next = at < count ? ids[at] - e.v0 : INT64_MAX;
-            }
-            v[i] = -INFINITY;
-          }
-      }
+      const bool take = walk.count > 0 && over == AGAIN;
+      if (!AGAIN && over) out = fmaxf(out, fmaf(mx, e.scale, -kBelow<T>));
       const float base = ref == -INFINITY ? 0.0f : ref;
       float add = 0.0f;
 #pragma unroll
@@ -266,7 +325,7 @@ struct EpiSoft {
       if (m >= e.M || n0 >= e.N) return;
       float* p = e.part + (n0 / e.tile_cols) * 2 * e.M + m;
       p[0] = sum;
-      p[e.M] = count > 0 ? out : -INFINITY;
+      p[e.M] = walk.count > 0 ? out : -INFINITY;
     }
   };
 };
@@ -566,21 +625,22 @@ __global__ void __launch_bounds__(1024) loss_rows_kernel(const float* part, int6
   loss[m] = count == 0 ? 0.0f : temperature * temperature * (rows.q0[m] + (lse - st.hit * kLn2));
 }
 
-// The first reference of each row: its maximum over the columns of the sample.
-__global__ void __launch_bounds__(1024) sample_kernel(const float* part, int64_t tiles, int64_t tokens, SoftRows soft) {
+// The first reference of each row: its maximum over the columns of the sample, less `below`.
+__global__ void __launch_bounds__(1024) sample_kernel(const float* part, int64_t tiles, int64_t tokens, float below,
+                                                      SoftRows soft) {
   pdl_wait();
   pdl_trigger();
   const int64_t m = int64_t(blockIdx.x) * 32 + (threadIdx.x & 31);
   const int sub = threadIdx.x >> 5;
   float mx = -INFINITY;
   if (m < tokens)
-    for (int64_t t = sub; t < tiles; t += 32) mx = fmaxf(mx, part[t * 3 * tokens + m]);
+    for (int64_t t = sub; t < tiles; t += 32) mx = fmaxf(mx, part[t * tokens + m]);
   __shared__ float sm[32][33];
   sm[sub][threadIdx.x & 31] = mx;
   __syncthreads();
   if (sub != 0 || m >= tokens) return;
   for (int i = 1; i < 32; ++i) mx = fmaxf(mx, sm[i][threadIdx.x]);
-  soft.ref[m] = mx;
+  soft.ref[m] = mx - below;
   soft.sum[m] = 0.0f;
 }
 
@@ -620,9 +680,10 @@ __global__ void __launch_bounds__(1024) soft_rows_kernel(const float* part, int6
   soft.sum[m] = sum * scale;
 }
 
-// The terms of a row's ids in this piece: acc += 2^(s'_k - r) W[id_k], acc_q += q_k W[id_k], in 32 bits;
-// and the sums of the groups that were multiplied again.  One CTA per row.  2048 rows of 3584 with one id
-// each take 28 us (132 MB, 4.7 TB/s), beside 640 us of products for a piece of 27000 rows.
+// The terms of a row's ids in this piece: acc += 2^(s'_k - r) W[id_k], acc_q += q_k W[id_k], in 32 bits,
+// or for a row of a single id acc_q = W[id] (soft_end_kernel knows its factor); and the sums of the groups
+// that were multiplied again.  One CTA per row.  2048 rows of 3584 with one id each take 28 us (132 MB,
+// 4.7 TB/s), beside 640 us of products for a piece of 27000 rows.
 template <typename T>
 __global__ void __launch_bounds__(128) gather_kernel(LossRows rows, SoftRows soft, const T* w, int64_t pitch,
                                                      int64_t v0, int64_t v1, int64_t cols, float* acc, float* acc_q,
@@ -646,6 +707,16 @@ __global__ void __launch_bounds__(128) gather_kernel(LossRows rows, SoftRows sof
     if (tid == 0) soft.sum[m] += s_sum[0];
   }
   if (a == b) return;
+  if (rows.top == 1) {
+    const T* src = w + (ids[0] - v0) * pitch;
+    for (int64_t c = 8 * tid; c < cols; c += 8 * 128) {
+      const uint4 q = *reinterpret_cast<const uint4*>(src + c);
+      float4* out = reinterpret_cast<float4*>(acc_q + m * ld + c);
+      out[0] = make_float4(Num<T>::lo(q.x), Num<T>::hi(q.x), Num<T>::lo(q.y), Num<T>::hi(q.y));
+      if (c + 4 < cols) out[1] = make_float4(Num<T>::lo(q.z), Num<T>::hi(q.z), Num<T>::lo(q.w), Num<T>::hi(q.w));
+    }
+    return;
+  }
   const float ref = soft.ref[m], base = ref == -INFINITY ? 0.0f : ref;
   for (int k = a + tid; k < b; k += 128) {
     // An id given twice is one column of the softmax: only its first entry carries it.
@@ -698,38 +769,78 @@ __device__ __forceinline__ void store_floats(float* p, const float* v) {
   else *p = v[0];
 }
 
-// A row's loss, and its gradient T (acc / sum - acc_q), V columns per thread.  One CTA per row.  Bound by
-// its bytes: 2048 x 3584 in 15 us (88 MB at 5.9 TB/s; one column at a time took 22 us).
+// Sum or maximum over a block of 128 threads, on every thread.
+template <bool MAX>
+__device__ __forceinline__ float block_join(float v, float* sm) {
+  for (int o = 16; o; o >>= 1) {
+    const float u = __shfl_xor_sync(0xFFFFFFFFu, v, o);
+    v = MAX ? fmaxf(v, u) : v + u;
+  }
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = v;
+  __syncthreads();
+  return MAX ? fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3])) : (sm[0] + sm[1]) + (sm[2] + sm[3]);
+}
+
+// A row's loss and its gradient, V columns per thread.  With S = sum over the columns that are no ids, of
+// 2^(s' - r), and E the same over the ids: lse' = r + log2(S + E), and the gradient is
+//   T (acc / (S + E) - acc_q)                      for several ids, acc and acc_q holding their terms,
+//   T (acc / (S + E) - S / (S + E) W[id])          for one (q = 1, acc_q = W[id]), whose loss is
+//                                                  log(1 + S / E): no difference of near numbers.
+// One CTA per row.  Bound by its bytes: 2048 x 3584 in 15 us (88 MB at 5.9 TB/s; one column at a time
+// took 22 us).
 template <int V>
 __global__ void __launch_bounds__(128) soft_end_kernel(LossRows rows, SoftRows soft, const float* __restrict__ acc,
                                                        const float* __restrict__ acc_q, int64_t ld, int64_t cols,
                                                        float temperature, float* loss, float* __restrict__ unit) {
   pdl_wait();
   pdl_trigger();
-  __shared__ float s_sum[128];
+  __shared__ float sm[4];
   const int64_t m = blockIdx.x;
   const int count = rows.count[m], tid = threadIdx.x;
-  float hit = 0.0f;
-  for (int k = tid; k < count; k += 128) hit += rows.q[m * rows.top + k] * soft.hit[m * rows.top + k];
-  s_sum[tid] = hit;
-  __syncthreads();
-  for (int o = 64; o; o >>= 1) {
-    if (tid < o) s_sum[tid] += s_sum[tid + o];
-    __syncthreads();
+  const float ref = soft.ref[m], sum = soft.sum[m];
+  const int32_t* ids = rows.ids + m * rows.top;
+  const float* q = rows.q + m * rows.top;
+  const float* hit = soft.hit + m * rows.top;
+  float nats = 0.0f, total = 1.0f, fq = 0.0f;  // the loss over T^2 less q0, S + E, the factor of acc_q
+  if (rows.top == 1) {
+    if (count > 0) {
+      const float s = hit[0] < INFINITY ? hit[0] : NAN;  // an infinite target has no loss
+      const float x = (ref - s) + log2f(sum), e = ref > -INFINITY ? ex2(s - ref) : s > -INFINITY ? 1.0f : NAN;
+      nats = fmaxf(x, 0.0f) * kLn2 + log1pf(exp2f(-fabsf(x)));
+      total = sum + e;
+      fq = -q[0] * (sum / total);
+    }
+  } else {
+    float mx = ref;
+    for (int k = tid; k < count; k += 128) mx = fmaxf(mx, hit[k]);
+    mx = block_join<true>(mx, sm);
+    const float base = ref == -INFINITY ? 0.0f : ref;
+    float e = 0.0f, z = 0.0f, d = 0.0f;
+    for (int k = tid; k < count; k += 128) {
+      if (k == 0 || ids[k] != ids[k - 1]) {  // an id given twice is one column of the softmax
+        e += ex2(hit[k] - base);
+        z += ex2(hit[k] - mx);
+      }
+      if (q[k] != 0.0f) d += q[k] * (mx - hit[k]);
+    }
+    e = block_join<false>(e, sm);
+    z = block_join<false>(z, sm);
+    d = block_join<false>(d, sm);
+    nats = (d + log2f(sum * ex2(ref - mx) + z)) * kLn2;
+    total = sum + e;
+    fq = -1.0f;
   }
-  const float sum = soft.sum[m];
-  if (tid == 0) {
-    const float lse = count < 0 ? NAN : (soft.ref[m] + log2f(sum)) * kLn2;
-    loss[m] = count == 0 ? 0.0f : temperature * temperature * (rows.q0[m] + (lse - s_sum[0] * kLn2));
-  }
-  const float f = temperature / sum;
+  if (tid == 0) loss[m] = count == 0 ? 0.0f : count < 0 ? NAN : temperature * temperature * (rows.q0[m] + nats);
+  const float f = temperature / total;
+  fq *= temperature;
 #pragma unroll 4
   for (int64_t c = V * tid; c < cols; c += V * 128) {
-    float a[V], q[V];
+    float a[V], g[V];
     load_floats<V>(acc + m * ld + c, a);
-    load_floats<V>(acc_q + m * ld + c, q);
+    load_floats<V>(acc_q + m * ld + c, g);
 #pragma unroll
-    for (int i = 0; i < V; ++i) a[i] = count < 0 ? NAN : count == 0 ? 0.0f : fmaf(a[i], f, -temperature * q[i]);
+    for (int i = 0; i < V; ++i) a[i] = count < 0 ? NAN : count == 0 ? 0.0f : fmaf(a[i], f, fq * g[i]);
     store_floats<V>(unit + m * cols + c, a);
   }
 }
@@ -1268,10 +1379,10 @@ int soft_piece(const LossGradPlan& p, const Matrix& xm, const Matrix& wm, int64_
   if (r0 == 0) {
     const Matrix first{wm.p, std::min(kSample, n), cols, wm.pitch};
     const Cut c = cut_of(tokens, first.rows, cols, p.sms, false);
-    const EpiStats e{rows, p.part, tokens, first.rows, 0, 0, 64 * c.cg, scale};
+    const EpiMax e{rows, p.part, tokens, first.rows, 64 * c.cg, scale};
     if (int rc = product<T, false>(xm, first, c, nullptr, e, p.w.status, s)) return rc;
     if (int rc = launch_after(sample_kernel, dim3(row_blocks), 1024, 0, s, "sample_kernel",
-                              static_cast<const float*>(p.part), cdiv(first.rows, 64 * c.cg), tokens, soft))
+                              static_cast<const float*>(p.part), cdiv(first.rows, 64 * c.cg), tokens, kBelow<T>, soft))
       return rc;
   }
   const EpiSoft<T, false> e{rows, soft, static_cast<T*>(p.prob), p.part, tokens, n, p.ldp, r0, half, scale};
