@@ -43,14 +43,17 @@ __device__ __forceinline__ float activate(int act, float z, float& slope) {
   }
 }
 
-// The derivative act'(z), kept for the backward pass as a 16-bit fixed-point number of step 2^-14
-// (every activation's lies in [-0.13, 1.13]): off by 2^-15 of a whole slope at most, an eighth of
-// a bf16 rounding, so the gradients are as exact as with a 32-bit slope.  -32768 stands for NaN.
-// (The sum's low 16 bits are the rounded product: 1.5 * 2^23 leaves no fraction bits.)
-__device__ __forceinline__ uint32_t slope_code(float s) {
-  return s != s ? 0x8000u : __float_as_uint(fmaf(s, 16384.0f, 12582912.0f)) & 0xFFFFu;
+// The derivative act'(z) is kept for the backward pass as float16 of 2^15 act'(z), whatever the weight's
+// type: every activation's derivative lies in [-0.13, 1.13], so the scaled one stays below 37100, and the
+// 15 exponents that a float16 would leave unused above 1 extend it downwards.  Off by 2^-11 of itself at
+// most (an eighth of a bf16 rounding, one of fp16) as far as |act'(z)| >= 2^-29, and by 2^-40 below:
+// silu' keeps its digits to z = -23, gelu' to -6.
+constexpr float kSlopeScale = 32768.0f;
+__device__ __forceinline__ uint32_t slope_codes(float s0, float s1) {
+  return Num<__half>::pack(s0 * kSlopeScale, s1 * kSlopeScale);
 }
-__device__ __forceinline__ float slope_value(int code) { return code == -32768 ? NAN : float(code) * (1.0f / 16384.0f); }
+__device__ __forceinline__ float slope_lo(uint32_t w) { return Num<__half>::lo(w) * (1.0f / kSlopeScale); }
+__device__ __forceinline__ float slope_hi(uint32_t w) { return Num<__half>::hi(w) * (1.0f / kSlopeScale); }
 
 // Per-warp staging: a thread holds 64 bytes (32 16-bit columns) of its own row; through shared
 // memory the warp writes them as 8 rows x 64 contiguous bytes per store.  The 16-byte chunks of a
@@ -121,7 +124,7 @@ struct EpiLinear {
   const T* bias;  // or null
   const T* res;   // or null
   T* y;
-  int16_t* slope;  // or null
+  __half* slope;  // or null
   int64_t ldr, ldy, M, N;
   int act;
   bool vec;  // 16-byte accesses: every pointer and pitch allows them, and N is a multiple of 8
@@ -144,7 +147,7 @@ struct EpiLinear {
         float s0, s1;
         v[2 * i] = activate<ACT, SLOPE>(v[2 * i], s0);
         v[2 * i + 1] = activate<ACT, SLOPE>(v[2 * i + 1], s1);
-        if (SLOPE) sw[i] = slope_code(s0) | (slope_code(s1) << 16);
+        if (SLOPE) sw[i] = slope_codes(s0, s1);
       }
       if (SLOPE) stage_rows(buf, sw, e.slope, e.ldy, m - (threadIdx.x & 31), e.M, n, e.N, e.vec);
     }
@@ -245,7 +248,7 @@ __device__ __forceinline__ void finish_value(const EpiLinear<T>& e, int64_t m, i
   z = e.slope ? activate<true>(e.act, z, sl) : activate<false>(e.act, z, sl);
   if (e.res) z += Num<T>::to(e.res[m * e.ldr + n]);
   e.y[m * e.ldy + n] = Num<T>::from(z);
-  if (e.slope) e.slope[m * e.ldy + n] = int16_t(slope_code(sl));
+  if (e.slope) e.slope[m * e.ldy + n] = Num<__half>::from(sl * kSlopeScale);
 }
 
 // y = act(z + bias) + residual from z = acc, or from weight_dot.

@@ -391,7 +391,7 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Fin
 constexpr int kSumRows = 64, kSumAll = 512;
 template <typename T, int V>
 __global__ void __launch_bounds__(256) slope_kernel(const T* __restrict__ dy, int64_t ldy,
-                                                    const int16_t* __restrict__ slope, T* __restrict__ dz, int64_t ldz,
+                                                    const __half* __restrict__ slope, T* __restrict__ dz, int64_t ldz,
                                                     float* __restrict__ part, T* __restrict__ dbias, int64_t M,
                                                     int64_t N, int64_t per) {
   pdl_wait();
@@ -423,8 +423,8 @@ __global__ void __launch_bounds__(256) slope_kernel(const T* __restrict__ dy, in
             for (int i = 0; i < 4; ++i) {
               float a = Num<T>::lo(gw[i]), b = Num<T>::hi(gw[i]);
               if (slope) {
-                a *= slope_value(int16_t(ww[i]));
-                b *= slope_value(int16_t(ww[i] >> 16));
+                a *= slope_lo(ww[i]);
+                b *= slope_hi(ww[i]);
               }
               z[i] = Num<T>::pack(a, b);
               s[2 * i] += a;
@@ -436,7 +436,7 @@ __global__ void __launch_bounds__(256) slope_kernel(const T* __restrict__ dy, in
     } else {
       for (int64_t m = mb * per + sub; m < m1; m += 8) {
         float d = Num<T>::to(dy[m * ldy + n]);
-        if (slope) d *= slope_value(slope[m * N + n]);
+        if (slope) d *= slope_lo(__half_as_ushort(slope[m * N + n]));
         if (dz) dz[m * ldz + n] = Num<T>::from(d);
         s[0] += d;
       }
@@ -1118,7 +1118,7 @@ EpiLinear<T> linear_epilogue(const void* bias, const void* res, int64_t ldr, voi
   e.bias = bias ? static_cast<const T*>(bias) + r0 : nullptr;
   e.res = res ? static_cast<const T*>(res) + r0 : nullptr;
   e.y = static_cast<T*>(y) + r0;
-  e.slope = slope ? static_cast<int16_t*>(slope) + r0 : nullptr;
+  e.slope = slope ? static_cast<__half*>(slope) + r0 : nullptr;
   e.ldr = ldr;
   e.ldy = ldy;
   e.M = M;
@@ -1195,7 +1195,7 @@ int run_linear_grad(const LinearGradPlan& p, const zn_weight* w, const void* dy,
     if (grid > 0x7FFFFFFF) return bad("zn_linear_grad");
     auto fn = vec ? slope_kernel<T, 8> : slope_kernel<T, 1>;
     if (int rc = launch_after(fn, dim3(unsigned(grid)), 256, 0, s, "slope_kernel", g, ldy,
-                              static_cast<const int16_t*>(slope), dz, p.ldz, p.part,
+                              static_cast<const __half*>(slope), dz, p.ldz, p.part,
                               dbias && !p.part ? static_cast<T*>(dbias) : nullptr, tokens, rows, p.sum_rows))
       return rc;
   }

@@ -174,7 +174,7 @@ typedef struct {
 
 /* y [tokens, rows] (contiguous) = act(x W^T + bias) + residual.  activation: 0 none, 1 relu, 2 gelu
  * (erf), 3 gelu (tanh), 4 silu.  bias, residual and slope may be NULL; slope [tokens, rows]
- * (int16) gets act'(z) in steps of 2^-14 (-32768: NaN), which zn_linear_grad takes. */
+ * gets 2^15 act'(z) as float16, which zn_linear_grad takes. */
 size_t zn_linear_temp_bytes(const zn_weight *w, const void *x, int64_t ldx, int64_t tokens);
 int zn_linear(const zn_weight *w, const void *x, int64_t ldx, int64_t tokens, const void *bias, int activation,
               const void *residual, int64_t ldr, void *y, void *slope, int32_t *status, void *temp,
