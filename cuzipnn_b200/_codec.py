@@ -440,15 +440,20 @@ def _parse_header(prefix: Buffer, off: int = 0, length: int | None = None
     return _DTYPES[code], shape, flags, chunk_bytes, n_comp, n
 
 
-# Status words of the calling thread's latest decompress call per device (0 = no decoding error).
-# Per thread, so that threads decoding on one device do not overwrite each other's status.
+# Status words of the calling thread's latest decompress call per device (0 = no decoding error): a
+# tensor, or a tuple of them.  Per thread, so that threads decoding on one device do not overwrite each
+# other's status.
 _STATUS = threading.local()
 
 
-def _set_status(device: torch.device, status: torch.Tensor) -> None:
+def _statuses() -> dict:
     if not hasattr(_STATUS, "by_dev"):
         _STATUS.by_dev = {}
-    _STATUS.by_dev[device.index] = status
+    return _STATUS.by_dev
+
+
+def _set_status(device: torch.device, status: torch.Tensor) -> None:
+    _statuses()[device.index] = status
 
 
 def last_decode_status(device: torch.device | str | int | None = None) -> int:
@@ -463,8 +468,9 @@ def last_decode_status(device: torch.device | str | int | None = None) -> int:
     if st is None:
         return 0
     bits = 0
-    for v in st.cpu().tolist():  # one word per blob of the latest call: OR them
-        bits |= int(v)
+    for words in st if isinstance(st, tuple) else (st,):
+        for v in words.cpu().tolist():  # one word per blob of the latest call: OR them
+            bits |= int(v)
     return bits
 
 

@@ -9,7 +9,8 @@ Blobs must be on the GPU of the other operands.  A blob that compress_tensor(...
 False) or upload_blob returned carries its header, and the calls neither read anything back nor
 synchronise, so they can be captured into a CUDA graph; another GPU blob costs one header read per
 call.  Decoding errors are reported by last_decode_status(), as for decompress_tensor (a malformed
-chunk counts as zeros).
+chunk counts as zeros); after a backward pass that decoded, it reports that pass and its forward pass,
+to the thread that called the operator.
 """
 
 from __future__ import annotations
@@ -22,7 +23,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._codec import (_CODES, _FIXED, _FLAG_REORDER, _FLAG_STORED, _MAX_NDIM, _REORDER, _check_device, _gpu,
-                     _known_header, _on, _parse_header, _remember, _set_status, _stream, _upload)
+                     _known_header, _on, _parse_header, _remember, _set_status, _statuses, _stream, _upload)
 
 _ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 _REDUCTIONS = {"mean": 0, "sum": 1, "none": 2}
@@ -167,7 +168,7 @@ class _Linear(torch.autograd.Function):
         want = act != 0 and (ctx.needs_input_grad[0] or ctx.needs_input_grad[2])
         y, slope = _linear_forward(w, x, shape, bias, act, residual, want, status)
         _set_status(w.device, status)
-        ctx.w, ctx.status, ctx.x_shape = w, status, x.shape
+        ctx.w, ctx.status, ctx.statuses, ctx.x_shape = w, status, _statuses(), x.shape
         ctx.save_for_backward(blob, slope)  # the blob: an in-place change before backward raises
         return y
 
@@ -184,9 +185,12 @@ class _Linear(torch.autograd.Function):
         if need_x or need_b:
             with _on(w.device):
                 g, ldy = _rows(dy, w.rows)
+                status = torch.empty(1, dtype=torch.int32, device=w.device)
                 w.call("zn_linear_grad",
                        (g.data_ptr(), ldy, g.shape[0], int(slope is not None), int(need_x), int(need_b)),
-                       (g.data_ptr(), ldy, g.shape[0], _ptr(slope), _ptr(dx), _ptr(db)), ctx.status)
+                       (g.data_ptr(), ldy, g.shape[0], _ptr(slope), _ptr(dx), _ptr(db)), status)
+                if need_x:  # it decoded; the engine's thread reports to the one that called the layer
+                    ctx.statuses[w.device.index] = (ctx.status, status)
         return dx, None, db, dy if need_r else None, None, None, None
 
 
