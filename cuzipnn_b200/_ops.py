@@ -19,6 +19,7 @@ import ctypes
 import math
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -146,6 +147,12 @@ def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+def _check_tangent(name: str, t: torch.Tensor) -> None:
+    """Operands with a forward-mode tangent: they need no gradient, so the tangent would be lost."""
+    if unpack_dual(t).tangent is not None:
+        raise NotImplementedError(f"{name} carries a forward-mode derivative: operators on blobs have none")
+
+
 def _linear_forward(w: _Weight, x, shape, bias, act: int, residual, want_slope: bool, status):
     y = torch.empty(shape, dtype=w.dtype, device=w.device)
     slope = torch.empty(shape, dtype=torch.float16, device=w.device) if want_slope else None
@@ -216,6 +223,7 @@ def blob_linear(
     if activation not in _ACTIVATIONS:
         raise ValueError(f"activation must be one of {sorted(map(str, _ACTIVATIONS))}, not {activation!r}")
     w = _Weight(blob, x, "x")
+    _check_tangent("x", x)
     shape = (*x.shape[:-1], w.rows)
     for name, t, expected in (("bias", bias, (w.rows,)), ("residual", residual, shape)):
         if t is None:
@@ -226,6 +234,7 @@ def blob_linear(
             raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {expected}")
         if t.device != w.device:
             raise ValueError(f"{name} is on {t.device}, x on {w.device}")
+        _check_tangent(name, t)
     w.place("x")
     act = _ACTIVATIONS[activation]
     with _on(w.device):
@@ -282,6 +291,7 @@ class _Loss(torch.autograd.Function):
 
 
 def _loss(hidden, w, ids, logits, top, ignore_index, temperature, reduction, shape):
+    _check_tangent("hidden", hidden)
     w.place("hidden")
     red = _REDUCTIONS[reduction]
     args = (ids, logits, top, ignore_index, temperature, red)
