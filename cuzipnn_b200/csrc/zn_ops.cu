@@ -621,8 +621,9 @@ __global__ void __launch_bounds__(1024) loss_rows_kernel(const float* part, int6
   if (sub != 0 || m >= tokens) return;
   for (int i = 1; i < 32; ++i) stats_join(st, sm[i][threadIdx.x].mx, sm[i][threadIdx.x].sum, sm[i][threadIdx.x].hit);
   const int count = rows.count[m];
-  const float lse = count < 0 ? NAN : (st.mx + log2f(st.sum)) * kLn2;
-  loss[m] = count == 0 ? 0.0f : temperature * temperature * (rows.q0[m] + (lse - st.hit * kLn2));
+  // (mx - hit first: a confident row's loss is small beside both.)
+  const float nats = count < 0 ? NAN : ((st.mx - st.hit) + log2f(st.sum)) * kLn2;
+  loss[m] = count == 0 ? 0.0f : temperature * temperature * (rows.q0[m] + nats);
 }
 
 // The first reference of each row: its maximum over the columns of the sample, less `below`.
