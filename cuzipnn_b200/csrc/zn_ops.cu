@@ -166,7 +166,7 @@ struct EpiStats {
 #pragma unroll
         for (int i = 0; i < 32; ++i)
           while (next == n0 + c + i) {
-            st.hit += q[at] * s[i];
+            if (q[at] != 0.0f) st.hit += q[at] * s[i];
             ++at;
             next = at < count ? ids[at] - e.v0 : INT64_MAX;
           }
@@ -582,7 +582,8 @@ __global__ void __launch_bounds__(256) dot_stats_kernel(DotValue v, LossRows row
     sum += ex2(s[i] - base);
     const int64_t n = n0 + threadIdx.x + 256 * i;
     if (n < n1)
-      for (int k = first_id(ids, count, n); k < count && ids[k] == n; ++k) hit += q[k] * s[i];
+      for (int k = first_id(ids, count, n); k < count && ids[k] == n; ++k)
+        if (q[k] != 0.0f) hit += q[k] * s[i];
   }
   __shared__ RowStats sm[8];
   RowStats st{mx, sum, hit};

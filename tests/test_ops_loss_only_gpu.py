@@ -117,3 +117,21 @@ def test_small_losses_keep_their_digits(tokens, grad):
     assert float(want.max()) < 0.1
     loss = z.blob_cross_entropy(h.requires_grad_(grad), blob, t, reduction="none")
     assert_within(loss, want, 2.0**-21 + 4 * 2.0**-24 * 205 * want)
+
+
+@pytest.mark.parametrize("tokens", [1, 30])
+@pytest.mark.parametrize("grad", [False, True])
+def test_infinite_logit_that_the_teacher_excludes(tokens, grad):
+    """An entry of probability 0 adds nothing to the loss, also where the student's logit is -inf."""
+    w = rnd(700, 128, scale=0.05)
+    w[9] = -math.inf
+    blob = z.compress_tensor(w, chunk_bytes=4096, min_compress_bytes=0, readback_to_cpu=False)
+    h = rnd(tokens, 128).abs() + 0.1
+    ids = torch.tensor([[3, 9, 600]], device=DEV).repeat(tokens, 1)
+    logits = torch.tensor([[1.0, -math.inf, 2.0]], device=DEV).repeat(tokens, 1)
+    loss = z.blob_distillation(h.requires_grad_(grad), blob, logits, ids, reduction="none")
+    logp = torch.log_softmax(h.detach().double() @ w.double().t(), 1)[:, [3, 600]]
+    q = torch.softmax(torch.tensor([1.0, 2.0], device=DEV).double(), 0)
+    want = (q * (q.log() - logp)).sum(1)
+    smax = (h.detach().double() @ rnd(700, 128, scale=0.05).double().abs().t()).amax(1)
+    assert_within(loss, want, 2 * sum_bound(128) * smax + 2.0**-20 * (10 + smax))
