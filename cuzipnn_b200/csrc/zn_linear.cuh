@@ -8,6 +8,25 @@ namespace zn {
 
 constexpr int kNone = 0, kRelu = 1, kGelu = 2, kGeluTanh = 3, kSilu = 4;
 
+// The normal distribution's upper tail at t >= 0 over exp(-t^2 / 2): a polynomial of degree 7 in
+// u = 1 / (1 + 0.2375 t), times u (fitted here to erfcx(t / sqrt(2)) / 2 for the least relative error on
+// [0, 16]: 2^-21 in 32-bit arithmetic; beyond, both go to 0 as 1 / t).  gelu's value and derivative are
+// differences of near numbers below zero if taken from 1 + erf, which has no digits left at -5; from the
+// tail itself they keep theirs.  4096 rows of 5120 x 1280 take 143 us (158 with the derivative); erfcf in
+// its place takes 176 (217), 1 + erff 148 (174).
+__device__ __forceinline__ float mills(float t) {
+  const float u = __fdividef(1.0f, fmaf(0.2375f, t, 1.0f));
+  float p = -0.05875275f;
+  p = fmaf(p, u, 0.18125452f);
+  p = fmaf(p, u, -0.10428442f);
+  p = fmaf(p, u, 0.14710677f);
+  p = fmaf(p, u, 0.05084207f);
+  p = fmaf(p, u, 0.09489430f);
+  p = fmaf(p, u, 0.09416503f);
+  p = fmaf(p, u, 0.09477440f);
+  return p * u;
+}
+
 // act(z) and its derivative (where asked for), in 32 bits.
 template <int ACT, bool SLOPE>
 __device__ __forceinline__ float activate(float z, float& slope) {
@@ -15,8 +34,8 @@ __device__ __forceinline__ float activate(float z, float& slope) {
     if (SLOPE) slope = z > 0.0f ? 1.0f : 0.0f;
     return z < 0.0f ? 0.0f : z;  // keeps NaN
   } else if constexpr (ACT == kGelu) {
-    const float cdf = 0.5f + 0.5f * erff(0.70710678118654752f * z);
-    if (SLOPE) slope = cdf + z * 0.3989422804014327f * __expf(-0.5f * z * z);
+    const float bell = __expf(-0.5f * z * z), tail = bell * mills(fabsf(z)), cdf = z > 0.0f ? 1.0f - tail : tail;
+    if (SLOPE) slope = cdf + z * 0.3989422804014327f * bell;
     return z * cdf;
   } else if constexpr (ACT == kGeluTanh) {  // 0.5 z (1 + tanh u) = z sigmoid(2u)
     const float c = 0.7978845608028654f, z2 = z * z;

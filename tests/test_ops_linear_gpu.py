@@ -51,3 +51,30 @@ def test_bias_gradient_of_far_units():
         db, want, bound = closed_units(act, at, BF, 200, 256)
         assert_within(db, want, bound)
         assert bool((want.abs() > 8 * bound).all())  # (the bound says something)
+
+
+@pytest.mark.parametrize("at", [-4.0, -5.0, -5.5])
+@pytest.mark.parametrize("tokens", [1, 200])
+def test_bias_gradient_of_units_far_below_gelus_zero(tokens, at):
+    db, want, bound = closed_units("gelu", at, BF, tokens, 256)
+    assert_within(db, want, bound)
+    assert bool((want.abs() > 4 * bound).all())
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("act,at", [("gelu", -3.0), ("gelu", -4.5), ("gelu", -6.0), ("gelu_tanh", -4.0), ("silu", -9.0),
+                                    ("gelu", 0.0), ("gelu", 2.0)])
+@pytest.mark.parametrize("tokens,rows", [(1, 64), (40, 333)])
+def test_values_of_closed_units(act, at, tokens, rows, dtype):
+    """act(z) is off by 2^-16 of itself, by z's error (as its derivative) and by one rounding."""
+    w, blob = weight(rows, 64, dtype)
+    x = rnd(tokens, 64, dtype=dtype, scale=0.25)
+    bias = (at + 0.5 * torch.linspace(-1, 1, rows, device=DEV)).to(dtype)
+    y = z.blob_linear(x, blob, bias=bias, activation=act)
+    zz = x.double() @ w.double().t() + bias.double()
+    want = ACTS[act](zz)
+    if act == "gelu":  # 1 + erf loses digits in 64 bits too
+        want = zz * 0.5 * torch.special.erfc(-zz * 0.5**0.5)
+    ez = sum_bound(64) * (x.double().abs() @ w.double().abs().t() + bias.double().abs())
+    bound = (2.0**-16 + u_of(dtype)) * want.abs() + 1.05 * ez * act_slope(act, zz).abs() + 2.0 * ez * ez
+    assert_within(y, want, bound + (2.0**-25 if dtype == HF else 0.0))
