@@ -399,7 +399,7 @@ struct StoreSink {
 };
 
 // DotSink: the elements are rows of a weight W[rows, cols] and are multiplied with the matching
-// elements of up to kDotRows vectors x as they leave the decoder; W itself is never written.
+// elements of a vector x as they leave the decoder; W itself is never written.
 //
 // A lane's 16 elements of a round lie in one row (cols and the chunk size are multiples of 16), and
 // a row is at least one round (128 elements) long, so a segment (8 lanes, one sub-chunk) crosses at
@@ -420,37 +420,31 @@ struct StoreSink {
 template <typename T>
 struct DotSink {
   static constexpr bool kDot = true;
-  static constexpr int kRows = kDotRows;
   using Elem = T;
   const T* x;
-  int64_t ldx, rows;
-  int cols, tokens;
-  float* z;     // [tokens][rows]
-  float* part;  // [chunk][2][kDotRows]
+  int cols;
+  float* z;     // [rows]
+  float* part;  // [chunk][2]
 };
 
-template <int MT>
 struct DotState {
-  float c[MT][2];  // row lane / 4, columns 2 (lane % 4) and + 1 of each accumulator
+  float c[2];      // row lane / 4, columns 2 (lane % 4) and + 1 of the accumulator
   DotCols cols;    // the segment's place in its current row
   int row;         // the segment's current row
   bool first;      // no row end met in this sub-chunk yet
   bool mid;        // the sub-chunk starts inside a row
-  uint4 x[MT][2];  // the round's elements of x, loaded before it is decoded
+  uint4 x[2];      // the round's elements of x, loaded before it is decoded
 };
 
-// Loads the next round's elements of x (those of row 0 for rows past the last).  Lanes without elements
-// load nothing: dot_products masks what they hold.
+// Loads the next round's elements of x.  Lanes without elements load nothing: dot_products masks what
+// they hold.
 template <class Sink>
-__device__ __forceinline__ void dot_load(const Sink& k, DotState<Sink::kRows>& st, int l, bool active) {
+__device__ __forceinline__ void dot_load(const Sink& k, DotState& st, int l, bool active) {
   const int col = st.cols.next(l, active, k.cols);
   if (col < 0) return;
-#pragma unroll
-  for (int m = 0; m < Sink::kRows; ++m) {
-    const uint4* xp = reinterpret_cast<const uint4*>(k.x + (m < k.tokens ? m * k.ldx : 0) + col);
-    st.x[m][0] = __ldg(xp);
-    st.x[m][1] = __ldg(xp + 1);
-  }
+  const uint4* xp = reinterpret_cast<const uint4*>(k.x + col);
+  st.x[0] = __ldg(xp);
+  st.x[1] = __ldg(xp + 1);
 }
 
 // One step of the products: rows 0-7 of A from a0, a2, rows 8-15 zero.
@@ -468,41 +462,32 @@ __device__ __forceinline__ void dot_mma(float* c, uint32_t a0, uint32_t a2, uint
 }
 // Lanes with `use` add their products, the others nothing (both factors are zeroed: 0 * inf is NaN).
 template <class Sink, bool MASKED>
-__device__ __forceinline__ void dot_products(DotState<Sink::kRows>& st, const uint32_t* e, bool use) {
-  uint32_t w[8];
+__device__ __forceinline__ void dot_products(DotState& st, const uint32_t* e, bool use) {
+  const uint4 a = st.x[0], b = st.x[1];
+  uint32_t w[8], x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) w[i] = !MASKED || use ? e[i] : 0u;
-#pragma unroll
-  for (int m = 0; m < Sink::kRows; ++m) {
-    const uint4 a = st.x[m][0], b = st.x[m][1];
-    uint32_t x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (MASKED && !use) x[i] = 0u;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) dot_mma(st.c[m], w[2 * i], w[2 * i + 1], x[2 * i], x[2 * i + 1], typename Sink::Elem());
+  for (int i = 0; i < 8; ++i) {
+    w[i] = !MASKED || use ? e[i] : 0u;
+    if (MASKED && !use) x[i] = 0u;
   }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) dot_mma(st.c, w[2 * i], w[2 * i + 1], x[2 * i], x[2 * i + 1], typename Sink::Elem());
 }
 
-// The segment's sums (on all its lanes): its two quads' diagonal elements.
-template <int MT>
-__device__ __forceinline__ void segment_sum(const DotState<MT>& st, float* v) {
+// The segment's sum (on all its lanes): its two quads' diagonal elements.
+__device__ __forceinline__ float segment_sum(const DotState& st) {
   const int lane = threadIdx.x & 31, quad = lane >> 2;
-  const bool mine = (lane & 3) == (quad >> 1);
+  float v = (lane & 3) == (quad >> 1) ? ((quad & 1) ? st.c[1] : st.c[0]) : 0.0f;
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    v[m] = mine ? ((quad & 1) ? st.c[m][1] : st.c[m][0]) : 0.0f;
-#pragma unroll
-    for (int o = 4; o; o >>= 1) v[m] += __shfl_xor_sync(0xFFFFFFFFu, v[m], o);
-  }
+  for (int o = 4; o; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+  return v;
 }
 
 // One round of a warp's segments: 16 elements per lane (8 words), none for inactive lanes.  Called
 // by whole warps.
 template <class Sink, bool ALL>
-__device__ __forceinline__ void dot_round(const Sink& k, DotState<Sink::kRows>& st, const uint32_t* e, bool active,
-                                          int l, int seg, float* slot0) {
-  constexpr int MT = Sink::kRows;
+__device__ __forceinline__ void dot_round(const Sink& k, DotState& st, const uint32_t* e, bool active, int l, int seg,
+                                          float* slot0) {
   st.cols.advance();
   const bool wrapped = st.cols.wrapped(l, active, k.cols);  // the lane's elements lie in the next row
   const uint32_t over = __ballot_sync(0xFFFFFFFFu, wrapped);
@@ -511,19 +496,13 @@ __device__ __forceinline__ void dot_round(const Sink& k, DotState<Sink::kRows>& 
     return;
   }
   dot_products<Sink, true>(st, e, active && !wrapped);
-  float v[MT];
-  segment_sum<MT>(st, v);
+  const float v = segment_sum(st);
   if ((over >> (8 * seg)) & 0xFF) {
     if (l == 0) {
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-        if (m < k.tokens) {
-          if (st.first && st.mid) slot0[m] = v[m];
-          else k.z[m * k.rows + st.row] = v[m];
-        }
+      if (st.first && st.mid) *slot0 = v;
+      else k.z[st.row] = v;
     }
-#pragma unroll
-    for (int m = 0; m < MT; ++m) st.c[m][0] = st.c[m][1] = 0.0f;
+    st.c[0] = st.c[1] = 0.0f;
     st.first = false;
     ++st.row;
     st.cols.wrap(k.cols);
@@ -536,36 +515,27 @@ __device__ __forceinline__ void dot_round(const Sink& k, DotState<Sink::kRows>& 
 template <class Sink>
 __device__ __forceinline__ void dot_finish_chunk(const Sink& k, int64_t j, int64_t g0, int64_t g1, int64_t sc,
                                                  const float* slots, bool bad) {
-  constexpr int MT = Sink::kRows;
   const int64_t r0 = g0 / k.cols, r1 = (g1 - 1) / k.cols;
   for (int64_t row = r0 + threadIdx.x; row <= r1; row += kDecThreads) {
     const int64_t lo = row * k.cols, hi = lo + k.cols;
     const bool starts = lo >= g0, complete = starts && hi <= g1;
     const int sa = int((max(lo, g0) - g0) / sc), sb = int((min(hi, g1) - 1 - g0) / sc);
     if (sa == sb && complete && !bad) continue;
-    float v[MT];
-#pragma unroll
-    for (int m = 0; m < MT; ++m) v[m] = 0.0f;
+    float v = 0.0f;
     if (!bad)
       for (int s = sa; s <= sb; ++s) {
         const int64_t s0 = g0 + s * sc, s1 = min(s0 + sc, g1);
-        const float* p = slots + (2 * s + (lo >= s0 && hi > s1 ? 1 : 0)) * MT;
-#pragma unroll
-        for (int m = 0; m < MT; ++m) v[m] += p[m];
+        v += slots[2 * s + (lo >= s0 && hi > s1 ? 1 : 0)];
       }
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-      if (m < k.tokens) {
-        if (complete) k.z[m * k.rows + row] = v[m];
-        else k.part[(2 * j + starts) * kDotRows + m] = v[m];
-      }
+    if (complete) k.z[row] = v;
+    else k.part[2 * j + starts] = v;
   }
 }
 
 // Offset (with kCodedBit, or -1) of the units of chunk j of a weight, by the whole CTA from the blob's
 // tables: what dscan_kernel computes for all units at once, with the same checks.  It reads the
 // tables up to the chunk's second unit (12 bytes per chunk of the blob, from L2 but for the first
-// CTA), so it pays for weights of up to kDirectChunks chunks, whose launch it saves.
+// CTA), so it pays for small weights (weight_direct), whose launch it saves.
 __device__ __forceinline__ void find_units(const DecArgs& a, int64_t j, DecSmem& S, int64_t* unit, bool* bad) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid < 2) S.coded[tid] = 0;
@@ -635,7 +605,7 @@ __device__ __forceinline__ void decode_chunk(const DecArgs& a, int64_t j, bool o
   DecSmem& S = *reinterpret_cast<DecSmem*>(smem_raw + KC * kM * 4 + KC * kChains * kRing * kDecThreads * sizeof(Slot));
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   static_assert(!Sink::kDot || (K == 2 && kChains == 1), "products take 16-bit elements, one chain per lane");
-  [[maybe_unused]] float* slots = reinterpret_cast<float*>(&S + 1);  // DotSink: [64 sub-chunks][2][MT]
+  [[maybe_unused]] float* slots = reinterpret_cast<float*>(&S + 1);  // DotSink: [64 sub-chunks][2]
   if (overflow_pass && !a.overflow[j]) return;
   const bool batched = a.in_ptrs != nullptr;
   int64_t m;
@@ -648,7 +618,7 @@ __device__ __forceinline__ void decode_chunk(const DecArgs& a, int64_t j, bool o
     outc = a.out + j * a.C * K;
   }
   if constexpr (Sink::kDot)
-    for (int i = tid; i < 64 * 2 * Sink::kRows; i += kDecThreads) slots[i] = 0.0f;
+    for (int i = tid; i < 64 * 2; i += kDecThreads) slots[i] = 0.0f;
   int flags = 0;  // weights: error bits of this chunk
   [[maybe_unused]] int64_t unit[2] = {-1, -1};
   if constexpr (WEIGHT)
@@ -812,7 +782,7 @@ __device__ __forceinline__ void decode_chunk(const DecArgs& a, int64_t j, bool o
     int r = 0;
     [[maybe_unused]] auto dot = [&] {
       if constexpr (Sink::kDot) {
-        DotState<Sink::kRows> st{};
+        DotState st{};
         const int64_t e0 = j * a.C + base[0];
         st.row = int(e0 / sink.cols);
         const int c0 = int(e0 - int64_t(st.row) * sink.cols);
@@ -825,7 +795,7 @@ __device__ __forceinline__ void decode_chunk(const DecArgs& a, int64_t j, bool o
       }
     }();
     [[maybe_unused]] float* slot0 = nullptr;
-    if constexpr (Sink::kDot) slot0 = slots + 2 * min(gi[0], 63) * Sink::kRows;
+    if constexpr (Sink::kDot) slot0 = slots + 2 * min(gi[0], 63);
     if constexpr (KC == 1) {
       // Full rounds (all 16 steps of every chain's state valid): no per-step predication, 32-bit
       // bookkeeping and running element offsets; the partial rounds at the end of a sub-chunk
@@ -1029,18 +999,13 @@ __device__ __forceinline__ void decode_chunk(const DecArgs& a, int64_t j, bool o
       for (int c = 0; c < kChains; ++c)
         if (q < ncoded && valid[c]) err |= (cur[q][c].x != kL) || (cur[q][c].ptr != cur[q][c].end);
     if constexpr (Sink::kDot) {
-      float sum[Sink::kRows];
-      segment_sum<Sink::kRows>(dot, sum);
+      const float sum = segment_sum(dot);
       if (valid[0]) {  // the row that the sub-chunk ends in
         const int64_t e1 = j * a.C + base[0] + len[0];
         const bool ended = e1 % sink.cols == 0, here = !(dot.first && dot.mid);
         if (l == 0) {
-#pragma unroll
-          for (int mm = 0; mm < Sink::kRows; ++mm)
-            if (mm < sink.tokens) {
-              if (ended && here) sink.z[mm * sink.rows + dot.row] = sum[mm];
-              else slot0[(here ? Sink::kRows : 0) + mm] = sum[mm];
-            }
+          if (ended && here) sink.z[dot.row] = sum;
+          else slot0[here ? 1 : 0] = sum;
         }
       }
     }

@@ -242,19 +242,19 @@ struct EpiLinear {
   };
 };
 
-// z[t, r] of weight_dot: from z, or the parts of a row that spans chunks, in order.
+// z[r] of weight_dot: from z, or the parts of a row that spans chunks, in order.
 struct DotValue {
   const float* z;
   const float* part;
   int64_t rows, cols, chunk;
-  __device__ __forceinline__ float get(int64_t t, int64_t r) const {
+  __device__ __forceinline__ float get(int64_t r) const {
     // The chunk of the row's first element, and how many more the row reaches into (32 bits: a chunk has
     // 2^24 elements at most, dot_shape's rows fewer than 2^30).
     const int64_t c0 = r * cols / chunk;
     const uint32_t more = (uint32_t(r * cols - c0 * chunk) + uint32_t(cols) - 1) / uint32_t(chunk);
-    if (more == 0) return z[t * rows + r];
-    float v = part[(2 * c0 + 1) * kDotRows + t];
-    for (int64_t c = c0 + 1; c <= c0 + more; ++c) v += part[2 * c * kDotRows + t];
+    if (more == 0) return z[r];
+    float v = part[2 * c0 + 1];
+    for (int64_t c = c0 + 1; c <= c0 + more; ++c) v += part[2 * c];
     return v;
   }
 };
@@ -273,7 +273,7 @@ __device__ __forceinline__ void finish_value(const EpiLinear<T>& e, int64_t m, i
 // y = act(z + bias) + residual from z = acc, or from weight_dot.
 template <typename T>
 struct Finish {
-  const float* acc;  // [M][ld], or null: dot
+  const float* acc;  // [M][ld], or null: dot (M = 1)
   int64_t M, N, ld;
   DotValue dot;
   EpiLinear<T> lin;
@@ -282,12 +282,12 @@ struct Finish {
 template <typename T>
 __device__ __forceinline__ void finish_element(const Finish<T>& f, int64_t i) {
   const int64_t m = i / f.N, n = i - m * f.N;
-  finish_value(f.lin, m, n, f.acc ? f.acc[m * f.ld + n] : f.dot.get(m, n));
+  finish_value(f.lin, m, n, f.acc ? f.acc[m * f.ld + n] : f.dot.get(n));
 }
 
 // weight_dot, then f (whose dot it fills in) on every element.
 template <typename T>
-int weight_linear(const WeightBlob& w, void* temp, const void* x, int64_t ldx, int tokens, float* z, float* part,
-                  const Finish<T>& f, int32_t* status, cudaStream_t s);
+int weight_linear(const WeightBlob& w, void* temp, const void* x, float* z, float* part, const Finish<T>& f,
+                  int32_t* status, cudaStream_t s);
 
 }  // namespace zn

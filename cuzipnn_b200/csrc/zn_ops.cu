@@ -7,7 +7,7 @@
 //   linear              y = act(x W^T + b) + r                   EpiLinear
 //   loss                running maximum and sum of exp           EpiStats (per row and half tile)
 //   loss and gradient   P = exp(s - r), one piece wide           EpiSoft, then acc += P W by EpiAccum
-// A product with at most kDotRows rows is bound by decoding; it runs inside the decoder instead
+// A product with one row is bound by decoding; it runs inside the decoder instead
 // (weight_dot) and W is never written at all.
 //
 // Losses.  With s = h W^T / T, lse = log sum_v exp s_v and a sparse distribution q over the ids of
@@ -554,25 +554,23 @@ __global__ void __launch_bounds__(128) loss_prep_kernel(const int64_t* ids, cons
   }
 }
 
-// Statistics of the logits of weight_dot: a block per (column tile of kStatCols, token).  A thread's
-// columns are a chain of divisions and loads each, so the tiles are small: 27000 columns take 4.8 us in
-// tiles of 512 and 12.3 in tiles of 2048.
+// Statistics of the logits of weight_dot: a block per column tile of kStatCols.  A thread's columns are a
+// chain of divisions and loads each, so the tiles are small: 27000 columns take 4.8 us in tiles of 512 and
+// 12.3 in tiles of 2048.
 constexpr int kStatCols = 512;
-__global__ void __launch_bounds__(256) dot_stats_kernel(DotValue v, LossRows rows, float* part, int64_t tokens,
-                                                        float scale) {
+__global__ void __launch_bounds__(256) dot_stats_kernel(DotValue v, LossRows rows, float* part, float scale) {
   pdl_wait();
   pdl_trigger();
-  const int64_t m = blockIdx.y, n0 = int64_t(blockIdx.x) * kStatCols;
-  const int64_t n1 = min(v.rows, n0 + kStatCols);
-  const int count = rows.count[m];
-  const int32_t* ids = rows.ids + m * rows.top;
-  const float* q = rows.q + m * rows.top;
+  const int64_t n0 = int64_t(blockIdx.x) * kStatCols, n1 = min(v.rows, n0 + kStatCols);
+  const int count = rows.count[0];
+  const int32_t* ids = rows.ids;
+  const float* q = rows.q;
   constexpr int kPer = kStatCols / 256;
   float s[kPer], mx = -INFINITY;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int64_t n = n0 + threadIdx.x + 256 * i;
-    s[i] = n < n1 ? v.get(m, n) * scale : -INFINITY;
+    s[i] = n < n1 ? v.get(n) * scale : -INFINITY;
     mx = fmaxf(mx, s[i]);
   }
   const float base = mx == -INFINITY ? 0.0f : mx;
@@ -596,10 +594,10 @@ __global__ void __launch_bounds__(256) dot_stats_kernel(DotValue v, LossRows row
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int i = 1; i < 8; ++i) stats_join(st, sm[i].mx, sm[i].sum, sm[i].hit);
-    float* p = part + int64_t(blockIdx.x) * 3 * tokens + m;
+    float* p = part + int64_t(blockIdx.x) * 3;
     p[0] = st.mx;
-    p[tokens] = st.sum;
-    p[2 * tokens] = st.hit;
+    p[1] = st.sum;
+    p[2] = st.hit;
   }
 }
 
@@ -1102,7 +1100,7 @@ int plan_linear(const zn_weight* w, const void* x, int64_t ldx, int64_t tokens, 
     p->w.b.direct = weight_direct(p->w.b, 1);
     p->w.status = status;
     p->w.temp = ar.take(weight_temp_bytes(p->w.b));
-    p->acc = ar.take<float>(size_t(tokens) * w->rows * 4);
+    p->acc = ar.take<float>(size_t(w->rows) * 4);
     p->part = ar.take<float>(dot_part_bytes(p->w.b));
     return ZN_OK;
   }
@@ -1144,7 +1142,7 @@ int run_linear(const LinearPlan& p, const void* x, int64_t ldx, int64_t tokens, 
     if (int rc = copy_pitch(x_job, s)) return rc;
     f.N = rows;
     f.lin = linear_epilogue<T>(bias, res, ldr, y, slope, rows, tokens, 0, rows, act);
-    return weight_linear<T>(p.w.b, p.w.temp, xm.p, xm.pitch, int(tokens), p.acc, p.part, f, p.w.status, s);
+    return weight_linear<T>(p.w.b, p.w.temp, xm.p, p.acc, p.part, f, p.w.status, s);
   }
   for (int64_t r0 = 0; r0 < rows; r0 += p.w.piece_rows) {
     const int64_t r1 = std::min(rows, r0 + p.w.piece_rows);
@@ -1274,7 +1272,7 @@ int plan_loss(const zn_weight* w, const void* x, int64_t ldx, int64_t tokens, in
     p->w.b.direct = weight_direct(p->w.b, 1);
     p->w.status = status;
     p->w.temp = ar.take(weight_temp_bytes(p->w.b));
-    p->z = ar.take<float>(size_t(tokens) * w->rows * 4);
+    p->z = ar.take<float>(size_t(w->rows) * 4);
     p->z_part = ar.take<float>(dot_part_bytes(p->w.b));
     p->tiles = cdiv(w->rows, kStatCols);
   } else {
@@ -1300,10 +1298,10 @@ int run_loss(const LossPlan& p, const void* x, int64_t ldx, int64_t tokens, cons
   const Matrix xm = load_matrix(x, tokens, cols, ldx, p.x_copy, &x_job);
   if (p.dot) {
     if (int rc = copy_pitch(x_job, s)) return rc;
-    if (int rc = weight_dot(p.w.b, p.w.temp, xm.p, xm.pitch, int(tokens), p.z, p.z_part, p.w.status, s)) return rc;
+    if (int rc = weight_dot(p.w.b, p.w.temp, xm.p, p.z, p.z_part, p.w.status, s)) return rc;
     const DotValue v{p.z, p.z_part, vocab, cols, p.w.b.chunk};
-    if (int rc = launch_after(dot_stats_kernel, dim3(unsigned(p.tiles), unsigned(tokens)), 256, 0, s, "dot_stats_kernel",
-                              v, rows, p.part, tokens, kLog2e * inv_t))
+    if (int rc = launch_after(dot_stats_kernel, dim3(unsigned(p.tiles)), 256, 0, s, "dot_stats_kernel", v, rows, p.part,
+                              kLog2e * inv_t))
       return rc;
   } else {
     for (int64_t r0 = 0; r0 < vocab; r0 += p.w.piece_rows) {

@@ -1,5 +1,5 @@
 // Weights as operands (zn_weight.cuh): ranges of a blob's chunks decoded into a buffer, or multiplied
-// with a few vectors inside the decoder.
+// with a vector inside the decoder.
 #include "zn_decode.cuh"
 #include "zn_linear.cuh"
 
@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(kDecThreads) weight_tail_kernel(const __grid_c
 
 template <class Sink>
 constexpr size_t sink_smem() {
-  if constexpr (Sink::kDot) return 64 * 2 * Sink::kRows * sizeof(float);
+  if constexpr (Sink::kDot) return 64 * 2 * sizeof(float);
   else return 0;
 }
 
@@ -135,9 +135,9 @@ int launch_weight(const DecArgs& a, int64_t c0, int64_t c1, const Sink& sink, co
 }
 
 template <typename T, bool REORDER, class Fin>
-int launch_dot(const DecArgs& a, const WeightBlob& w, const void* x, int64_t ldx, int tokens, float* z, float* part,
-               const Fin& fin, int64_t work, cudaStream_t s) {
-  const DotSink<T> k{static_cast<const T*>(x), ldx, w.rows, int(w.cols), tokens, z, part};
+int launch_dot(const DecArgs& a, const WeightBlob& w, const void* x, float* z, float* part, const Fin& fin, int64_t work,
+               cudaStream_t s) {
+  const DotSink<T> k{static_cast<const T*>(x), int(w.cols), z, part};
   return launch_weight<REORDER>(a, 0, a.nch, k, fin, work, s);
 }
 
@@ -165,26 +165,25 @@ int weight_wave(const WeightBlob& w, int64_t* chunks) {
   return ZN_OK;
 }
 
-size_t dot_part_bytes(const WeightBlob& w) { return size_t(weight_chunks(w)) * 2 * kDotRows * sizeof(float); }
+size_t dot_part_bytes(const WeightBlob& w) { return size_t(weight_chunks(w)) * 2 * sizeof(float); }
 
-int weight_dot(const WeightBlob& w, void* temp, const void* x, int64_t ldx, int tokens, float* z, float* part,
-               int32_t* status, cudaStream_t s) {
+int weight_dot(const WeightBlob& w, void* temp, const void* x, float* z, float* part, int32_t* status, cudaStream_t s) {
   const DecArgs a = weight_args(w, temp, status, w.direct ? kDirect : kScanned);
-  return w.bf16 ? launch_dot<__nv_bfloat16, true>(a, w, x, ldx, tokens, z, part, NoFin(), 0, s)
-                : launch_dot<__half, false>(a, w, x, ldx, tokens, z, part, NoFin(), 0, s);
+  return w.bf16 ? launch_dot<__nv_bfloat16, true>(a, w, x, z, part, NoFin(), 0, s)
+                : launch_dot<__half, false>(a, w, x, z, part, NoFin(), 0, s);
 }
 
 template <typename T>
-int weight_linear(const WeightBlob& w, void* temp, const void* x, int64_t ldx, int tokens, float* z, float* part,
-                  const Finish<T>& f, int32_t* status, cudaStream_t s) {
+int weight_linear(const WeightBlob& w, void* temp, const void* x, float* z, float* part, const Finish<T>& f,
+                  int32_t* status, cudaStream_t s) {
   const DecArgs a = weight_args(w, temp, status, w.direct ? kDirect : kScanned);
   LinearFin<T> fin{f};
   fin.f.dot = {z, part, w.rows, w.cols, w.chunk};
-  return launch_dot<T, Num<T>::kCode == 1>(a, w, x, ldx, tokens, z, part, fin, f.M * f.N, s);
+  return launch_dot<T, Num<T>::kCode == 1>(a, w, x, z, part, fin, f.N, s);
 }
-template int weight_linear<__nv_bfloat16>(const WeightBlob&, void*, const void*, int64_t, int, float*, float*,
+template int weight_linear<__nv_bfloat16>(const WeightBlob&, void*, const void*, float*, float*,
                                           const Finish<__nv_bfloat16>&, int32_t*, cudaStream_t);
-template int weight_linear<__half>(const WeightBlob&, void*, const void*, int64_t, int, float*, float*,
-                                   const Finish<__half>&, int32_t*, cudaStream_t);
+template int weight_linear<__half>(const WeightBlob&, void*, const void*, float*, float*, const Finish<__half>&, int32_t*,
+                                   cudaStream_t);
 
 }  // namespace zn

@@ -1,6 +1,6 @@
 // A compressed weight as the operand of a product: a rows x cols matrix of 16-bit floats held as a
 // blob (the non-stored layout), decoded a range of chunks at a time into a caller's buffer, or
-// multiplied with a few vectors inside the decoder.  Implemented in zn_weight.cu (weight_scan in zn_decode.cu).
+// multiplied with a vector inside the decoder.  Implemented in zn_weight.cu (weight_scan in zn_decode.cu).
 #pragma once
 
 #include "zn_common.cuh"
@@ -16,14 +16,12 @@ struct WeightBlob {
   bool direct;    // every chunk finds its units itself, without weight_scan (weight_direct)
 };
 
-// Rows of one product inside the decoder, and the shape rule of that path (see DotSink).  Measured over
-// 152064 x 3584 (128 Ki chunks), in the decoder with 1, 2 and 4 rows 689, 1016 and 1141 us (a second
-// row's registers cost a fifth of the decoder's occupancy), against 1000 us for decoding and a product
+// Whether a product runs inside the decoder (see DotSink): that of one token.  Measured over 152064 x 3584
+// (128 Ki chunks) with a form for several, 1, 2 and 4 tokens took 689, 1016 and 1141 us there (a second
+// token's registers cost a fifth of the decoder's occupancy), against 1000 us for decoding and a product
 // of any number up to 128; over 3584 x 3584 (16 Ki) 51, 52 and 57 us against 54.
-constexpr int kDotRows = 1;
 inline bool dot_shape(int64_t tokens, int64_t cols, int64_t chunk) {
-  return tokens >= 1 && tokens <= kDotRows && cols % 16 == 0 && cols >= kRound && cols < (int64_t(1) << 30) &&
-         chunk % 16 == 0;
+  return tokens == 1 && cols % 16 == 0 && cols >= kRound && cols < (int64_t(1) << 30) && chunk % 16 == 0;
 }
 
 inline int64_t weight_chunks(const WeightBlob& w) { return cdiv(w.rows * w.cols, w.chunk); }
@@ -85,13 +83,11 @@ int weight_decode(const WeightBlob& w, void* temp, int64_t c0, int64_t c1, void*
 // Chunks that the decoder works on at once on this device (its resident blocks).
 int weight_wave(const WeightBlob& w, int64_t* chunks);
 
-// Product inside the decoder: z[t, r] = sum_c x[t, c] * W[r, c] for tokens <= kDotRows rows of x
-// (16-bit, 16-byte aligned, pitch ldx a multiple of 8).  Rows that lie in one chunk go to z (pitch
-// w.rows); the parts of rows that span chunks go to `part` ([chunk][2][kDotRows], dot_part_bytes):
-// slot 1 holds the part of a row that starts in the chunk, slot 0 of one that started before it.
+// Product inside the decoder: z[r] = sum_c x[c] * W[r, c] (x 16-bit, 16-byte aligned).  Rows that lie in one
+// chunk go to z; the parts of rows that span chunks go to `part` ([chunk][2], dot_part_bytes): slot 1
+// holds the part of a row that starts in the chunk, slot 0 of one that started before it.
 size_t dot_part_bytes(const WeightBlob& w);
 // Without w.direct, weight_scan comes first.
-int weight_dot(const WeightBlob& w, void* temp, const void* x, int64_t ldx, int tokens, float* z, float* part,
-               int32_t* status, cudaStream_t s);
+int weight_dot(const WeightBlob& w, void* temp, const void* x, float* z, float* part, int32_t* status, cudaStream_t s);
 
 }  // namespace zn
