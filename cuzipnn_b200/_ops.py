@@ -386,5 +386,9 @@ def blob_distillation(
     if teacher_logits.device != w.device:
         raise ValueError(f"teacher_logits is on {teacher_logits.device}, hidden on {w.device}")
     ids = teacher_ids.detach().reshape(-1, top).contiguous()
-    logits = teacher_logits.detach().reshape(-1, top).float().contiguous()
+    logits = teacher_logits.detach().reshape(-1, top)
+    if logits.dtype == torch.float64:  # less their maximum first, or 32 bits would lose the small differences of large ones
+        peak = logits.masked_fill(ids < 0, -math.inf).amax(1, keepdim=True)
+        logits = logits - torch.where(peak.isfinite(), peak, 0.0)
+    logits = logits.float().contiguous()
     return _loss(hidden, w, ids, logits, top, 0, temperature, reduction, shape)

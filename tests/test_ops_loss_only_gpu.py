@@ -135,3 +135,27 @@ def test_infinite_logit_that_the_teacher_excludes(tokens, grad):
     want = (q * (q.log() - logp)).sum(1)
     smax = (h.detach().double() @ rnd(700, 128, scale=0.05).double().abs().t()).amax(1)
     assert_within(loss, want, 2 * sum_bound(128) * smax + 2.0**-20 * (10 + smax))
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_teacher_logits_in_64_bits(grad):
+    """Large ones with small differences, and entries masked by the type's lowest value, all of a row's
+    among them (uniform then, as in any other type)."""
+    w, blob = weight(700, 128, BF)
+    ids, _ = teacher(8, 700, 5)
+    ids[:, 0] = torch.arange(8, device=DEV)
+    logits = torch.randn((8, 5), device=DEV, dtype=torch.double, generator=torch.Generator(device=DEV).manual_seed(2)) + 3e9
+    low = torch.finfo(torch.double).min
+    logits[1] = low
+    logits[2, 1:] = low
+    logits[3, 2] = -math.inf
+    logits[4] = -math.inf
+    logits[5] = 1e300
+    logits[6, 0] = -1e300
+    q, counts = distribution(ids, logits, 1.0)
+    assert bool(counts[1]) and not bool(counts[4])
+    h = rnd(8, 128)
+    want, *_, lse = reference_loss(h, w, ids, q, counts, 1.0, "none")
+    smax = (h.double().abs() @ w.double().abs().t()).amax(1)
+    loss = z.blob_distillation(h.requires_grad_(grad), blob, logits, ids, reduction="none")
+    assert_within(loss, want, torch.where(counts, 2 * sum_bound(128) * smax + 2.0**-20 * (10 + smax), 0.0))
