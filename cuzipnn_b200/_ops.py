@@ -344,8 +344,11 @@ def blob_cross_entropy(
     w = _Weight(blob, hidden, "hidden")
     shape = tuple(hidden.shape[:-1])
     _check_ids("targets", targets, shape, w)
+    ignore_index = int(ignore_index)
+    if not -(1 << 63) <= ignore_index < 1 << 63:
+        raise ValueError(f"ignore_index must be an int64, not {ignore_index}")
     ids = targets.detach().reshape(-1).contiguous()
-    return _loss(hidden, w, ids, None, 1, int(ignore_index), 1.0, reduction, shape)
+    return _loss(hidden, w, ids, None, 1, ignore_index, 1.0, reduction, shape)
 
 
 def blob_distillation(
