@@ -441,7 +441,7 @@ def _parse_header(prefix: Buffer, off: int = 0, length: int | None = None
 
 
 # Status words of the calling thread's latest decompress call per device (0 = no decoding error): a
-# tensor, or a tuple of them.  Per thread, so that threads decoding on one device do not overwrite each
+# tensor, or one and how many of its words are set.  Per thread, so that threads decoding on one device do not overwrite each
 # other's status.
 _STATUS = threading.local()
 
@@ -452,7 +452,7 @@ def _statuses() -> dict:
     return _STATUS.by_dev
 
 
-def _set_status(device: torch.device, status: torch.Tensor) -> None:
+def _set_status(device: torch.device, status: torch.Tensor | tuple[torch.Tensor, int]) -> None:
     _statuses()[device.index] = status
 
 
@@ -467,10 +467,10 @@ def last_decode_status(device: torch.device | str | int | None = None) -> int:
     st = getattr(_STATUS, "by_dev", {}).get(dev.index if dev.type == "cuda" else int(dev))
     if st is None:
         return 0
+    st = st[0][: st[1]] if isinstance(st, tuple) else st
     bits = 0
-    for words in st if isinstance(st, tuple) else (st,):
-        for v in words.cpu().tolist():  # one word per blob of the latest call: OR them
-            bits |= int(v)
+    for v in st.cpu().tolist():  # one word per blob of the latest call: OR them
+        bits |= int(v)
     return bits
 
 

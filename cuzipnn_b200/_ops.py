@@ -19,7 +19,7 @@ import ctypes
 import math
 
 import torch
-from torch.autograd.forward_ad import unpack_dual
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -119,14 +119,15 @@ class _Weight:
                 self.blob = b = b.clone(memory_format=torch.contiguous_format)
         self.desc = _lib.Weight(b.data_ptr(), b.numel(), self.rows, self.cols, self.chunk_bytes, _CODES[self.dtype])
 
-    def call(self, name: str, query: tuple, args: tuple, status: torch.Tensor) -> None:
+    def call(self, name: str, query: tuple, args: tuple, status: int) -> None:
         """Run entry point `name` on the device's current stream: scratch from <name>_temp_bytes
-        (with the `query` arguments), then (weight, *args, status, scratch, stream)."""
+        (with the `query` arguments), then (weight, *args, status, scratch, stream).  `status`: the
+        address of its status word."""
         w = ctypes.byref(self.desc)
         temp_bytes, run = _ENTRIES[name]
         nbytes = temp_bytes(w, *query)
         temp = torch.empty(nbytes or 1, dtype=torch.uint8, device=self.device)
-        status_code = run(w, *args, status.data_ptr(), temp.data_ptr(), nbytes, _stream(self.device))
+        status_code = run(w, *args, status, temp.data_ptr(), nbytes, _stream(self.device))
         if status_code:
             _lib.check(status_code, name)
 
@@ -149,7 +150,7 @@ def _ptr(t: torch.Tensor | None) -> int | None:
 
 def _check_tangent(name: str, t: torch.Tensor) -> None:
     """Operands with a forward-mode tangent: they need no gradient, so the tangent would be lost."""
-    if unpack_dual(t).tangent is not None:
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
         raise NotImplementedError(f"{name} carries a forward-mode derivative: operators on blobs have none")
 
 
@@ -162,7 +163,7 @@ def _linear_forward(w: _Weight, x, shape, bias, act: int, residual, want_slope: 
     tokens = x2.shape[0]
     if tokens:
         w.call("zn_linear", (x2.data_ptr(), ldx, tokens),
-               (x2.data_ptr(), ldx, tokens, _ptr(b), act, _ptr(r2), ldr, y.data_ptr(), _ptr(slope)), status)
+               (x2.data_ptr(), ldx, tokens, _ptr(b), act, _ptr(r2), ldr, y.data_ptr(), _ptr(slope)), status.data_ptr())
     else:
         status.zero_()
     return y, slope
@@ -171,10 +172,10 @@ def _linear_forward(w: _Weight, x, shape, bias, act: int, residual, want_slope: 
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, blob, bias, residual, w, shape, act):
-        status = torch.empty(1, dtype=torch.int32, device=w.device)
+        status = torch.empty(2, dtype=torch.int32, device=w.device)  # of this pass, and of the backward pass
         want = act != 0 and (ctx.needs_input_grad[0] or ctx.needs_input_grad[2])
         y, slope = _linear_forward(w, x, shape, bias, act, residual, want, status)
-        _set_status(w.device, status)
+        _set_status(w.device, (status, 1))
         ctx.w, ctx.status, ctx.statuses, ctx.x_shape = w, status, _statuses(), x.shape
         ctx.save_for_backward(blob, slope)  # the blob: an in-place change before backward raises
         return y
@@ -192,12 +193,12 @@ class _Linear(torch.autograd.Function):
         if need_x or need_b:
             with _on(w.device):
                 g, ldy = _rows(dy, w.rows)
-                status = torch.empty(1, dtype=torch.int32, device=w.device)
                 w.call("zn_linear_grad",
                        (g.data_ptr(), ldy, g.shape[0], int(slope is not None), int(need_x), int(need_b)),
-                       (g.data_ptr(), ldy, g.shape[0], _ptr(slope), _ptr(dx), _ptr(db)), status)
+                       (g.data_ptr(), ldy, g.shape[0], _ptr(slope), _ptr(dx), _ptr(db)),
+                       ctx.status.data_ptr() + 4)
                 if need_x:  # it decoded; the engine's thread reports to the one that called the layer
-                    ctx.statuses[w.device.index] = (ctx.status, status)
+                    ctx.statuses[w.device.index] = (ctx.status, 2)
         return dx, None, db, dy if need_r else None, None, None, None
 
 
@@ -257,7 +258,7 @@ def _loss_forward(w: _Weight, hidden, ids, logits, top, ignore_index, temperatur
     if tokens:
         w.call("zn_loss", (h.data_ptr(), ldh, tokens, top, int(want_grad)),
                (h.data_ptr(), ldh, tokens, ids.data_ptr(), _ptr(logits), top, ignore_index, temperature, reduction,
-                loss.data_ptr(), _ptr(unit), state.data_ptr()), status)
+                loss.data_ptr(), _ptr(unit), state.data_ptr()), status.data_ptr())
     else:
         loss.zero_()
         status.zero_()
