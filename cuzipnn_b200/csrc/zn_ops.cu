@@ -383,10 +383,10 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Fin
   for (int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += step) finish_element(f, i);
 }
 
-// dz = dy * slope in 16 bits (the operand of dx = dz W; dz null: not wanted) and the column sums of
-// the unrounded products over `per` rows per block: to dbias when that is all rows (one launch less
+// dz = dy * slope in 16 bits (the operand of dx = dz W, as the gradient between two layers would be; the
+// tensor cores take no 32-bit one at this rate; dz null: not wanted) and the column sums of the unrounded products over `per` rows per block: to dbias when that is all rows (one launch less
 // for a few tokens), else to part[row block][n] (32 bits), which column_sum_kernel adds in order.
-// V columns per thread: 8 in 16-byte accesses, four rows in flight, where the matrices allow it (72 us
+// V columns per thread: 8 in 16-byte accesses, four rows in flight, where the matrices allow it (70 us
 // for 4096 x 18944, the bandwidth of its 465 MB), else 1.
 constexpr int kSumRows = 64, kSumAll = 512;
 template <typename T, int V>
@@ -682,8 +682,8 @@ __global__ void __launch_bounds__(1024) soft_rows_kernel(const float* part, int6
 
 // The terms of a row's ids in this piece: acc += 2^(s'_k - r) W[id_k], acc_q += q_k W[id_k], in 32 bits,
 // or for a row of a single id acc_q = W[id] (soft_end_kernel knows its factor); and the sums of the groups
-// that were multiplied again.  One CTA per row.  2048 rows of 3584 with one id each take 28 us (132 MB,
-// 4.7 TB/s), beside 640 us of products for a piece of 27000 rows.
+// that were multiplied again.  One CTA per row.  4096 rows of 3584 with one id each take 10 us in each of
+// three pieces, beside 2000 us of products; 2048 rows of 2560 with 32 ids 75 us in each of two, beside 860.
 template <typename T>
 __global__ void __launch_bounds__(128) gather_kernel(LossRows rows, SoftRows soft, const T* w, int64_t pitch,
                                                      int64_t v0, int64_t v1, int64_t cols, float* acc, float* acc_q,
