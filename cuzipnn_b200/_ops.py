@@ -339,8 +339,9 @@ def blob_cross_entropy(
     Differentiable in hidden: where hidden requires a gradient, the forward pass computes it with the
     loss, in the same pass over the vocabulary, a piece at a time, and keeps it in 32 bits (tokens x
     cols).  The softmax's weights are rounded to the dtype before the product with a piece, except
-    at the row's own target (sums are in 32 bits); ignored rows get zero gradients whatever they
-    hold."""
+    at the row's own target (sums are in 32 bits), where softmax - 1 is taken from the other weights'
+    sum, so that confident rows are as exact as others; in float16, weights below about 2^-33 of the
+    largest vanish.  Ignored rows get zero gradients whatever they hold."""
     _check_reduction(reduction)
     w = _Weight(blob, hidden, "hidden")
     shape = tuple(hidden.shape[:-1])

@@ -383,9 +383,10 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Fin
   for (int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += step) finish_element(f, i);
 }
 
-// dz = dy * slope in 16 bits (the operand of dx = dz W, as the gradient between two layers would be; the
-// tensor cores take no 32-bit one at this rate; dz null: not wanted) and the column sums of the unrounded products over `per` rows per block: to dbias when that is all rows (one launch less
-// for a few tokens), else to part[row block][n] (32 bits), which column_sum_kernel adds in order.
+// dz = dy * slope in 16 bits (the operand of dx = dz W, as the gradient between two layers would be: the
+// tensor cores take no 32-bit one at this rate; dz null: not wanted) and the column sums of the unrounded
+// products over `per` rows per block: to dbias when that is all rows (one launch less for a few tokens),
+// else to part[row block][n] (32 bits), which column_sum_kernel adds in order.
 // V columns per thread: 8 in 16-byte accesses, four rows in flight, where the matrices allow it (70 us
 // for 4096 x 18944, the bandwidth of its 465 MB), else 1.
 constexpr int kSumRows = 64, kSumAll = 512;
