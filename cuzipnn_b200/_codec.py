@@ -441,7 +441,7 @@ def _parse_header(prefix: Buffer, off: int = 0, length: int | None = None
 
 
 # Status words of the calling thread's latest decompress call per device (0 = no decoding error): a
-# tensor, or one and how many of its words are set.  Per thread, so that threads decoding on one device do not overwrite each
+# tensor, how many of its words are set (None: all), and the stream they are set on.  Per thread, so that threads decoding on one device do not overwrite each
 # other's status.
 _STATUS = threading.local()
 
@@ -452,8 +452,8 @@ def _statuses() -> dict:
     return _STATUS.by_dev
 
 
-def _set_status(device: torch.device, status: torch.Tensor | tuple[torch.Tensor, int]) -> None:
-    _statuses()[device.index] = status
+def _set_status(device: torch.device, status: torch.Tensor, words: int | None = None) -> None:
+    _statuses()[device.index] = (status, words, _stream(device))
 
 
 def last_decode_status(device: torch.device | str | int | None = None) -> int:
@@ -464,12 +464,14 @@ def last_decode_status(device: torch.device | str | int | None = None) -> int:
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     if dev.type == "cuda" and dev.index is None:
         dev = torch.device("cuda", torch.cuda.current_device())
-    st = getattr(_STATUS, "by_dev", {}).get(dev.index if dev.type == "cuda" else int(dev))
-    if st is None:
+    latest = _statuses().get(dev.index if dev.type == "cuda" else int(dev))
+    if latest is None:
         return 0
-    st = st[0][: st[1]] if isinstance(st, tuple) else st
+    st, words, stream = latest
+    if stream != _stream(st.device):  # another stream than the call's: the copy below would not wait for it
+        torch.cuda.synchronize(st.device)
     bits = 0
-    for v in st.cpu().tolist():  # one word per blob of the latest call: OR them
+    for v in st[:words].cpu().tolist():  # one word per blob of the latest call: OR them
         bits |= int(v)
     return bits
 

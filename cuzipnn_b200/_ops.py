@@ -175,7 +175,7 @@ class _Linear(torch.autograd.Function):
         status = torch.empty(2, dtype=torch.int32, device=w.device)  # of this pass, and of the backward pass
         want = act != 0 and (ctx.needs_input_grad[0] or ctx.needs_input_grad[2])
         y, slope = _linear_forward(w, x, shape, bias, act, residual, want, status)
-        _set_status(w.device, (status, 1))
+        _set_status(w.device, status, 1)
         ctx.w, ctx.status, ctx.statuses, ctx.x_shape = w, status, _statuses(), x.shape
         ctx.save_for_backward(blob, slope)  # the blob: an in-place change before backward raises
         return y
@@ -198,7 +198,7 @@ class _Linear(torch.autograd.Function):
                        (g.data_ptr(), ldy, g.shape[0], _ptr(slope), _ptr(dx), _ptr(db)),
                        ctx.status.data_ptr() + 4)
                 if need_x:  # it decoded; the engine's thread reports to the one that called the layer
-                    ctx.statuses[w.device.index] = (ctx.status, 2)
+                    ctx.statuses[w.device.index] = (ctx.status, 2, _stream(w.device))
         return dx, None, db, dy if need_r else None, None, None, None
 
 

@@ -53,3 +53,26 @@ def test_status_of_the_forward_pass_stays():
     y.sum().backward()
     assert z.last_decode_status() != 0
     assert z.blob_linear(x, blob).shape == (30, 64) and z.last_decode_status() == 0
+
+
+def test_status_read_on_another_stream():
+    """The calls run on a side stream behind 50 ms of other work; the status is read from the default
+    stream, which waits for them."""
+    w, blob = weight(64, 256, BF, chunk=4096)
+    bad, x = damaged(blob), rnd(30, 256)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    calls = (lambda b: z.blob_linear(x, b), lambda b: z.blob_linear(x[:1], b), lambda b: z.decompress_tensor(b),
+             lambda b: z.decompress_tensors([b, blob]),
+             lambda b: z.blob_linear(x.clone().requires_grad_(), b).sum().backward())
+    for call in calls:
+        with torch.cuda.stream(side):
+            call(blob)
+            side.synchronize()
+            torch.cuda._sleep(100_000_000)
+            call(bad)
+        assert z.last_decode_status() != 0
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(100_000_000)
+            call(blob)
+        assert z.last_decode_status() == 0
