@@ -441,8 +441,8 @@ def _parse_header(prefix: Buffer, off: int = 0, length: int | None = None
 
 
 # Status words of the calling thread's latest decompress call per device (0 = no decoding error): a
-# tensor, how many of its words are set (None: all), and the stream they are set on.  Per thread, so that threads decoding on one device do not overwrite each
-# other's status.
+# tensor, how many of its words are set (None: all), and the stream they are set on.  Per thread, so that
+# threads decoding on one device do not overwrite each other's status.
 _STATUS = threading.local()
 
 
