@@ -50,3 +50,42 @@ def test_single_token_at_the_end_of_its_memory():
     pool = torch.empty(64 << 20, dtype=BF, device=DEV)
     x = pool[-512:].view(1, 512).copy_(rnd(1, 512))
     check_linear(x, w, blob)
+
+
+@pytest.mark.parametrize("tokens", [1, 30])
+def test_captured_calls_without_gradients(tokens):
+    """One graph of a layer and both losses, replayed on other inputs and beside another graph of the
+    same calls on a second stream."""
+    w, blob = weight(5000, 256, BF, chunk=4096)
+    gen = torch.Generator(device=DEV).manual_seed(4)
+
+    def inputs():
+        return (torch.randn((tokens, 256), generator=gen, device=DEV).to(BF),
+                torch.randint(5000, (tokens,), generator=gen, device=DEV),
+                torch.randint(5000, (tokens, 7), generator=gen, device=DEV),
+                torch.randn((tokens, 7), generator=gen, device=DEV))
+
+    def step(x, t, ids, logits):
+        return [z.blob_linear(x, blob, activation="gelu"), z.blob_cross_entropy(x, blob, t),
+                z.blob_distillation(x, blob, logits, ids, temperature=2.0, reduction="none")]
+
+    sets = [inputs() for _ in range(3)]
+    want = [step(*s) for s in sets]
+    graphs = []
+    for _ in range(2):
+        held = [v.clone() for v in sets[0]]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step(*held)
+        graphs.append((graph, held, out, torch.cuda.Stream()))
+    for i in (1, 2, 0, 1):
+        torch.cuda.synchronize()
+        for j, (graph, held, out, stream) in enumerate(graphs):  # both at once, on different inputs
+            with torch.cuda.stream(stream):
+                for a, b in zip(held, sets[(i + j) % 3]):
+                    a.copy_(b)
+                graph.replay()
+        torch.cuda.synchronize()
+        for j, (_, _, out, _) in enumerate(graphs):
+            for a, b in zip(out, want[(i + j) % 3]):
+                assert torch.equal(a, b)
